@@ -6,7 +6,7 @@
 * ``libcerebro_da.so``  — the C++ Direct-Access reader / pglz codec
   (``csrc/da/*.cpp``), host-only.
 
-Objects are cached by source/header mtime; ``python -m
+Objects are cached by the mtime of source, headers and this file (its flags); ``python -m
 cerebro_ds_kpgi_amd.tools.build`` rebuilds what changed.
 """
 
@@ -22,7 +22,10 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = os.environ.get("PYTORCH_ROCM_ARCH", "gfx950")
 
 HIP_FLAGS = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=" + ARCH, "-munsafe-fp-atomics",
-             "-Wno-unused-result"]
+             "-Wno-unused-result",
+             # no packed fp32 arithmetic (v_pk_add / mul / fma_f32): some of its
+             # forms gave wrong results on gfx950 without an error
+             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 CXX_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-pthread", "-Wall", "-Wno-unused-function"]
 
 
@@ -30,7 +33,7 @@ def _newer(src, obj, headers):
     if not os.path.exists(obj):
         return True
     t = os.path.getmtime(obj)
-    return any(os.path.getmtime(f) > t for f in [src] + headers)
+    return any(os.path.getmtime(f) > t for f in [src, os.path.abspath(__file__)] + headers)
 
 
 def _run(cmd):
