@@ -1636,3 +1636,75 @@ def embbag_bwd(dy, idx, y, wref, bref, relu):
     rc = _fn("cer_embbag_bwd", dy)(_ptr(_act(dy)), _ptr(y), _ptr(idx.contiguous()), G, B, nnz,
                               c_p(gp), gs, c_p(bp), bs, N, 1 if relu else 0, _stream())
     _check(rc, "cer_embbag_bwd")
+
+
+# ---------------------------------------------------------------------------
+# packed dense layer with bias, activation and residual (csrc/hip/dense.hip)
+# ---------------------------------------------------------------------------
+_SIGS.update({
+    "cer_dense_ws": [c_i, c_i, c_i, c_i, c_i, c_i, c_i],
+    "cer_dense_fwd": [c_p, c_i64, c_p, c_i64, c_p, c_i64, c_p, c_i64, c_p, c_p, c_i, c_i, c_i,
+                      c_i, c_i, c_p, c_i64, c_p],
+    "cer_dense_bwd": [c_p, c_p, c_p, c_p, c_i64, c_p, c_i64, c_p, c_p, c_i64, c_p, c_i64, c_i,
+                      c_i, c_i, c_i, c_i, c_p, c_i64, c_p],
+})
+_RET_I64 |= {"cer_dense_ws"}
+IMPLEMENTED |= {"linear_act"}
+
+
+def _on(t):
+    """Launches inside go to ``t``'s device (and that device's current stream)."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _dense_ws(kind, M, N, K, G, x, act):
+    n = lib().cer_dense_ws(kind, M, N, K, G, int(x.dtype == torch.bfloat16), act)
+    if n < 0:
+        raise ValueError("linear_act: M={} N={} K={} G={} is beyond the kernels' 32-bit tile "
+                         "offsets".format(M, N, K, G))
+    ws = torch.empty(n, dtype=torch.float32, device=x.device) if n else None
+    return ws, n
+
+
+def linear_act_fwd(x, wref, bref, act, residual, train):
+    """x [M, G*K] (rows may be pitched) -> (y [M, G*N], act'(z) or None)."""
+    with _on(x):
+        M, G = x.shape[0], wref.G
+        N, K = wref.spec.shape
+        y = torch.empty((M, G * N), dtype=x.dtype, device=x.device)
+        d = None
+        if train and act:
+            d = torch.empty((M, G * N), dtype=torch.float32 if act > 6 else torch.uint8,
+                            device=x.device)
+        ws, n = _dense_ws(0, M, N, K, G, x, act)
+        wp, wst = wref.work_ptr()
+        bp, bst = bref.work_ptr() if bref is not None else (0, 0)
+        rc = _fn("cer_dense_fwd", x)(
+            _ptr(x), x.stride(0), c_p(wp), wst, c_p(bp), bst, _ptr(residual),
+            residual.stride(0) if residual is not None else 0, _ptr(y), _ptr(d), M, N, K, G, act,
+            _ptr(ws), n, _stream())
+        _check(rc, "cer_dense_fwd")
+    return y, d
+
+
+def linear_act_bwd(dy, d, x, wref, bref, act, need_dx):
+    """dx (or None); the weight and bias gradients go to the arena."""
+    with _on(x):
+        M, G = x.shape[0], wref.G
+        N, K = wref.spec.shape
+        dx = torch.empty((M, G * K), dtype=x.dtype, device=x.device) if need_dx else None
+        dz = None
+        if act:
+            dz = torch.empty((M, G * N), dtype=torch.float32 if act > 6 else x.dtype,
+                             device=x.device)
+        ws, n = _dense_ws(1, M, N, K, G, x, act)
+        wp, wst = wref.work_ptr()
+        gp, gst = wref.grad_ptr()
+        bp, bst = bref.grad_ptr() if bref is not None else (0, 0)
+        rc = _fn("cer_dense_bwd", x)(
+            _ptr(dy), _ptr(d), _ptr(dz), _ptr(x), x.stride(0), c_p(wp), wst, _ptr(dx), c_p(gp), gst,
+            c_p(bp), bst, M, N, K, G, act, _ptr(ws), n, _stream())
+        _check(rc, "cer_dense_bwd")
+    return dx

@@ -17,6 +17,7 @@ Each op dispatches to our HIP kernel (``ops._hip``) or to the PyTorch oracle
 implementation in this file (``ops.backend``).
 """
 
+import math
 import os
 
 import torch
@@ -733,6 +734,145 @@ class PackedLinear(torch.autograd.Function):
 
 def linear(x, wref, bref=None, relu=False, anchor=None):
     return PackedLinear.apply(x, anchor, wref, bref, relu)
+
+
+# ---------------------------------------------------------------------------
+# grouped linear + bias + activation + residual
+# ---------------------------------------------------------------------------
+
+# activation names -> codes (csrc/hip/dense.hip); relu / relu6 as everywhere here
+LINEAR_ACTS = {"none": 0, "relu": 1, "relu6": 6, "gelu": 7, "gelu_tanh": 8, "silu": 9}
+
+
+def _act_and_grad(z, code):
+    """act(z), act'(z) of an fp32 tensor."""
+    if code in (0, 1, 6):
+        return _act(z, code), _act_grad(torch.ones_like(z), _act(z, code), code)
+    if code == 7:
+        cdf = 0.5 * (1.0 + torch.erf(z * math.sqrt(0.5)))
+        return z * cdf, cdf + z * torch.exp(-0.5 * z * z) / math.sqrt(2.0 * math.pi)
+    if code == 8:
+        c = math.sqrt(2.0 / math.pi)
+        t = torch.tanh(c * (z + 0.044715 * z ** 3))
+        return (0.5 * z * (1.0 + t),
+                0.5 * (1.0 + t) + 0.5 * z * (1.0 - t * t) * c * (1.0 + 0.134145 * z * z))
+    s = torch.sigmoid(z)
+    return z * s, s * (1.0 + z * (1.0 - s))
+
+
+class PackedLinearAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, anchor, residual, wref, bref, act, train):
+        ctx.wref, ctx.bref, ctx.act, ctx.shape = wref, bref, act, x.shape
+        G = wref.G
+        N, K = wref.spec.shape
+        lead = x.shape[:-1]
+        x2 = _rows(x, G * K)
+        r2 = _rows(residual, G * N) if residual is not None else None
+        M = x2.shape[0]
+        ctx.hip = use_hip("linear_act", x)
+        if M == 0:
+            y, d = x2.new_empty(0, G * N), None
+        elif ctx.hip:
+            y, d = _hip().linear_act_fwd(x2, wref, bref, act, r2, train)
+        else:
+            z = torch.bmm(x2.reshape(M, G, K).transpose(0, 1).float(),
+                          wref.work().float().transpose(1, 2))              # [G, M, N]
+            if bref is not None:
+                z = z + bref.work().float().unsqueeze(1)
+            y, d = _act_and_grad(z, act)
+            y = y.transpose(0, 1).reshape(M, G * N)
+            if r2 is not None:
+                y = y + r2.float()
+            y = y.to(x.dtype)
+        if train:
+            ctx.save_for_backward(x2, d)
+        return y.view(*lead, G * N)
+
+    @staticmethod
+    def backward(ctx, dy):
+        x2, d = ctx.saved_tensors
+        wref, bref = ctx.wref, ctx.bref
+        G = wref.G
+        N, K = wref.spec.shape
+        M = x2.shape[0]
+        need_dx, _, need_dr = ctx.needs_input_grad[:3]
+        dr = dy if need_dr else None
+        if M == 0:
+            wref.grad().zero_()
+            if bref is not None:
+                bref.grad().zero_()
+            return dy.new_empty(ctx.shape) if need_dx else None, None, dr, None, None, None, None
+        dy2 = dy.contiguous().view(M, G * N)
+        if ctx.hip:
+            dx = _hip().linear_act_bwd(dy2, d, x2, wref, bref, ctx.act, need_dx)
+        else:
+            dz = dy2.view(M, G, N).transpose(0, 1).float() * d              # [G, M, N]
+            xg = x2.reshape(M, G, K).transpose(0, 1).float()                # [G, M, K]
+            wref.grad().copy_(torch.bmm(dz.transpose(1, 2), xg))
+            if bref is not None:
+                bref.grad().copy_(dz.sum(1))
+            dx = None
+            if need_dx:
+                dx = torch.bmm(dz, wref.work().float())
+                dx = dx.transpose(0, 1).reshape(M, G * K).to(x2.dtype)
+        return dx.view(ctx.shape) if need_dx else None, None, dr, None, None, None, None
+
+
+def _rows(t, width):
+    """``t`` as [rows, width] with neighbouring elements of a row adjacent;
+    a row pitch is kept, any other layout is copied."""
+    if getattr(t, "_cer_hl", False):
+        t = _hip().hl_to_fp32(t)
+    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= width:
+        return t
+    return t.contiguous().view(-1, width)
+
+
+def linear_act(x, wref, bref=None, act="none", residual=None, anchor=None):
+    """y = residual + act(x W^T + b), config by config, in one GEMM.
+
+    ``x [..., G*K]`` and ``residual [..., G*N]`` in the arena's compute dtype
+    (fp32 or bf16), any number of rows, ``wref`` a ``[N, K]`` and ``bref`` a
+    ``[N]`` parameter of the same arena; ``act`` one of ``LINEAR_ACTS`` (gelu
+    is the erf form).  Differentiable in ``x`` and ``residual``; with either of
+    them, or ``anchor``, requiring a gradient the backward writes the weight and
+    bias gradients into the arena as every op of this module does -- it writes,
+    it does not add, so a parameter is used once per step.  Rounding: fp32
+    products run on the two-plane split (16 significand bits per factor, fp32
+    sums), bf16 products are exact with fp32 sums, and every output is rounded
+    once; act'(z) is kept in fp32 between the passes.
+    """
+    if act not in LINEAR_ACTS:
+        raise ValueError("linear_act: act {!r} is not one of {}".format(act, sorted(LINEAR_ACTS)))
+    arena = wref.arena
+    if len(wref.spec.shape) != 2:
+        raise ValueError("linear_act: weight {} is not [N, K]".format(wref.spec.shape))
+    N, K = wref.spec.shape
+    G = wref.G
+    if x.dtype != arena.compute_dtype or x.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError("linear_act: x is {}, the arena computes in {} (fp32 and bf16 are "
+                        "supported)".format(x.dtype, arena.compute_dtype))
+    if x.dim() < 1 or x.shape[-1] != G * K:
+        raise ValueError("linear_act: x {} does not end in G*K = {}".format(tuple(x.shape), G * K))
+    if bref is not None and (bref.arena is not arena or tuple(bref.spec.shape) != (N,)):
+        raise ValueError("linear_act: the bias must be an [{}] parameter of the weight's arena"
+                         .format(N))
+    if x.device != arena.state.device:
+        raise ValueError("linear_act: x is on {}, the arena on {}".format(x.device,
+                                                                          arena.state.device))
+    if residual is not None:
+        if tuple(residual.shape) != tuple(x.shape[:-1]) + (G * N,):
+            raise ValueError("linear_act: residual {} is not {}".format(
+                tuple(residual.shape), tuple(x.shape[:-1]) + (G * N,)))
+        if residual.dtype != x.dtype or residual.device != x.device:
+            raise TypeError("linear_act: residual is {} on {}, x is {} on {}".format(
+                residual.dtype, residual.device, x.dtype, x.device))
+    train = torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in (x, anchor, residual))
+    if train and arena.grad is None:
+        raise ValueError("linear_act: this arena holds no gradients (trainable=False)")
+    return PackedLinearAct.apply(x, anchor, residual, wref, bref, LINEAR_ACTS[act], train)
 
 
 # ---------------------------------------------------------------------------

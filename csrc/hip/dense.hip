@@ -1,0 +1,839 @@
+// Packed dense layer with bias, activation and residual in the epilogue
+// (ops.nn.linear_act), forward and backward.
+//
+//   z = x_g W_g^T + b_g,   y_g = r_g + act(z)              (forward, NT)
+//   dz = dy * act'(z),  dx = dz W,  dW = dz^T x,  db = sum_m dz
+//
+// Three GEMMs from one kernel template.  They differ in which operands are
+// stored with the reduction axis contiguous:
+//
+//   forward  A = x  [M][K] k-contiguous   B = W  [N][K] k-contiguous
+//   dgrad    A = dz [M][N] k-contiguous   B = W  [N][K] k-strided (k = N)
+//   wgrad    A = dz [M][N] k-strided      B = x  [M][K] k-strided (k = M)
+//
+// Operands are staged global -> registers -> LDS.  A k-strided operand is
+// transposed on the way: a thread loads 8 k-rows of V neighbouring columns and
+// writes V chunks of 8 consecutive k, so the LDS image, the fragments and the
+// MFMA loop are the same for all three.
+//
+// Precision.  A bf16 operand is one plane; its products are exact in the fp32
+// accumulators of v_mfma_f32_16x16x32_bf16.  An fp32 operand is split when it
+// is staged into two bf16 planes, hi = RNE(x) and lo = RNE(x - hi), 16 bits of
+// the significand, and the product runs as lo*hi + hi*lo + hi*hi: the dropped
+// part (lo*lo and the rounding of lo) is at most 3 * 2^-18 of |x||w| per term.
+// That is the framework's fp32 mode (conv.hip), at 3/16 of the cost of fp32
+// MFMA.  In bf16 mode dz = dy * act'(z) has more than 8 bits: it is kept in
+// fp32, enters dW as two planes (dW is an fp32 tensor) and dx as one (dx is
+// rounded to bf16 anyway).  A non-finite fp32 factor gives a non-finite
+// result, NaN where a single fp32 product would give an infinity.
+#include "common.h"
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+// element-aligned vectors: odd row lengths keep wide loads (gfx950 takes any
+// element alignment for global accesses)
+typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t u32_a2 __attribute__((aligned(2)));
+typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef float f32x2_a4 __attribute__((ext_vector_type(2), aligned(4)));
+typedef uint32_t u32_a1 __attribute__((aligned(1)));
+
+enum { ACT_NONE = 0, ACT_RELU = 1, ACT_RELU6 = 6, ACT_GELU = 7, ACT_GELU_TANH = 8, ACT_SILU = 9 };
+enum { EPI_FWD = 0, EPI_T = 1, EPI_F32 = 2 };
+
+static inline bool act_known(int a) {
+  return a == ACT_NONE || a == ACT_RELU || a == ACT_RELU6 || (a >= ACT_GELU && a <= ACT_SILU);
+}
+__host__ __device__ static inline bool act_smooth(int a) { return a >= ACT_GELU; }
+
+// act(z), and act'(z) in d.  NaN passes through every branch (comparisons with
+// NaN are false), unlike fmaxf.
+__device__ __forceinline__ float act_fwd(float z, int act, float& d) {
+  if (act == ACT_NONE) {
+    d = 1.f;
+    return z;
+  }
+  if (act == ACT_RELU) {
+    d = z > 0.f ? 1.f : 0.f;
+    return z <= 0.f ? 0.f : z;
+  }
+  if (act == ACT_RELU6) {
+    d = (z > 0.f && z < 6.f) ? 1.f : 0.f;
+    return z <= 0.f ? 0.f : (z >= 6.f ? 6.f : z);
+  }
+  if (act == ACT_GELU) {
+    // Phi(z) by Abramowitz & Stegun 7.1.26 (|error of erf| <= 1.5e-7), whose
+    // exp(-z^2/2) is also the density that act' needs: one exponential and one
+    // reciprocal for both
+    const float x = fabsf(z) * 0.70710678118654752f;
+    const float e = __expf(-x * x);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
+    float p = fmaf(t, 1.061405429f, -1.453152027f);
+    p = fmaf(t, p, 1.421413741f);
+    p = fmaf(t, p, -0.284496736f);
+    p = fmaf(t, p, 0.254829592f);
+    const float tail = 0.5f * p * t * e;              // Phi(-|z|)
+    const float cdf = z < 0.f ? tail : 1.f - tail;
+    d = fmaf(z, e * 0.39894228040143268f, cdf);
+    // beyond the float range of exp the limits, not inf * 0
+    if (fabsf(z) > 1e4f) {
+      d = z < 0.f ? 0.f : 1.f;
+      return z < 0.f ? 0.f : z;
+    }
+    return z * cdf;
+  }
+  if (act == ACT_GELU_TANH) {
+    const float c = 0.79788456080286536f;
+    const float u = c * z * fmaf(0.044715f * z, z, 1.f);
+    // tanh(u) = 1 - 2 / (exp(2u) + 1); exp overflows to inf -> 1, 0 -> -1
+    const float q = __builtin_amdgcn_rcpf(__expf(2.f * u) + 1.f);   // (1 - tanh u) / 2
+    const float s = 1.f - q;                                        // (1 + tanh u) / 2
+    if (fabsf(z) > 1e4f) {
+      d = z < 0.f ? 0.f : 1.f;
+      return z < 0.f ? 0.f : z;
+    }
+    d = fmaf(2.f * z * s * q, c * fmaf(0.134145f * z, z, 1.f), s);
+    return z * s;
+  }
+  // silu
+  const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z));
+  if (z < -1e4f) {
+    d = 0.f;
+    return 0.f;
+  }
+  if (z > 1e4f) {
+    d = 1.f;
+    return z;
+  }
+  d = s * fmaf(z, 1.f - s, 1.f);
+  return z * s;
+}
+
+struct GemmP {
+  const void* a;        // A + g * a_gs, leading dimension lda (elements)
+  const void* b;
+  int64_t lda, ldb, a_gs, b_gs;
+  int m, n, k, G;
+  void* c;              // out + g * c_gs + row * ldc + col
+  int64_t ldc, c_gs;
+  const void* bias;     // EPI_FWD: + g * bias_gs + col (or null)
+  int64_t bias_gs;
+  const void* res;      // EPI_FWD: residual (or null), config stride = c_gs
+  int64_t ldr;
+  void* d;              // EPI_FWD: act'(z) out (or null): fp32, or u8 for relu / relu6
+  int act;
+  float* part;          // split-K partials [split][g][m][n] (splits > 1)
+  int splits, steps;    // k steps per split
+  int tm, tn;           // tiles
+};
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(bf16_t v) { return bf2f(v); }
+
+// 4 consecutive outputs of one row, the last `nv` < 4 of a ragged edge
+template <typename T>
+__device__ __forceinline__ void st4(T* p, const float* v, int nv) {
+  if (nv >= 4) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<f32x4_a4*>(p) = f32x4_a4{v[0], v[1], v[2], v[3]};
+    } else {
+      *reinterpret_cast<u32x2_a2*>(p) = u32x2_a2{cvt_pk_bf16(v[0], v[1]), cvt_pk_bf16(v[2], v[3])};
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      if (i < nv) st1(p + i, v[i]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void ld4(const T* p, float* v, int nv) {
+  if (nv >= 4) {
+    if constexpr (sizeof(T) == 4) {
+      const f32x4_a4 u = *reinterpret_cast<const f32x4_a4*>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = u[i];
+    } else {
+      const u32x2_a2 u = *reinterpret_cast<const u32x2_a2*>(p);
+      v[0] = __uint_as_float(u.x << 16);
+      v[1] = __uint_as_float(u.x & 0xffff0000u);
+      v[2] = __uint_as_float(u.y << 16);
+      v[3] = __uint_as_float(u.y & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < nv ? ld1(p + i) : 0.f;
+  }
+}
+
+// finished sums of row `row`, columns col .. col + 3 of config g
+template <int EPI, typename T>
+__device__ __forceinline__ void epilogue(const GemmP& P, int g, int row, int col, float* z) {
+  const int nv = P.n - col;
+  const int64_t o = (int64_t)g * P.c_gs + (int64_t)row * P.ldc + col;
+  if constexpr (EPI == EPI_FWD) {
+    if (P.bias) {
+      float b[4];
+      ld4(reinterpret_cast<const T*>(P.bias) + g * P.bias_gs + col, b, nv);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) z[i] += b[i];
+    }
+    float d[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) z[i] = act_fwd(z[i], P.act, d[i]);
+    if (P.d) {
+      if (act_smooth(P.act)) {
+        st4(reinterpret_cast<float*>(P.d) + o, d, nv);
+      } else {
+        uint8_t* p = reinterpret_cast<uint8_t*>(P.d) + o;
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w |= (d[i] != 0.f ? 1u : 0u) << (8 * i);
+        if (nv >= 4) {
+          *reinterpret_cast<u32_a1*>(p) = w;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 3; ++i)
+            if (i < nv) p[i] = (uint8_t)(w >> (8 * i));
+        }
+      }
+    }
+    if (P.res) {
+      float r[4];
+      ld4(reinterpret_cast<const T*>(P.res) + g * P.c_gs + (int64_t)row * P.ldr + col, r, nv);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) z[i] += r[i];
+    }
+    st4(reinterpret_cast<T*>(P.c) + o, z, nv);
+  } else if constexpr (EPI == EPI_T) {
+    st4(reinterpret_cast<T*>(P.c) + o, z, nv);
+  } else {
+    st4(reinterpret_cast<float*>(P.c) + o, z, nv);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// operand staging: rows R x BK of one operand per step, T threads; every
+// thread moves V = R * BK / (8 T) chunks of 8 k
+// ---------------------------------------------------------------------------
+template <int BK>
+__device__ __forceinline__ int lds_off(int row, int chunk) {
+  // 16-B chunks of a row are XOR-swizzled so that neither 8 neighbouring rows
+  // (fragment reads) nor 8 rows V apart (transposing writes) share a bank
+  if constexpr (BK == 64) return row * 128 + ((chunk ^ ((row ^ (row >> 3)) & 7)) << 4);
+  else return row * 64 + ((chunk ^ (((row >> 1) ^ (row >> 3)) & 3)) << 4);
+}
+
+template <typename S, bool KS, int R, int BK, int T, int PL>
+struct Stage {
+  static constexpr int V = R * BK / (8 * T);
+  static_assert(V >= 1 && V * 8 * T == R * BK, "one unit per thread");
+  static constexpr int CH = BK / 8;
+  static constexpr bool F32 = sizeof(S) == 4;
+  static constexpr int NR = F32 ? 8 * V : (KS ? 8 * (V > 1 ? V / 2 : 1) : 4 * V);
+  static constexpr int BYTES = PL * R * BK * 2;
+  uint32_t r[NR];
+  uint32_t off[KS ? 1 : V];   // byte offsets inside a step's tile
+  const char* base;           // uniform: tile origin
+  int64_t step_bytes;         // uniform: bytes from one step to the next
+  uint32_t ldb;               // row pitch in bytes
+  int row0, rows, kc;         // tile origin, operand extent; this thread's k chunk
+  bool colfull;
+
+  __device__ __forceinline__ void init(const void* src, int64_t ld, int r0, int nrows, int tid) {
+    rows = nrows;
+    row0 = r0;
+    ldb = (uint32_t)(ld * sizeof(S));
+    if constexpr (KS) {
+      base = reinterpret_cast<const char*>(src) + (int64_t)r0 * sizeof(S);
+      step_bytes = (int64_t)BK * ld * sizeof(S);
+      kc = tid / (R / V);
+      int c = (tid % (R / V)) * V;
+      colfull = r0 + R <= nrows || nrows % V == 0;
+      if (colfull && r0 + c + V > nrows) c = nrows - V - r0;   // wholly outside: any columns
+      off[0] = (uint32_t)(kc * 8) * ldb + (uint32_t)(c * (int)sizeof(S));
+    } else {
+      base = reinterpret_cast<const char*>(src) + (int64_t)r0 * ld * sizeof(S);
+      step_bytes = (int64_t)BK * sizeof(S);
+      kc = tid % CH;
+      colfull = true;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        int row = tid / CH + i * (T / CH);
+        if (r0 + row >= nrows) row = nrows - 1 - r0;           // discarded rows: any row
+        off[i] = (uint32_t)row * ldb + (uint32_t)(kc * 8 * (int)sizeof(S));
+      }
+    }
+  }
+
+  __device__ __forceinline__ void load_full(int step) {
+    const char* p = base + step * step_bytes;
+    if constexpr (!KS) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if constexpr (F32) {
+          const f32x4_a4 a = *reinterpret_cast<const f32x4_a4*>(p + off[i]);
+          const f32x4_a4 b = *reinterpret_cast<const f32x4_a4*>(p + off[i] + 16);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            r[8 * i + e] = __float_as_uint(a[e]);
+            r[8 * i + 4 + e] = __float_as_uint(b[e]);
+          }
+        } else {
+          const u32x4_a2 a = *reinterpret_cast<const u32x4_a2*>(p + off[i]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) r[4 * i + e] = a[e];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const char* q = p + (uint64_t)e * ldb + off[0];
+        if constexpr (F32) {
+          if constexpr (V == 1) {
+            r[e] = *reinterpret_cast<const uint32_t*>(q);
+          } else if constexpr (V == 2) {
+            const f32x2_a4 a = *reinterpret_cast<const f32x2_a4*>(q);
+            r[2 * e] = __float_as_uint(a.x);
+            r[2 * e + 1] = __float_as_uint(a.y);
+          } else {
+            const f32x4_a4 a = *reinterpret_cast<const f32x4_a4*>(q);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) r[4 * e + v] = __float_as_uint(a[v]);
+          }
+        } else {
+          if constexpr (V == 1) {
+            r[e] = *reinterpret_cast<const bf16_t*>(q);
+          } else if constexpr (V == 2) {
+            r[e] = *reinterpret_cast<const u32_a2*>(q);
+          } else {
+            const u32x2_a2 a = *reinterpret_cast<const u32x2_a2*>(q);
+            r[2 * e] = a.x;
+            r[2 * e + 1] = a.y;
+          }
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ uint32_t elem(const char* p) const {
+    if constexpr (F32) return *reinterpret_cast<const uint32_t*>(p);
+    else return *reinterpret_cast<const bf16_t*>(p);
+  }
+
+  // a step that reaches past the operand: elements outside are zero
+  __device__ __forceinline__ void load_edge(int step, int kleft, int tid) {
+    const char* p = base + step * step_bytes;
+#pragma unroll
+    for (int i = 0; i < NR; ++i) r[i] = 0;
+    if constexpr (!KS) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          uint32_t v = 0;
+          if (kc * 8 + e < kleft) v = elem(p + off[i] + e * sizeof(S));
+          if constexpr (F32) r[8 * i + e] = v;
+          else r[4 * i + e / 2] |= v << (16 * (e & 1));
+        }
+      }
+    } else {
+      const int c = (tid % (R / V)) * V;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const char* q = p + (uint64_t)(kc * 8 + e) * ldb + c * (int)sizeof(S);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          uint32_t w = 0;
+          if (kc * 8 + e < kleft && row0 + c + v < rows) w = elem(q + v * sizeof(S));
+          if constexpr (F32) r[V * e + v] = w;
+          else if constexpr (V == 1) r[e] = w;
+          else r[(V / 2) * e + v / 2] |= w << (16 * (v & 1));
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void load(int step, int k, int tid) {
+    const int kleft = k - step * BK;
+    if (kleft >= BK && colfull) load_full(step);
+    else load_edge(step, kleft, tid);
+  }
+
+  // the 8 k of chunk i as PL bf16 planes into LDS
+  __device__ __forceinline__ void store(char* lds, int tid) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int row = KS ? (tid % (R / V)) * V + i : tid / CH + i * (T / CH);
+      const int o = lds_off<BK>(row, kc);
+      uint32_t h[4];
+      if constexpr (F32) {
+        uint32_t l[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float a = __uint_as_float(KS ? r[V * (2 * q) + i] : r[8 * i + 2 * q]);
+          const float b = __uint_as_float(KS ? r[V * (2 * q + 1) + i] : r[8 * i + 2 * q + 1]);
+          h[q] = cvt_pk_bf16(a, b);
+          if constexpr (PL == 2)
+            l[q] = cvt_pk_bf16(a - __uint_as_float(h[q] << 16),
+                               b - __uint_as_float(h[q] & 0xffff0000u));
+        }
+        if constexpr (PL == 2)
+          *reinterpret_cast<uint4*>(lds + R * BK * 2 + o) = make_uint4(l[0], l[1], l[2], l[3]);
+      } else if constexpr (KS) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if constexpr (V == 1) {
+            h[q] = r[2 * q] | (r[2 * q + 1] << 16);
+          } else {
+            const uint32_t a = r[(V / 2) * (2 * q) + i / 2], b = r[(V / 2) * (2 * q + 1) + i / 2];
+            h[q] = (i & 1) ? __builtin_amdgcn_perm(b, a, 0x07060302u)
+                           : __builtin_amdgcn_perm(b, a, 0x05040100u);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) h[q] = r[4 * i + q];
+      }
+      *reinterpret_cast<uint4*>(lds + o) = make_uint4(h[0], h[1], h[2], h[3]);
+    }
+  }
+};
+
+// ---------------------------------------------------------------------------
+// C tile BM x BN per block; WM x WN waves; LDS double buffered: the tile of
+// step t + 1 goes from registers to LDS and step t + 2 is requested while step
+// t is multiplied, one barrier per step
+// ---------------------------------------------------------------------------
+template <typename SA, typename SB, int PA, int PB, bool KA, bool KB, int BM, int BN, int BK,
+          int WM, int WN, int EPI, typename TO>
+__global__ __launch_bounds__(WM * WN * 64, 2) void dense_gemm(const GemmP P) {
+  constexpr int T = WM * WN * 64;
+  constexpr int IM = BM / WM / 16, JN = BN / WN / 16;
+  typedef Stage<SA, KA, BM, BK, T, PA> StA;
+  typedef Stage<SB, KB, BN, BK, T, PB> StB;
+  constexpr int BUF = StA::BYTES + StB::BYTES;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  // Blocks go to the 8 XCDs round robin: give each XCD a contiguous range of
+  // the work, so neighbouring tiles share its L2
+  const int nblk = gridDim.x;
+  int w = blockIdx.x;
+  {
+    const int per = nblk >> 3, cut = per << 3;
+    if (w < cut) w = (w & 7) * per + (w >> 3);
+  }
+  const int per_split = P.G * P.tm * P.tn;
+  const int split = w / per_split;
+  w -= split * per_split;
+  const int g = w / (P.tm * P.tn);
+  w -= g * P.tm * P.tn;
+  // bands of 4 tile rows: consecutive blocks reuse 4 A panels and one B panel
+  const int band = w / (4 * P.tn), in = w - band * 4 * P.tn;
+  const int bh = min(4, P.tm - band * 4);
+  const int tm = band * 4 + in % bh, tn = in / bh;
+  const int m0 = tm * BM, n0 = tn * BN;
+
+  StA sa;
+  StB sb;
+  sa.init(reinterpret_cast<const SA*>(P.a) + g * P.a_gs, P.lda, m0, P.m, tid);
+  sb.init(reinterpret_cast<const SB*>(P.b) + g * P.b_gs, P.ldb, n0, P.n, tid);
+
+  const int total = (P.k + BK - 1) / BK;
+  const int s0 = split * P.steps;
+  const int s1 = min(total, s0 + P.steps);
+
+  f32x4 acc[IM][JN];
+#pragma unroll
+  for (int i = 0; i < IM; ++i)
+#pragma unroll
+    for (int j = 0; j < JN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
+  const int fr = lane & 15, fc = lane >> 4;
+
+  if (s0 < s1) {
+    sa.load(s0, P.k, tid);
+    sb.load(s0, P.k, tid);
+    sa.store(smem, tid);
+    sb.store(smem + StA::BYTES, tid);
+    if (s0 + 1 < s1) {
+      sa.load(s0 + 1, P.k, tid);
+      sb.load(s0 + 1, P.k, tid);
+    }
+    __syncthreads();
+    for (int s = s0; s < s1; ++s) {
+      const char* cur = smem + ((s - s0) & 1) * BUF;
+      if (s + 1 < s1) {
+        char* nxt = smem + ((s + 1 - s0) & 1) * BUF;
+        sa.store(nxt, tid);
+        sb.store(nxt + StA::BYTES, tid);
+        if (s + 2 < s1) {
+          sa.load(s + 2, P.k, tid);
+          sb.load(s + 2, P.k, tid);
+        }
+      }
+#pragma unroll
+      for (int kk = 0; kk < BK / 32; ++kk) {
+        bf16x8 bf[JN][PB];
+#pragma unroll
+        for (int j = 0; j < JN; ++j)
+#pragma unroll
+          for (int p = 0; p < PB; ++p)
+            bf[j][p] = *reinterpret_cast<const bf16x8*>(
+                cur + StA::BYTES + p * (BN * BK * 2) +
+                lds_off<BK>(wn + j * 16 + fr, kk * 4 + fc));
+#pragma unroll
+        for (int i = 0; i < IM; ++i) {
+          bf16x8 af[PA];
+#pragma unroll
+          for (int p = 0; p < PA; ++p)
+            af[p] = *reinterpret_cast<const bf16x8*>(
+                cur + p * (BM * BK * 2) + lds_off<BK>(wm + i * 16 + fr, kk * 4 + fc));
+          // operands swapped: a lane ends with 4 neighbouring columns of a row
+#pragma unroll
+          for (int j = 0; j < JN; ++j) {
+            if constexpr (PA == 2)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[j][0], af[1], acc[i][j], 0, 0, 0);
+            if constexpr (PB == 2)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[j][1], af[0], acc[i][j], 0, 0, 0);
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[j][0], af[0], acc[i][j], 0, 0, 0);
+          }
+        }
+      }
+      __syncthreads();
+    }
+  }
+
+#pragma unroll
+  for (int i = 0; i < IM; ++i) {
+    const int row = m0 + wm + i * 16 + fr;
+    if (row >= P.m) continue;
+#pragma unroll
+    for (int j = 0; j < JN; ++j) {
+      const int col = n0 + wn + j * 16 + fc * 4;
+      if (col >= P.n) continue;
+      float z[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+      if (P.splits > 1) {
+        float* q = P.part + (((int64_t)split * P.G + g) * P.m + row) * P.n + col;
+        st4(q, z, P.n - col);
+      } else {
+        epilogue<EPI, TO>(P, g, row, col, z);
+      }
+    }
+  }
+}
+
+// sums the split-K partials in split order (the result does not depend on
+// which block finished first) and runs the epilogue
+template <int EPI, typename TO>
+__global__ __launch_bounds__(256) void dense_join(const GemmP P) {
+  const int nq = (P.n + 3) / 4;
+  const int64_t total = (int64_t)P.G * P.m * nq;
+  const int64_t slab = (int64_t)P.G * P.m * P.n;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * 256) {
+    const int64_t rr = i / nq;
+    const int col = (int)(i - rr * nq) * 4;
+    const int g = (int)(rr / P.m), row = (int)(rr - (int64_t)g * P.m);
+    const float* q = P.part + rr * P.n + col;
+    float z[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < P.splits; ++s, q += slab) {
+      float v[4];
+      ld4(q, v, P.n - col);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[e] += v[e];
+    }
+    epilogue<EPI, TO>(P, g, row, col, z);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// dz = dy * act'(z) and the column sums of dz (db).  Blocks own 64 columns x a
+// range of rows; the partial sums of several row ranges meet in dense_dbsum in
+// a fixed order.
+// ---------------------------------------------------------------------------
+constexpr int DA_COLS = 64, DA_ROWS = 128;
+
+// D: 0 none (dz is dy, only db is made), 1 u8 mask, 2 fp32 derivative
+template <typename T, int D, typename TZ>
+__global__ __launch_bounds__(256) void dense_dact(const T* __restrict__ dy, const void* __restrict__ d,
+                                                  TZ* __restrict__ dz, float* __restrict__ db,
+                                                  int64_t db_gs, float* __restrict__ part, int M,
+                                                  int C, int N) {
+  __shared__ float sm[4][DA_COLS];
+  const int c = blockIdx.x * DA_COLS + (threadIdx.x & 63), w = threadIdx.x >> 6;
+  const int r0 = blockIdx.y * DA_ROWS, r1 = min(M, r0 + DA_ROWS);
+  float s = 0.f;
+  if (c < C) {
+#pragma unroll 8
+    for (int r = r0 + w; r < r1; r += 4) {
+      const int64_t i = (int64_t)r * C + c;
+      float v = ld1(dy + i);
+      if constexpr (D == 1) v = reinterpret_cast<const uint8_t*>(d)[i] ? v : 0.f;
+      if constexpr (D == 2) v *= reinterpret_cast<const float*>(d)[i];
+      if constexpr (D != 0) st1(dz + i, v);
+      s += v;
+    }
+  }
+  if (!db) return;
+  sm[w][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (w == 0 && c < C) {
+    s = (sm[0][threadIdx.x] + sm[1][threadIdx.x]) + (sm[2][threadIdx.x] + sm[3][threadIdx.x]);
+    if (gridDim.y > 1) part[(int64_t)blockIdx.y * C + c] = s;
+    else db[(c / N) * db_gs + c % N] = s;
+  }
+}
+
+__global__ __launch_bounds__(256) void dense_dbsum(const float* __restrict__ part, int rows,
+                                                   float* __restrict__ db, int64_t db_gs, int C,
+                                                   int N) {
+  __shared__ float sm[4][DA_COLS];
+  const int c = blockIdx.x * DA_COLS + (threadIdx.x & 63), w = threadIdx.x >> 6;
+  float s = 0.f;
+  if (c < C)
+    for (int r = w; r < rows; r += 4) s += part[(int64_t)r * C + c];
+  sm[w][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (w == 0 && c < C)
+    db[(c / N) * db_gs + c % N] =
+        (sm[0][threadIdx.x] + sm[1][threadIdx.x]) + (sm[2][threadIdx.x] + sm[3][threadIdx.x]);
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+struct Plan {
+  int tile;      // 0: 256x256, 1: 128x128, 2: 64x64, 3: 32x64
+  int bm, bn, bk, tm, tn, splits, steps;
+};
+
+// planes: of both operands together (2: bf16, 3: one fp32, 4: both fp32)
+static Plan make_plan(int64_t m, int64_t n, int64_t k, int G, int planes) {
+  static const int BMs[4] = {256, 128, 64, 32}, BNs[4] = {256, 128, 64, 64};
+  Plan p;
+  auto tiles = [&](int t) {
+    return (int64_t)G * ((m + BMs[t] - 1) / BMs[t]) * ((n + BNs[t] - 1) / BNs[t]);
+  };
+  int t;
+  if (m <= 32) t = 3;
+  else if (planes == 2 && tiles(0) >= 192) t = 0;
+  else if (tiles(1) >= 192) t = 1;
+  else t = 2;
+  p.tile = t;
+  p.bm = BMs[t];
+  p.bn = BNs[t];
+  p.bk = (t == 1 && planes > 2) ? 32 : 64;
+  p.tm = (int)((m + p.bm - 1) / p.bm);
+  p.tn = (int)((n + p.bn - 1) / p.bn);
+  const int64_t total = (k + p.bk - 1) / p.bk;
+  const int64_t nt = tiles(t);
+  int64_t s = 1;
+  if (nt < 512) {
+    s = (768 + nt - 1) / nt;
+    if (s > total / 4) s = total / 4;
+    if (s > 32) s = 32;
+    if (s < 1) s = 1;
+  }
+  p.steps = (int)((total + s - 1) / s);
+  if (p.steps < 1) p.steps = 1;
+  p.splits = (int)((total + p.steps - 1) / p.steps);
+  if (p.splits < 1) p.splits = 1;
+  return p;
+}
+
+template <typename SA, typename SB, int PA, int PB, bool KA, bool KB, int BM, int BN, int BK, int WM,
+          int WN, int EPI, typename TO>
+static int launch_gemm(GemmP& P, const Plan& p, hipStream_t st) {
+  P.tm = p.tm;
+  P.tn = p.tn;
+  P.splits = p.splits;
+  P.steps = p.steps;
+  const int64_t blocks = (int64_t)P.G * p.tm * p.tn * p.splits;
+  if (blocks > 0x7fffffff) return (int)hipErrorInvalidValue;
+  constexpr int lds = 2 * (PA * BM + PB * BN) * BK * 2;
+  auto kern = dense_gemm<SA, SB, PA, PB, KA, KB, BM, BN, BK, WM, WN, EPI, TO>;
+  if (lds > 64 * 1024) {
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
+                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return (int)e;
+  }
+  kern<<<(int)blocks, WM * WN * 64, lds, st>>>(P);
+  if (p.splits > 1) {
+    const int64_t q = (int64_t)P.G * P.m * ((P.n + 3) / 4);
+    int64_t b = (q + 255) / 256;
+    if (b > 4096) b = 4096;
+    dense_join<EPI, TO><<<(int)b, 256, 0, st>>>(P);
+  }
+  return (int)hipGetLastError();
+}
+
+template <typename SA, typename SB, int PA, int PB, bool KA, bool KB, int EPI, typename TO>
+static int run_gemm(GemmP& P, const Plan& p, hipStream_t st) {
+  constexpr int BK1 = (PA + PB > 2) ? 32 : 64;
+  switch (p.tile) {
+    case 0:
+      if constexpr (PA + PB == 2)
+        return launch_gemm<SA, SB, PA, PB, KA, KB, 256, 256, 64, 2, 4, EPI, TO>(P, p, st);
+      else
+        return (int)hipErrorInvalidValue;
+    case 1: return launch_gemm<SA, SB, PA, PB, KA, KB, 128, 128, BK1, 2, 2, EPI, TO>(P, p, st);
+    case 2: return launch_gemm<SA, SB, PA, PB, KA, KB, 64, 64, 64, 2, 2, EPI, TO>(P, p, st);
+    default: return launch_gemm<SA, SB, PA, PB, KA, KB, 32, 64, 64, 1, 4, EPI, TO>(P, p, st);
+  }
+}
+
+static inline int planes_of(int kind, int is_bf16, int act) {
+  if (!is_bf16) return 4;
+  return kind == 2 && act_smooth(act) ? 3 : 2;
+}
+
+static inline Plan plan_of(int kind, int M, int N, int K, int G, int is_bf16, int act) {
+  const int pl = planes_of(kind, is_bf16, act);
+  if (kind == 0) return make_plan(M, N, K, G, pl);
+  if (kind == 1) return make_plan(M, K, N, G, pl);
+  return make_plan(N, K, M, G, pl);
+}
+
+static inline bool sizes_ok(int M, int N, int K, int G, int64_t ldx) {
+  // byte offsets inside a tile are 32-bit: 256 rows of the longest row
+  const int64_t most = ((int64_t)1 << 31) / (256 * 4);
+  return M > 0 && N > 0 && K > 0 && G > 0 && (int64_t)G * N < most && (int64_t)G * K < most &&
+         N < most && K < most && ldx >= (int64_t)G * K && ldx < most;
+}
+
+// fp32 workspace (floats) of a call: kind 0 forward, 1 backward; 0 for none,
+// -1 for sizes out of range
+CER_API int64_t cer_dense_ws(int kind, int M, int N, int K, int G, int is_bf16, int act) {
+  if (!sizes_ok(M, N, K, G, (int64_t)G * K) || !act_known(act)) return -1;
+  auto need = [&](int kd, int64_t m, int64_t n) {
+    const Plan p = plan_of(kd, M, N, K, G, is_bf16, act);
+    return p.splits > 1 ? (int64_t)p.splits * G * m * n : 0;
+  };
+  if (kind == 0) return need(0, M, N);
+  const int64_t a = need(1, M, K), b = need(2, N, K);
+  const int64_t nb = (M + DA_ROWS - 1) / DA_ROWS;
+  const int64_t c = nb > 1 ? nb * G * N : 0;
+  return a > b ? (a > c ? a : c) : (b > c ? b : c);
+}
+
+// y = r + act(x W^T + b).  x: row pitch ldx, config g at column g K; W, b: per-
+// config strides ws, bs (elements); r, y, d: [M][G N], r with row pitch ldr.
+// d (or null): act'(z), fp32 for the smooth activations, u8 for relu / relu6.
+template <typename T>
+static int dense_fwd(const T* x, int64_t ldx, const T* w, int64_t ws, const T* b, int64_t bs,
+                     const T* r, int64_t ldr, T* y, void* d, int M, int N, int K, int G, int act,
+                     float* part, int64_t part_floats, hipStream_t st) {
+  if (!sizes_ok(M, N, K, G, ldx) || !act_known(act) || !x || !w || !y)
+    return (int)hipErrorInvalidValue;
+  constexpr int is_bf16 = sizeof(T) == 2;
+  if (part_floats < cer_dense_ws(0, M, N, K, G, is_bf16, act)) return (int)hipErrorInvalidValue;
+  GemmP P = {};
+  P.a = x; P.lda = ldx; P.a_gs = K;
+  P.b = w; P.ldb = K; P.b_gs = ws;
+  P.m = M; P.n = N; P.k = K; P.G = G;
+  P.c = y; P.ldc = (int64_t)G * N; P.c_gs = N;
+  P.bias = b; P.bias_gs = bs;
+  P.res = r; P.ldr = ldr;
+  P.d = act == ACT_NONE ? nullptr : d;
+  P.act = act;
+  P.part = part;
+  const Plan p = plan_of(0, M, N, K, G, is_bf16, act);
+  constexpr int PL = is_bf16 ? 1 : 2;
+  return run_gemm<T, T, PL, PL, false, false, EPI_FWD, T>(P, p, st);
+}
+
+// gradients: dx (or null) [M][G K], dW -> gw (fp32, config stride gs),
+// db -> gb (or null).  d: act'(z) of the forward; dz: scratch [M][G N] (fp32
+// for the smooth activations, else T; unused for act none).
+template <typename T>
+static int dense_bwd(const T* dy, const void* d, void* dz, const T* x, int64_t ldx, const T* w,
+                     int64_t ws, T* dx, float* gw, int64_t gs, float* gb, int64_t gbs, int M, int N,
+                     int K, int G, int act, float* part, int64_t part_floats, hipStream_t st) {
+  if (!sizes_ok(M, N, K, G, ldx) || !act_known(act) || !dy || !x || !w || !gw)
+    return (int)hipErrorInvalidValue;
+  if (act != ACT_NONE && (!d || !dz)) return (int)hipErrorInvalidValue;
+  constexpr int is_bf16 = sizeof(T) == 2;
+  if (part_floats < cer_dense_ws(1, M, N, K, G, is_bf16, act)) return (int)hipErrorInvalidValue;
+  const int C = G * N;
+  const bool smooth = act_smooth(act);
+  if (act != ACT_NONE || gb) {
+    const dim3 grid((C + DA_COLS - 1) / DA_COLS, (M + DA_ROWS - 1) / DA_ROWS);
+    if (grid.y > 65535) return (int)hipErrorInvalidValue;
+    if (act == ACT_NONE)
+      dense_dact<T, 0, T><<<grid, 256, 0, st>>>(dy, nullptr, nullptr, gb, gbs, part, M, C, N);
+    else if (smooth)
+      dense_dact<T, 2, float><<<grid, 256, 0, st>>>(dy, d, (float*)dz, gb, gbs, part, M, C, N);
+    else
+      dense_dact<T, 1, T><<<grid, 256, 0, st>>>(dy, d, (T*)dz, gb, gbs, part, M, C, N);
+    if (gb && grid.y > 1)
+      dense_dbsum<<<grid.x, 256, 0, st>>>(part, grid.y, gb, gbs, C, N);
+  }
+  const void* z = act == ACT_NONE ? (const void*)dy : dz;
+  int rc;
+  {
+    GemmP P = {};
+    P.a = z; P.lda = C; P.a_gs = N;
+    P.b = x; P.ldb = ldx; P.b_gs = K;
+    P.m = N; P.n = K; P.k = M; P.G = G;
+    P.c = gw; P.ldc = K; P.c_gs = gs;
+    P.part = part;
+    const Plan p = plan_of(2, M, N, K, G, is_bf16, act);
+    if constexpr (!is_bf16)
+      rc = run_gemm<float, float, 2, 2, true, true, EPI_F32, float>(P, p, st);
+    else if (smooth)
+      rc = run_gemm<float, bf16_t, 2, 1, true, true, EPI_F32, float>(P, p, st);
+    else
+      rc = run_gemm<bf16_t, bf16_t, 1, 1, true, true, EPI_F32, float>(P, p, st);
+    if (rc) return rc;
+  }
+  if (!dx) return 0;
+  GemmP P = {};
+  P.a = z; P.lda = C; P.a_gs = N;
+  P.b = w; P.ldb = K; P.b_gs = ws;
+  P.m = M; P.n = K; P.k = N; P.G = G;
+  P.c = dx; P.ldc = (int64_t)G * K; P.c_gs = K;
+  P.part = part;
+  const Plan p = plan_of(1, M, N, K, G, is_bf16, act);
+  if constexpr (!is_bf16)
+    return run_gemm<float, float, 2, 2, false, true, EPI_T, float>(P, p, st);
+  else if (smooth)
+    return run_gemm<float, bf16_t, 1, 1, false, true, EPI_T, bf16_t>(P, p, st);
+  else
+    return run_gemm<bf16_t, bf16_t, 1, 1, false, true, EPI_T, bf16_t>(P, p, st);
+}
+
+CER_API int cer_dense_fwd(const bf16_t* x, int64_t ldx, const bf16_t* w, int64_t ws,
+                          const bf16_t* b, int64_t bs, const bf16_t* r, int64_t ldr, bf16_t* y,
+                          void* d, int M, int N, int K, int G, int act, float* part,
+                          int64_t part_floats, hipStream_t st) {
+  return dense_fwd<bf16_t>(x, ldx, w, ws, b, bs, r, ldr, y, d, M, N, K, G, act, part, part_floats,
+                           st);
+}
+
+CER_API int cer_dense_fwd_f32(const float* x, int64_t ldx, const float* w, int64_t ws,
+                              const float* b, int64_t bs, const float* r, int64_t ldr, float* y,
+                              void* d, int M, int N, int K, int G, int act, float* part,
+                              int64_t part_floats, hipStream_t st) {
+  return dense_fwd<float>(x, ldx, w, ws, b, bs, r, ldr, y, d, M, N, K, G, act, part, part_floats,
+                          st);
+}
+
+CER_API int cer_dense_bwd(const bf16_t* dy, const void* d, void* dz, const bf16_t* x, int64_t ldx,
+                          const bf16_t* w, int64_t ws, bf16_t* dx, float* gw, int64_t gs, float* gb,
+                          int64_t gbs, int M, int N, int K, int G, int act, float* part,
+                          int64_t part_floats, hipStream_t st) {
+  return dense_bwd<bf16_t>(dy, d, dz, x, ldx, w, ws, dx, gw, gs, gb, gbs, M, N, K, G, act, part,
+                           part_floats, st);
+}
+
+CER_API int cer_dense_bwd_f32(const float* dy, const void* d, void* dz, const float* x, int64_t ldx,
+                              const float* w, int64_t ws, float* dx, float* gw, int64_t gs,
+                              float* gb, int64_t gbs, int M, int N, int K, int G, int act,
+                              float* part, int64_t part_floats, hipStream_t st) {
+  return dense_bwd<float>(dy, d, dz, x, ldx, w, ws, dx, gw, gs, gb, gbs, M, N, K, G, act, part,
+                          part_floats, st);
+}

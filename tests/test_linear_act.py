@@ -1,0 +1,98 @@
+"""Refusals and the CPU path of ops.nn.linear_act (no GPU)."""
+
+import math
+
+import pytest
+import torch
+
+from cerebro_ds_kpgi_amd.ops import nn as P
+from cerebro_ds_kpgi_amd.runtime.arena import Arena, ModelLayout, ParamRef, ParamSpec
+
+F = torch.nn.functional
+ACT64 = {"none": lambda z: z, "relu": F.relu, "relu6": F.relu6, "gelu": F.gelu,
+         "gelu_tanh": lambda z: F.gelu(z, approximate="tanh"), "silu": F.silu}
+
+
+def make(G=2, N=3, K=5, dtype=torch.float32, bias=True, trainable=True, device="cpu"):
+    specs = [ParamSpec("d/kernel", (N, K), "weight")]
+    if bias:
+        specs.append(ParamSpec("d/bias", (N,), "bias"))
+    arena = Arena(ModelLayout(specs), G, device, dtype, trainable=trainable)
+    refs = [ParamRef(arena, s) for s in specs]
+    gen = torch.Generator().manual_seed(N * 1000 + K)
+    refs[0].master().copy_((torch.randn(G, N, K, generator=gen) / math.sqrt(K)).to(dtype))
+    if bias:
+        refs[1].master().copy_(torch.randn(G, N, generator=gen).to(dtype))
+    arena.sync_work()
+    return arena, refs[0], refs[1] if bias else None
+
+
+@pytest.mark.parametrize("act", sorted(ACT64))
+@pytest.mark.parametrize("residual", [False, True])
+def test_cpu_path_matches_64_bits(act, residual):
+    G, M, N, K = 2, 4, 3, 5
+    arena, w, b = make(G, N, K)
+    gen = torch.Generator().manual_seed(1)
+    x = torch.randn(2, M // 2, G * K, generator=gen, requires_grad=True)
+    r = torch.randn(2, M // 2, G * N, generator=gen, requires_grad=True) if residual else None
+    dy = torch.randn(2, M // 2, G * N, generator=gen)
+    y = P.linear_act(x, w, b, act, r)
+    y.backward(dy)
+    x64 = x.detach().double().requires_grad_(True)
+    w64 = w.work().double().requires_grad_(True)
+    b64 = b.work().double().requires_grad_(True)
+    z = torch.stack([F.linear(x64.view(M, G, K)[:, g], w64[g], b64[g]) for g in range(G)], 1)
+    y64 = ACT64[act](z).reshape(x.shape[:-1] + (G * N,))
+    if residual:
+        y64 = y64 + r.detach().double()
+    y64.backward(dy.double())
+    # sums of K = 5 and N = 3 terms of size ~1 in fp32
+    kw = dict(rtol=16 * 2 ** -24, atol=64 * 2 ** -24)
+    torch.testing.assert_close(y.detach().double(), y64.detach(), **kw)
+    torch.testing.assert_close(x.grad.double(), x64.grad, **kw)
+    torch.testing.assert_close(w.grad().double(), w64.grad, **kw)
+    torch.testing.assert_close(b.grad().double(), b64.grad, **kw)
+    if residual:
+        assert torch.equal(r.grad, dy)
+
+
+def test_cpu_bf16_and_empty():
+    arena, w, b = make(dtype=torch.bfloat16)
+    x = torch.randn(4, 10).bfloat16().requires_grad_(True)
+    y = P.linear_act(x, w, b, "silu")
+    assert y.dtype == torch.bfloat16 and y.shape == (4, 6)
+    y.sum().backward()
+    assert x.grad.dtype == torch.bfloat16 and w.grad().abs().sum() > 0
+    e = torch.zeros(0, 10, dtype=torch.bfloat16, requires_grad=True)
+    P.linear_act(e, w, b, "silu").sum().backward()
+    assert not w.grad().any() and not b.grad().any() and e.grad.shape == (0, 10)
+
+
+def test_refusals():
+    arena, w, b = make()
+    x = torch.zeros(4, 10)
+    with pytest.raises(ValueError, match="not one of"):
+        P.linear_act(x, w, b, "tanh")
+    with pytest.raises(ValueError, match="G\\*K"):
+        P.linear_act(torch.zeros(4, 9), w, b)
+    with pytest.raises(TypeError, match="computes in"):
+        P.linear_act(x.bfloat16(), w, b)
+    with pytest.raises(TypeError, match="computes in"):
+        P.linear_act(x.half(), w, b)
+    with pytest.raises(ValueError, match="residual"):
+        P.linear_act(x, w, b, "none", torch.zeros(3, 6))
+    with pytest.raises(ValueError, match="residual"):
+        P.linear_act(x, w, b, "none", torch.zeros(1, 6))
+    with pytest.raises(TypeError, match="residual"):
+        P.linear_act(x, w, b, "none", torch.zeros(4, 6).double())
+    with pytest.raises(ValueError, match="bias"):
+        P.linear_act(x, w, make()[2])
+    with pytest.raises(ValueError, match="bias"):
+        P.linear_act(x, w, w)
+    with pytest.raises(ValueError, match="\\[N, K\\]"):
+        P.linear_act(x, b)
+    _, w2, b2 = make(trainable=False)
+    with pytest.raises(ValueError, match="no gradients"):
+        P.linear_act(x.clone().requires_grad_(True), w2, b2)
+    with torch.no_grad():
+        assert P.linear_act(x, w2, b2).shape == (4, 6)
