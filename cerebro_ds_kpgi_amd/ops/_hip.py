@@ -1708,3 +1708,72 @@ def linear_act_bwd(dy, d, x, wref, bref, act, need_dx):
             c_p(bp), bst, M, N, K, G, act, _ptr(ws), n, _stream())
         _check(rc, "cer_dense_bwd")
     return dx
+
+
+# ---------------------------------------------------------------------------
+# distillation loss (csrc/hip/distill.hip), top logits (csrc/hip/toplogits.hip)
+# ---------------------------------------------------------------------------
+_TEACHER = [c_p, c_i, c_i64, c_i64, c_p, c_i64, c_i64]
+_SIGS.update({
+    "cer_distill_ws": [c_i, c_i, c_i, c_i],
+    "cer_distill_fwd": [c_p, c_i64, c_p] + _TEACHER + [c_p, c_p, c_p, c_p, c_p, c_p, c_i, c_i, c_i,
+                                                       c_i, c_p, c_i64, c_p],
+    "cer_distill_bwd": [c_p, c_i64, c_p] + _TEACHER + [c_p, c_p, c_p, c_p, c_p, c_i, c_i, c_i, c_i,
+                                                       c_p],
+    "cer_top_ws": [c_i, c_i, c_i, c_i, c_i],
+    "cer_top_logits": [c_p, c_i64, c_p, c_p, c_i, c_i, c_i, c_i, c_p, c_i64, c_p],
+})
+_RET_I64 |= {"cer_distill_ws", "cer_top_ws"}
+IMPLEMENTED |= {"distill", "top_logits"}
+
+
+def _teacher(val, idx):
+    """Arguments of a teacher's entries [G, B, K], entries adjacent."""
+    return (_ptr(val), int(val.dtype == torch.float32), val.stride(0), val.stride(1), _ptr(idx),
+            idx.stride(0), idx.stride(1))
+
+
+def distill_fwd(logits, labels, acc, G, val, idx, alpha, tau, need_grad):
+    """(loss [G], stats for ``distill_bwd``, gradient for a loss gradient of
+    ones or None)."""
+    with _on(logits):
+        B, GN = logits.shape
+        N, K = GN // G, val.shape[2]
+        dev = logits.device
+        n = lib().cer_distill_ws(B, G, N, int(logits.dtype == torch.bfloat16))
+        # loss, stats and workspace in one allocation
+        buf = torch.empty(G + 4 * G * B + n, dtype=torch.float32, device=dev)
+        loss, stats, ws = buf[:G], buf[G:G + 4 * G * B], buf[G + 4 * G * B:]
+        d = torch.empty((B, GN), dtype=logits.dtype, device=dev) if need_grad else None
+        rc = _fn("cer_distill_fwd", logits)(
+            _ptr(logits), logits.stride(0), _ptr(labels), *_teacher(val, idx), _ptr(alpha),
+            _ptr(tau), _ptr(stats), _ptr(d), _ptr(loss), _ptr(acc), B, G, N, K, _ptr(ws), n,
+            _stream())
+        _check(rc, "cer_distill_fwd")
+    return loss, stats, d
+
+
+def distill_bwd(logits, labels, G, val, idx, alpha, tau, dloss, stats):
+    with _on(logits):
+        B, GN = logits.shape
+        d = torch.empty((B, GN), dtype=logits.dtype, device=logits.device)
+        rc = _fn("cer_distill_bwd", logits)(
+            _ptr(logits), logits.stride(0), _ptr(labels), *_teacher(val, idx), _ptr(alpha),
+            _ptr(tau), _ptr(dloss), _ptr(stats), _ptr(d), B, G, GN // G, val.shape[2], _stream())
+        _check(rc, "cer_distill_bwd")
+    return d
+
+
+def top_logits(logits, G, k):
+    with _on(logits):
+        B, GN = logits.shape
+        N = GN // G
+        dev = logits.device
+        val = torch.empty((G, B, k), dtype=logits.dtype, device=dev)
+        idx = torch.empty((G, B, k), dtype=torch.int32, device=dev)
+        n = lib().cer_top_ws(B, G, N, k, int(logits.dtype == torch.bfloat16))
+        ws = torch.empty(n, dtype=torch.int64, device=dev) if n > 0 else None
+        rc = _fn("cer_top_logits", logits)(_ptr(logits), logits.stride(0), _ptr(val), _ptr(idx), B,
+                                           G, N, k, _ptr(ws), max(n, 0), _stream())
+        _check(rc, "cer_top_logits")
+    return val, idx

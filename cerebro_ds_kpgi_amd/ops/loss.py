@@ -90,3 +90,192 @@ def eval_metrics(logits, labels, acc, G):
 class _Ctx(object):
     def save_for_backward(self, *a):
         pass
+
+
+# ---------------------------------------------------------------------------
+# distillation from a teacher's top logits
+# ---------------------------------------------------------------------------
+MAX_TOP = 1024          # teacher entries of a row (csrc/hip/distill.hip KMAX)
+
+
+def _logit_rows(what, logits, G):
+    """[B, G*N] logits with adjacent columns; (rows, N)."""
+    if logits.dim() != 2 or G < 1 or logits.shape[1] % G or logits.shape[1] == 0:
+        raise ValueError("{}: logits {} are not [B, G*N] for G = {}".format(
+            what, tuple(logits.shape), G))
+    if logits.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError("{}: logits are {}, not fp32 or bf16".format(what, logits.dtype))
+    if logits.shape[0] == 0:
+        raise ValueError("{}: no rows".format(what))
+    if logits.stride(1) != 1 or logits.stride(0) < logits.shape[1]:
+        logits = logits.contiguous()
+    return logits, logits.shape[1] // G
+
+
+def top_logits(logits, G, k):
+    """The ``k`` largest logits of every row and their classes.
+
+    logits ``[B, G*N]`` (fp32 or bf16) -> values ``[G, B, k]`` in the logits'
+    dtype and classes ``[G, B, k]`` int32, in descending order, equal values by
+    class number (+0 equals -0, NaN counts as largest); 1 <= k <= min(N, 1024).
+    No gradient: this is what a teacher hands to ``distill_ce``.
+    """
+    z, N = _logit_rows("top_logits", logits.detach(), G)
+    if not 1 <= k <= min(N, MAX_TOP):
+        raise ValueError("top_logits: k = {} is not in 1 .. min(N = {}, {})".format(k, N, MAX_TOP))
+    if use_hip("top_logits", z):
+        from . import _hip
+        return _hip.top_logits(z, G, k)
+    v, i = torch.sort(z.reshape(-1, G, N).transpose(0, 1), dim=2, descending=True, stable=True)
+    return v[:, :, :k].contiguous(), i[:, :, :k].to(torch.int32)
+
+
+class DistillCE(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, acc, G, val, idx, alpha, tau, unit, train):
+        ctx.unit, ctx.G, ctx.shape = unit, G, logits.shape
+        ctx.hip = use_hip("distill", logits)
+        if ctx.hip:
+            from . import _hip
+            loss, stats, d = _hip.distill_fwd(logits, labels, acc, G, val, idx, alpha, tau,
+                                              train and unit)
+            if train:
+                if unit:
+                    ctx.save_for_backward(d)
+                else:
+                    ctx.save_for_backward(logits, labels, val, idx, alpha, tau, stats)
+            return loss
+        loss, d = _distill_torch(logits, labels, acc, G, val, idx, alpha, tau)
+        if train:
+            ctx.save_for_backward(d.to(logits.dtype) if unit else d)
+            ctx.dtype = logits.dtype
+        return loss
+
+    @staticmethod
+    def backward(ctx, dloss):
+        none = (None,) * 9
+        if ctx.unit:                    # dloss is ones by the caller's contract
+            return (ctx.saved_tensors[0],) + none
+        if ctx.hip:
+            from . import _hip
+            logits, labels, val, idx, alpha, tau, stats = ctx.saved_tensors
+            return (_hip.distill_bwd(logits, labels, ctx.G, val, idx, alpha, tau,
+                                     dloss.contiguous(), stats),) + none
+        d, = ctx.saved_tensors
+        d = d.view(d.shape[0], ctx.G, -1) * dloss.view(1, ctx.G, 1)
+        return (d.reshape(ctx.shape).to(ctx.dtype),) + none
+
+
+def _distill_torch(logits, labels, acc, G, val, idx, alpha, tau):
+    """Loss [G] and its gradient [B, G*N] (fp32, for dloss = 1); the oracle."""
+    B = logits.shape[0]
+    N = logits.shape[1] // G
+    inf = float("inf")
+    z = logits.detach().reshape(B, G, N).float()
+    lab = labels.t().long()                                             # [B, G]
+    v, i = val.transpose(0, 1).float(), idx.transpose(0, 1).long()      # [B, G, K]
+    a, ta = alpha.view(1, G), tau.view(1, G)
+    hard_on = (lab >= 0) & (a != 1)
+    there = (i >= 0) & (v != -inf) & (a != 0).unsqueeze(2)
+    bad = (lab >= N) | ((i >= N) & (a != 0).unsqueeze(2)).any(2)
+    there = there & (i < N)
+    soft_on = there.any(2)
+    yi = lab.clamp(0, N - 1).unsqueeze(2)
+    ii = i.clamp(0, N - 1)
+
+    zy = z.gather(2, yi)
+    lse = torch.logsumexp(z, dim=2)
+    hard = torch.where(hard_on, lse - zy.squeeze(2), torch.zeros_like(lse))
+    vt = torch.where(there, v, torch.full_like(v, -inf)) / ta.unsqueeze(2)
+    vt = torch.where(soft_on.unsqueeze(2), vt, torch.zeros_like(vt))
+    p = torch.where(there, torch.softmax(vt, dim=2), torch.zeros_like(vt))
+    logp = torch.log_softmax(vt, dim=2)
+    logq = torch.log_softmax(z / ta.unsqueeze(2), dim=2)
+    kl = torch.where(p > 0, p * (logp - logq.gather(2, ii)), p)
+    soft = torch.where(soft_on, kl.sum(2), torch.zeros_like(lse))
+    row = torch.where(hard_on, (1 - a) * hard, torch.zeros_like(hard))
+    row = row + torch.where(soft_on, a * ta * ta * soft, torch.zeros_like(soft))
+    row = torch.where(bad, torch.full_like(row, float("nan")), row)
+
+    onehot = torch.zeros_like(z).scatter_(2, yi, 1.0)
+    d = torch.where(hard_on.unsqueeze(2), (1 - a).unsqueeze(2) * (torch.softmax(z, 2) - onehot),
+                    torch.zeros_like(z))
+    mass = torch.zeros_like(z).scatter_add_(2, ii, p)
+    d = d + torch.where(soft_on.unsqueeze(2), (a * ta).unsqueeze(2) * (logq.exp() - mass),
+                        torch.zeros_like(z))
+    d = torch.where(bad.unsqueeze(2), torch.full_like(d, float("nan")), d) / B
+
+    known = (lab >= 0) & (lab < N)
+    cols = torch.arange(N, device=z.device).view(1, 1, N)
+    rank = ((z > zy) | ((z == zy) & (cols < yi))).sum(2)
+    top1 = ((rank < 1) & known).float().sum(0)
+    top5 = (((rank < 5) & known).float().sum(0) if N > 2 else torch.full_like(top1, float(B)))
+    acc += torch.stack([row.sum(0), top1, top5, torch.full_like(top1, float(B))], 1)
+    return row.mean(0), d.reshape(B, G * N)
+
+
+def _per_config(what, x, G, device, lo, hi):
+    """A hyper-parameter as an fp32 [G] tensor; numbers are range-checked."""
+    if isinstance(x, torch.Tensor):
+        if tuple(x.shape) != (G,) or x.dtype != torch.float32 or x.device != device:
+            raise ValueError("distill_ce: {} must be a number or an fp32 [{}] tensor on {}".format(
+                what, G, device))
+        return x.detach().contiguous()
+    if not lo <= float(x) <= hi:
+        raise ValueError("distill_ce: {} = {} is not in [{}, {}]".format(what, x, lo, hi))
+    return torch.full((G,), float(x), dtype=torch.float32, device=device)
+
+
+def distill_ce(logits, labels, acc, G, top_val, top_idx, alpha=0.5, tau=1.0, unit=False):
+    """Per-config mean ``[G]`` of cross-entropy mixed with distillation from a
+    teacher known by its top logits (``top_logits``), with metrics.
+
+    Row (g, b), student logits z, label y, teacher entries (i_k, v_k)::
+
+        p = softmax_k(v_k / tau)      q = softmax(z / tau)
+        (1 - alpha) (lse(z) - z_y) + alpha tau^2 sum_k p_k (log p_k - log q_{i_k})
+
+    ``logits [B, G*N]`` fp32 or bf16; ``labels [G, B]`` int32, negative = no
+    label; ``top_val`` (fp32 or bf16) and ``top_idx`` (int32) ``[G, B, K]``, or
+    ``[B, K]`` for one teacher of all configurations, 0 <= K <= 1024: a negative
+    class or a value of -inf is no entry, a class named twice counts twice.
+    ``alpha`` in [0, 1] and ``tau`` > 0 are numbers or fp32 ``[G]`` device
+    tensors (not range-checked there).  A row without a label has no first term,
+    one without entries no second, and a term of weight zero is not computed;
+    a label or class >= N makes the row's loss and gradient NaN.  The mean is
+    over all B rows.
+
+    ``acc [G, 4]`` fp32 += (sum of the rows' losses, top-1, top-5, B), as in
+    ``softmax_ce``; unlabelled rows are no hits (with N == 2 every row is a top-5
+    hit).  Gradient in ``logits`` only.  ``unit=True``: the caller
+    back-propagates a gradient of ones, and the forward writes the gradient in
+    the same pass over the logits.
+    """
+    z, N = _logit_rows("distill_ce", logits, G)
+    B, dev = z.shape[0], z.device
+    if top_val.dim() == 2:
+        top_val = top_val.unsqueeze(0).expand(G, -1, -1)
+    if top_idx.dim() == 2:
+        top_idx = top_idx.unsqueeze(0).expand(G, -1, -1)
+    for name, t, dt, shape in (
+            ("labels", labels, (torch.int32,), (G, B)), ("acc", acc, (torch.float32,), (G, 4)),
+            ("top_val", top_val, (torch.float32, torch.bfloat16), (G, B, top_val.shape[-1])),
+            ("top_idx", top_idx, (torch.int32,), (G, B, top_val.shape[-1]))):
+        if tuple(t.shape) != shape or t.dtype not in dt or t.device != dev:
+            raise ValueError("distill_ce: {} is {} {} on {}, not {} {} on {}".format(
+                name, tuple(t.shape), t.dtype, t.device, shape,
+                " or ".join(str(d) for d in dt), dev))
+    if top_val.shape[2] > MAX_TOP:
+        raise ValueError("distill_ce: {} teacher entries, at most {}".format(top_val.shape[2],
+                                                                             MAX_TOP))
+    if not acc.is_contiguous():
+        raise ValueError("distill_ce: acc must be contiguous")
+    alpha = _per_config("alpha", alpha, G, dev, 0.0, 1.0)
+    tau = _per_config("tau", tau, G, dev, 1e-6, 1e6)
+    if top_val.shape[2] and top_val.stride(2) != 1:
+        top_val = top_val.contiguous()
+    if top_idx.shape[2] and top_idx.stride(2) != 1:
+        top_idx = top_idx.contiguous()
+    train = torch.is_grad_enabled() and z.requires_grad
+    return DistillCE.apply(z, labels.contiguous(), acc, G, top_val.detach(), top_idx, alpha, tau,
+                           unit, train)

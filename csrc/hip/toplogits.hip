@@ -1,0 +1,375 @@
+// The K largest logits of every row and their classes, in descending order,
+// equal values by class number (ops.loss.top_logits).
+//
+// Order: NaN before everything, +0 equal to -0, otherwise by value; equal
+// values lowest class first.  With key(z) an unsigned integer that increases
+// with that order, element j is the 64-bit number key << 32 | ~j: all distinct,
+// so "the K largest" has one answer and any way of finding them gives it.
+//
+// A row is read once, into the registers of a block.  Selection by filter:
+// each wave finds the ceil(K / waves)-th largest of its threads' maxima, the
+// smallest of these bounds is at most the K-th largest element, and only the
+// elements that reach it (some tens for K = 10, some hundreds for K = 200) go
+// to LDS to be ordered.  Rows that defeat the filter -- NaN, or so many equal
+// values that the candidates overflow -- are narrowed by a radix search over
+// the 64-bit numbers instead: exact for any input, slower.
+//
+// What bounds it: the one read of the logits.  Rows longer than a block's
+// registers, and long rows that are too few to fill the chip, are cut into
+// chunks; the chunks' lists are merged.
+#include "rowreg.h"
+
+constexpr int TOP_KMAX = 1024;
+constexpr int TOP_CAND = 4096;       // candidates in LDS
+constexpr int TOP_MERGE = 8192;      // numbers a merging block sorts
+
+struct TopP {
+  const void* z;
+  int64_t ldz;
+  void* val;             // [G][B][K]
+  int* idx;
+  uint64_t* list;        // chunked: [rows][chunks][K]
+  int B, G, N, K, chunks, chunk;
+};
+
+__device__ __forceinline__ uint32_t key_of(float z) {
+  uint32_t u = __float_as_uint(z);
+  if (z != z) return 0xffffffffu;
+  if (z == 0.f) u = 0;
+  return (u >> 31) ? ~u : u | 0x80000000u;
+}
+
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k);
+}
+
+__device__ __forceinline__ uint64_t number_of(float z, int j) {
+  return ((uint64_t)key_of(z) << 32) | (uint32_t)~j;
+}
+
+// s[0 .. n) in descending order; n a power of two, all TH threads
+template <int TH>
+__device__ __forceinline__ void bitonic(uint64_t* s, int n) {
+  for (int k = 2; k <= n; k <<= 1) {
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < n / 2; i += TH) {
+        const int a = 2 * i - (i & (j - 1)), b = a + j;
+        const uint64_t x = s[a], y = s[b];
+        if ((x < y) == ((a & k) == 0)) {
+          s[a] = y;
+          s[b] = x;
+        }
+      }
+    }
+  }
+  __syncthreads();
+}
+
+// The C numbers in s (room for the next power of two, above 512) in descending
+// order to out(rank, number) for rank < K.
+template <int TH, typename F>
+__device__ __forceinline__ void ordered(uint64_t* s, int C, int K, F out) {
+  if (C <= 512) {
+    // few: every number counts the larger ones
+    const int c2 = (C + 1) & ~1;
+    if (threadIdx.x == 0 && c2 > C) s[C] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < C; i += TH) {
+      const uint64_t me = s[i];
+      int rank = 0;
+      for (int c = 0; c < c2; c += 2) rank += (s[c] > me ? 1 : 0) + (s[c + 1] > me ? 1 : 0);
+      if (rank < K) out(rank, me);
+    }
+    return;
+  }
+  int n = 1024;
+  while (n < C) n <<= 1;
+  for (int i = C + threadIdx.x; i < n; i += TH) s[i] = 0;
+  bitonic<TH>(s, n);
+  for (int i = threadIdx.x; i < K; i += TH) out(i, s[i]);
+}
+
+// Radix search of a row for its K-th largest number, 8 bits at a time from the
+// top, until what reaches the prefix fits `room`; those go to cand.  Reads the
+// row from memory (one of the last levels of cache has it).
+template <typename T, int TH>
+__device__ __noinline__ int radix_candidates(const T* zr, int n, int lo, int K, uint64_t* cand,
+                                             int room, int* hist, int* count) {
+  const int tid = threadIdx.x;
+  uint64_t prefix = 0;
+  int above = 0;                       // elements above the prefix
+  for (int sh = 56; sh >= 0; sh -= 8) {
+    __syncthreads();
+    for (int i = tid; i < 256; i += TH) hist[i] = 0;
+    __syncthreads();
+    for (int j = tid; j < n; j += TH) {
+      const uint64_t x = number_of(ld1(zr + j), lo + j);
+      if (sh == 56 || (x >> (sh + 8)) == (prefix >> (sh + 8)))
+        atomicAdd(&hist[(int)(x >> sh) & 255], 1);
+    }
+    __syncthreads();
+    // hist[d] = elements with the prefix and a digit >= d
+    for (int o = 1; o < 256; o <<= 1) {
+      int add[(256 + TH - 1) / TH];
+#pragma unroll
+      for (int i = 0; i < (256 + TH - 1) / TH; ++i) {
+        const int d = tid + i * TH;
+        add[i] = d + o < 256 ? hist[d + o] : 0;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < (256 + TH - 1) / TH; ++i) {
+        const int d = tid + i * TH;
+        if (d < 256) hist[d] += add[i];
+      }
+      __syncthreads();
+    }
+    // the largest digit that K elements reach
+    int lo_d = 0, hi_d = 255;
+    while (lo_d < hi_d) {
+      const int mid = (lo_d + hi_d + 1) >> 1;
+      if (above + hist[mid] >= K) lo_d = mid;
+      else hi_d = mid - 1;
+    }
+    prefix |= (uint64_t)lo_d << sh;
+    const int reach = above + hist[lo_d];
+    if (reach <= room) break;
+    if (lo_d < 255) above += hist[lo_d + 1];
+  }
+  __syncthreads();
+  if (tid == 0) *count = 0;
+  __syncthreads();
+  for (int j = tid; j < n; j += TH) {
+    const uint64_t x = number_of(ld1(zr + j), lo + j);
+    if (x >= prefix) cand[atomicAdd(count, 1)] = x;
+  }
+  __syncthreads();
+  return *count;
+}
+
+template <typename T, int TH, int R>
+__global__ __launch_bounds__(TH) void top_rows(const TopP P) {
+  constexpr int W = TH / 64, V = RowRegs<T, TH, R>::V, CAP = RowRegs<T, TH, R>::CAP;
+  constexpr int GR = R >= 4 ? 4 : 1;          // maxima a thread keeps for larger K
+  // candidates: a short row fits whole (up to 512 are ranked, which needs one
+  // more place; above that the size is a power of two for the sort)
+  constexpr int ROOM = CAP <= 512 ? 514 : (CAP < TOP_CAND ? CAP : TOP_CAND);
+  __shared__ __attribute__((aligned(16))) uint64_t cand[ROOM];
+  __shared__ uint32_t bound[16];
+  __shared__ int hist[CAP > TOP_CAND ? 256 : 1], count, nanflag;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int row = blockIdx.x / P.chunks, ch = blockIdx.x - row * P.chunks;
+  const int g = row / P.B, b = row - g * P.B;
+  const int lo = ch * P.chunk, n = min(P.chunk, P.N - lo);
+  const T* zr = reinterpret_cast<const T*>(P.z) + (int64_t)b * P.ldz + (int64_t)g * P.N + lo;
+  RowRegs<T, TH, R> regs;
+  if (tid == 0) {
+    count = 0;
+    nanflag = 0;
+  }
+  regs.load(zr, n, tid);
+  const int K = min(P.K, n);
+  const int kw = (K + W - 1) / W;
+  __syncthreads();
+
+  // maxima of GR groups of this thread's elements; NaN is only noted
+  float m[GR];
+#pragma unroll
+  for (int q = 0; q < GR; ++q) m[q] = -INFINITY;
+  bool nan = regs.edge != regs.edge;
+  m[0] = fmaxf(m[0], regs.edge);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const uint4 u = regs.fresh(r);
+    float t = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float z = regs.get(u, e);
+      nan |= z != z;
+      t = fmaxf(t, z);
+    }
+    m[r % GR] = fmaxf(m[r % GR], t);
+  }
+  if (__ballot(nan) && lane == 0) nanflag = 1;
+  if (GR > 1 && kw <= 16) {
+#pragma unroll
+    for (int q = 1; q < GR; ++q) {
+      m[0] = fmaxf(m[0], m[q]);
+      m[q] = -INFINITY;
+    }
+  }
+  uint32_t mk[GR];
+#pragma unroll
+  for (int q = 0; q < GR; ++q) mk[q] = key_of(m[q]);
+  // this wave's kw-th largest maximum, its upper 20 bits
+  uint32_t t = 0;
+  if (kw <= 64 * GR) {
+    for (int bit = 31; bit >= 12; --bit) {
+      const uint32_t c = t | (1u << bit);
+      int reach = 0;
+#pragma unroll
+      for (int q = 0; q < GR; ++q) reach += __popcll(__ballot(mk[q] >= c));
+      if (reach >= kw) t = c;
+    }
+  }
+  if (lane == 0) bound[wave] = t;
+  __syncthreads();
+  uint32_t lim = bound[0];
+#pragma unroll
+  for (int w = 1; w < W; ++w) lim = min(lim, bound[w]);
+  const bool has_nan = nanflag != 0;
+  int C = ROOM + 1;
+  if (!has_nan || CAP <= TOP_CAND) {
+    // a bound below -inf's key takes every element; so does a short row with NaN
+    const float fl = has_nan || lim <= 0x007fffffu ? -INFINITY : key_value(lim);
+    auto push = [&](int j, float z) {
+      if (!(z < fl) && j < n) {
+        const int at = atomicAdd(&count, 1);
+        if (at < ROOM) cand[at] = number_of(z, lo + j);
+      }
+    };
+    regs.vecs(tid, [&](int j, const float* z) {
+      bool any = false;
+#pragma unroll
+      for (int e = 0; e < V; ++e) any |= !(z[e] < fl);
+      if (__ballot(any)) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) push(j + e, z[e]);
+      }
+    });
+    push(regs.ej >= 0 ? regs.ej : 0x7fffffff, regs.edge);
+    __syncthreads();
+    C = count;
+  }
+  if constexpr (CAP > TOP_CAND) {
+    if (C > ROOM) C = radix_candidates<T, TH>(zr, n, lo, K, cand, ROOM, hist, &count);
+  }
+  if (P.chunks == 1) {
+    T* val = reinterpret_cast<T*>(P.val) + (int64_t)row * P.K;
+    int* idx = P.idx + (int64_t)row * P.K;
+    ordered<TH>(cand, C, K, [&](int k, uint64_t x) {
+      const int j = (int)~(uint32_t)x;
+      idx[k] = j;
+      val[k] = zr[j];
+    });
+  } else {
+    uint64_t* out = P.list + (int64_t)blockIdx.x * P.K;
+    ordered<TH>(cand, C, K, [&](int k, uint64_t x) { out[k] = x; });
+    for (int k = K + tid; k < P.K; k += TH) out[k] = 0;     // a last chunk shorter than K
+  }
+}
+
+// `per` lists of K numbers into one; the last merge writes the result
+template <typename T, int TH>
+__global__ __launch_bounds__(TH) void top_merge(const TopP P, const uint64_t* __restrict__ in,
+                                                uint64_t* __restrict__ out, int lists, int per,
+                                                int last) {
+  extern __shared__ __attribute__((aligned(16))) uint64_t s[];
+  const int groups = (lists + per - 1) / per;
+  const int row = blockIdx.x / groups, gr = blockIdx.x - row * groups;
+  const int l0 = gr * per, nl = min(per, lists - l0);
+  const int C = nl * P.K;
+  int n = 2;
+  while (n < C) n <<= 1;
+  const uint64_t* src = in + ((int64_t)row * lists + l0) * P.K;
+  for (int i = threadIdx.x; i < n; i += TH) s[i] = i < C ? src[i] : 0;
+  bitonic<TH>(s, n);
+  if (!last) {
+    uint64_t* o = out + ((int64_t)row * groups + gr) * P.K;
+    for (int k = threadIdx.x; k < P.K; k += TH) o[k] = s[k];
+    return;
+  }
+  const int g = row / P.B, b = row - g * P.B;
+  const T* zr = reinterpret_cast<const T*>(P.z) + (int64_t)b * P.ldz + (int64_t)g * P.N;
+  for (int k = threadIdx.x; k < P.K; k += TH) {
+    const int j = (int)~(uint32_t)s[k];
+    P.idx[(int64_t)row * P.K + k] = j;
+    reinterpret_cast<T*>(P.val)[(int64_t)row * P.K + k] = zr[j];
+  }
+}
+
+template <typename T>
+static int top_chunk(int64_t rows, int N, int K) {
+  constexpr int V = 16 / (int)sizeof(T);
+  int c = N;
+  if (N > 1024 * 16 * V) c = 1024 * 16 * V;
+  // few rows: shorter chunks put more of the chip to work
+  if (rows < 128 && N > 256 * 8 * V) c = 256 * 8 * V;
+  return c;
+}
+
+static inline bool top_sizes(int B, int G, int N, int K) {
+  return B > 0 && G > 0 && N > 0 && N < 0x7ffffff0 && K > 0 && K <= N && K <= TOP_KMAX &&
+         (int64_t)B * G <= 0x7fffffff;
+}
+
+// 64-bit numbers of workspace, -1 for sizes out of range
+template <typename T>
+static int64_t top_ws(int B, int G, int N, int K) {
+  if (!top_sizes(B, G, N, K)) return -1;
+  const int64_t rows = (int64_t)B * G;
+  const int c = top_chunk<T>(rows, N, K);
+  const int64_t chunks = (N + c - 1) / c;
+  if (rows * chunks > 0x7fffffff) return -1;
+  return chunks > 1 ? 2 * rows * chunks * K : 0;
+}
+
+CER_API int64_t cer_top_ws(int B, int G, int N, int K, int is_bf16) {
+  return is_bf16 ? top_ws<bf16_t>(B, G, N, K) : top_ws<float>(B, G, N, K);
+}
+
+template <typename T>
+static int top_launch(const T* z, int64_t ldz, T* val, int* idx, int B, int G, int N, int K,
+                      uint64_t* ws, int64_t ws_n, hipStream_t st) {
+  const int64_t need = top_ws<T>(B, G, N, K);
+  if (need < 0 || ws_n < need || !z || !val || !idx || ldz < (int64_t)G * N)
+    return (int)hipErrorInvalidValue;
+  const int64_t rows = (int64_t)B * G;
+  TopP P = {};
+  P.z = z; P.ldz = ldz; P.val = val; P.idx = idx;
+  P.B = B; P.G = G; P.N = N; P.K = K;
+  P.chunk = top_chunk<T>(rows, N, K);
+  P.chunks = (N + P.chunk - 1) / P.chunk;
+  P.list = ws;
+  const int grid = (int)(rows * P.chunks);
+  const int n = P.chunk;
+  constexpr int V = 16 / (int)sizeof(T);
+  if (n <= 64 * V) top_rows<T, 64, 1><<<grid, 64, 0, st>>>(P);
+  else if (n <= 256 * V) top_rows<T, 256, 1><<<grid, 256, 0, st>>>(P);
+  else if (n <= 256 * 4 * V) top_rows<T, 256, 4><<<grid, 256, 0, st>>>(P);
+  else if (n <= 256 * 8 * V) top_rows<T, 256, 8><<<grid, 256, 0, st>>>(P);
+  else if (n <= 512 * 8 * V) top_rows<T, 512, 8><<<grid, 512, 0, st>>>(P);
+  else if (n <= 512 * 16 * V) top_rows<T, 512, 16><<<grid, 512, 0, st>>>(P);
+  else top_rows<T, 1024, 16><<<grid, 1024, 0, st>>>(P);
+  if (P.chunks > 1) {
+    int per = TOP_MERGE / K;
+    const uint64_t* in = ws;
+    uint64_t* out = ws + rows * P.chunks * K;
+    int lists = P.chunks;
+    while (true) {
+      const int groups = (lists + per - 1) / per;
+      const int nl = lists < per ? lists : per;
+      int p2 = 2;
+      while (p2 < nl * K) p2 <<= 1;
+      const int last = groups == 1;
+      top_merge<T, 512><<<(int)(rows * groups), 512, p2 * 8, st>>>(P, in, out, lists, per, last);
+      if (last) break;
+      lists = groups;
+      uint64_t* t = const_cast<uint64_t*>(in);
+      in = out;
+      out = t;
+    }
+  }
+  return (int)hipGetLastError();
+}
+
+CER_API int cer_top_logits(const bf16_t* z, int64_t ldz, bf16_t* val, int* idx, int B, int G, int N,
+                           int K, uint64_t* ws, int64_t ws_n, hipStream_t st) {
+  return top_launch<bf16_t>(z, ldz, val, idx, B, G, N, K, ws, ws_n, st);
+}
+
+CER_API int cer_top_logits_f32(const float* z, int64_t ldz, float* val, int* idx, int B, int G,
+                               int N, int K, uint64_t* ws, int64_t ws_n, hipStream_t st) {
+  return top_launch<float>(z, ldz, val, idx, B, G, N, K, ws, ws_n, st);
+}
