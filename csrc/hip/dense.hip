@@ -18,14 +18,19 @@
 //
 // Precision.  A bf16 operand is one plane; its products are exact in the fp32
 // accumulators of v_mfma_f32_16x16x32_bf16.  An fp32 operand is split when it
-// is staged into two bf16 planes, hi = RNE(x) and lo = RNE(x - hi), 16 bits of
-// the significand, and the product runs as lo*hi + hi*lo + hi*hi: the dropped
-// part (lo*lo and the rounding of lo) is at most 3 * 2^-18 of |x||w| per term.
-// That is the framework's fp32 mode (conv.hip), at 3/16 of the cost of fp32
-// MFMA.  In bf16 mode dz = dy * act'(z) has more than 8 bits: it is kept in
-// fp32, enters dW as two planes (dW is an fp32 tensor) and dx as one (dx is
-// rounded to bf16 anyway).  A non-finite fp32 factor gives a non-finite
-// result, NaN where a single fp32 product would give an infinity.
+// is staged into three bf16 planes p0 + p1 + p2, each the rounding of what the
+// ones before it leave: together its 24 bits.  The product runs as the six
+// terms p_i q_j with i + j <= 2, smallest first; what is dropped is below
+// 2^-24 of |x||w| a term, so the result is that of an fp32 product (measured
+// against 64 bits: as near as the library's) at 6/16 of the time of fp32 MFMA.
+// In bf16 mode dz = dy * act'(z) has more than 8 bits: it is kept in fp32,
+// enters dW as DZ_PLANES planes (dW is an fp32 tensor) and dx as one (dx is
+// rounded to bf16 anyway).  A non-finite fp32 factor gives a non-finite result,
+// NaN where a single fp32 product would give an infinity; |x| above 3.39e38
+// rounds to infinity.
+#include <atomic>
+#include <math.h>
+
 #include "common.h"
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -219,10 +224,17 @@ __device__ __forceinline__ void epilogue(const GemmP& P, int g, int row, int col
 // ---------------------------------------------------------------------------
 template <int BK>
 __device__ __forceinline__ int lds_off(int row, int chunk) {
-  // 16-B chunks of a row are XOR-swizzled so that neither 8 neighbouring rows
-  // (fragment reads) nor 8 rows V apart (transposing writes) share a bank
-  if constexpr (BK == 64) return row * 128 + ((chunk ^ ((row ^ (row >> 3)) & 7)) << 4);
-  else return row * 64 + ((chunk ^ (((row >> 1) ^ (row >> 3)) & 3)) << 4);
+  // 16-B chunks are XOR-swizzled by row.  A wave's 16-B LDS access goes 16 lanes
+  // at a time, 256 B; in a fragment read those are 16 neighbouring rows at one
+  // chunk, or 8 of them at that chunk and 8 at its neighbour (c ^ 1): the
+  // patterns below give 16 different places either way.  The transposing
+  // writes (rows V apart) keep two lanes to a place.
+  if constexpr (BK == 64) {
+    return row * 128 + ((chunk ^ (((row >> 1) ^ (row >> 4)) & 7)) << 4);
+  } else {
+    const int i = row >> 2;
+    return row * 64 + ((chunk ^ ((i ^ ((i & 1) << 1)) & 3)) << 4);
+  }
 }
 
 template <typename S, bool KS, int R, int BK, int T, int PL>
@@ -233,7 +245,9 @@ struct Stage {
   static constexpr bool F32 = sizeof(S) == 4;
   static constexpr int NR = F32 ? 8 * V : (KS ? 8 * (V > 1 ? V / 2 : 1) : 4 * V);
   static constexpr int BYTES = PL * R * BK * 2;
-  uint32_t r[NR];
+  struct Regs {
+    uint32_t r[NR];
+  };
   uint32_t off[KS ? 1 : V];   // byte offsets inside a step's tile
   const char* base;           // uniform: tile origin
   int64_t step_bytes;         // uniform: bytes from one step to the next
@@ -267,7 +281,8 @@ struct Stage {
     }
   }
 
-  __device__ __forceinline__ void load_full(int step) {
+  __device__ __forceinline__ void load_full(Regs& q_, int step) const {
+    uint32_t* r = q_.r;
     const char* p = base + step * step_bytes;
     if constexpr (!KS) {
 #pragma unroll
@@ -323,7 +338,8 @@ struct Stage {
   }
 
   // a step that reaches past the operand: elements outside are zero
-  __device__ __forceinline__ void load_edge(int step, int kleft, int tid) {
+  __device__ __forceinline__ void load_edge(Regs& q_, int step, int kleft, int tid) const {
+    uint32_t* r = q_.r;
     const char* p = base + step * step_bytes;
 #pragma unroll
     for (int i = 0; i < NR; ++i) r[i] = 0;
@@ -355,32 +371,41 @@ struct Stage {
     }
   }
 
-  __device__ __forceinline__ void load(int step, int k, int tid) {
-    const int kleft = k - step * BK;
-    if (kleft >= BK && colfull) load_full(step);
-    else load_edge(step, kleft, tid);
+  __device__ __forceinline__ bool full(int step, int k) const {
+    return k - step * BK >= BK && colfull;
+  }
+
+  __device__ __forceinline__ void load(Regs& q_, int step, int k, int tid) const {
+    if (full(step, k)) load_full(q_, step);
+    else load_edge(q_, step, k - step * BK, tid);
   }
 
   // the 8 k of chunk i as PL bf16 planes into LDS
-  __device__ __forceinline__ void store(char* lds, int tid) const {
+  __device__ __forceinline__ void store(const Regs& q_, char* lds, int tid) const {
+    const uint32_t* r = q_.r;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int row = KS ? (tid % (R / V)) * V + i : tid / CH + i * (T / CH);
       const int o = lds_off<BK>(row, kc);
       uint32_t h[4];
       if constexpr (F32) {
-        uint32_t l[4];
+        float a[4], b[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const float a = __uint_as_float(KS ? r[V * (2 * q) + i] : r[8 * i + 2 * q]);
-          const float b = __uint_as_float(KS ? r[V * (2 * q + 1) + i] : r[8 * i + 2 * q + 1]);
-          h[q] = cvt_pk_bf16(a, b);
-          if constexpr (PL == 2)
-            l[q] = cvt_pk_bf16(a - __uint_as_float(h[q] << 16),
-                               b - __uint_as_float(h[q] & 0xffff0000u));
+          a[q] = __uint_as_float(KS ? r[V * (2 * q) + i] : r[8 * i + 2 * q]);
+          b[q] = __uint_as_float(KS ? r[V * (2 * q + 1) + i] : r[8 * i + 2 * q + 1]);
         }
-        if constexpr (PL == 2)
-          *reinterpret_cast<uint4*>(lds + R * BK * 2 + o) = make_uint4(l[0], l[1], l[2], l[3]);
+#pragma unroll
+        for (int p = 0; p < PL; ++p) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            h[q] = cvt_pk_bf16(a[q], b[q]);
+            a[q] -= __uint_as_float(h[q] << 16);
+            b[q] -= __uint_as_float(h[q] & 0xffff0000u);
+          }
+          *reinterpret_cast<uint4*>(lds + p * (R * BK * 2) + o) = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+        continue;
       } else if constexpr (KS) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -402,12 +427,12 @@ struct Stage {
 };
 
 // ---------------------------------------------------------------------------
-// C tile BM x BN per block; WM x WN waves; LDS double buffered: the tile of
-// step t + 1 goes from registers to LDS and step t + 2 is requested while step
-// t is multiplied, one barrier per step
+// C tile BM x BN per block; WM x WN waves; LDS double buffered: while step t is
+// multiplied, the tile of step t + 1 goes from registers to LDS and that of step
+// t + 1 + PF is requested; one barrier per step.  PF tiles wait in registers.
 // ---------------------------------------------------------------------------
 template <typename SA, typename SB, int PA, int PB, bool KA, bool KB, int BM, int BN, int BK,
-          int WM, int WN, int EPI, typename TO>
+          int WM, int WN, int PF, int EPI, typename TO>
 __global__ __launch_bounds__(WM * WN * 64, 2) void dense_gemm(const GemmP P) {
   constexpr int T = WM * WN * 64;
   constexpr int IM = BM / WM / 16, JN = BN / WN / 16;
@@ -454,75 +479,125 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void dense_gemm(const GemmP P) {
   const int wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
   const int fr = lane & 15, fc = lane >> 4;
 
-  if (s0 < s1) {
-    sa.load(s0, P.k, tid);
-    sb.load(s0, P.k, tid);
-    sa.store(smem, tid);
-    sb.store(smem + StA::BYTES, tid);
-    if (s0 + 1 < s1) {
-      sa.load(s0 + 1, P.k, tid);
-      sb.load(s0 + 1, P.k, tid);
+  auto mma = [&](const char* cur, int kk) {
+    bf16x8 bf[JN][PB];
+#pragma unroll
+    for (int j = 0; j < JN; ++j)
+#pragma unroll
+      for (int p = 0; p < PB; ++p)
+        bf[j][p] = *reinterpret_cast<const bf16x8*>(cur + StA::BYTES + p * (BN * BK * 2) +
+                                                    lds_off<BK>(wn + j * 16 + fr, kk * 4 + fc));
+#pragma unroll
+    for (int i = 0; i < IM; ++i) {
+      bf16x8 af[PA];
+#pragma unroll
+      for (int p = 0; p < PA; ++p)
+        af[p] = *reinterpret_cast<const bf16x8*>(cur + p * (BM * BK * 2) +
+                                                 lds_off<BK>(wm + i * 16 + fr, kk * 4 + fc));
+      // operands swapped: a lane ends with 4 neighbouring columns of a row
+#pragma unroll
+      for (int t = 2; t >= 0; --t)
+#pragma unroll
+        for (int p = PA - 1; p >= 0; --p) {
+          if (t - p < 0 || t - p >= PB) continue;
+#pragma unroll
+          for (int j = 0; j < JN; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[j][t - p], af[p], acc[i][j], 0,
+                                                                0, 0);
+        }
     }
+  };
+
+  typename StA::Regs ra[PF];
+  typename StB::Regs rb[PF];
+  auto load = [&](int q, int s) {
+    sa.load(ra[q], s, P.k, tid);
+    sb.load(rb[q], s, P.k, tid);
+  };
+  auto store = [&](int q, char* buf) {
+    sa.store(ra[q], buf, tid);
+    sb.store(rb[q], buf + StA::BYTES, tid);
+  };
+  if (s0 < s1) {
+    // tile s0 + i waits in registers i % PF
+    load(0, s0);
+    store(0, smem);
+#pragma unroll
+    for (int i = 1; i <= PF; ++i)
+      if (s0 + i < s1) load(i % PF, s0 + i);
     __syncthreads();
-    for (int s = s0; s < s1; ++s) {
-      const char* cur = smem + ((s - s0) & 1) * BUF;
-      if (s + 1 < s1) {
-        char* nxt = smem + ((s + 1 - s0) & 1) * BUF;
-        sa.store(nxt, tid);
-        sb.store(nxt + StA::BYTES, tid);
-        if (s + 2 < s1) {
-          sa.load(s + 2, P.k, tid);
-          sb.load(s + 2, P.k, tid);
-        }
+    int s = s0;
+    char *cur = smem, *nxt = smem + BUF;
+    // steps whose requests stay inside both operands: no branch between the
+    // multiplications, the stores and the requests
+    for (; s + 2 * PF < s1 && sa.full(s + 2 * PF, P.k) && sb.full(s + 2 * PF, P.k); s += PF) {
+#pragma unroll
+      for (int u = 0; u < PF; ++u) {
+        mma(cur, 0);
+        store((u + 1) % PF, nxt);
+        sa.load_full(ra[(u + 1) % PF], s + u + 1 + PF);
+        sb.load_full(rb[(u + 1) % PF], s + u + 1 + PF);
+#pragma unroll
+        for (int kk = 1; kk < BK / 32; ++kk) mma(cur, kk);
+        __syncthreads();
+        char* t = cur;
+        cur = nxt;
+        nxt = t;
       }
+    }
+    for (; s < s1; s += PF) {
 #pragma unroll
-      for (int kk = 0; kk < BK / 32; ++kk) {
-        bf16x8 bf[JN][PB];
-#pragma unroll
-        for (int j = 0; j < JN; ++j)
-#pragma unroll
-          for (int p = 0; p < PB; ++p)
-            bf[j][p] = *reinterpret_cast<const bf16x8*>(
-                cur + StA::BYTES + p * (BN * BK * 2) +
-                lds_off<BK>(wn + j * 16 + fr, kk * 4 + fc));
-#pragma unroll
-        for (int i = 0; i < IM; ++i) {
-          bf16x8 af[PA];
-#pragma unroll
-          for (int p = 0; p < PA; ++p)
-            af[p] = *reinterpret_cast<const bf16x8*>(
-                cur + p * (BM * BK * 2) + lds_off<BK>(wm + i * 16 + fr, kk * 4 + fc));
-          // operands swapped: a lane ends with 4 neighbouring columns of a row
-#pragma unroll
-          for (int j = 0; j < JN; ++j) {
-            if constexpr (PA == 2)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[j][0], af[1], acc[i][j], 0, 0, 0);
-            if constexpr (PB == 2)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[j][1], af[0], acc[i][j], 0, 0, 0);
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[j][0], af[0], acc[i][j], 0, 0, 0);
+      for (int u = 0; u < PF; ++u) {
+        if (s + u < s1) {
+          if (s + u + 1 < s1) {
+            store((u + 1) % PF, nxt);
+            if (s + u + 1 + PF < s1) load((u + 1) % PF, s + u + 1 + PF);
           }
+#pragma unroll
+          for (int kk = 0; kk < BK / 32; ++kk) mma(cur, kk);
+          __syncthreads();
+          char* t = cur;
+          cur = nxt;
+          nxt = t;
         }
       }
-      __syncthreads();
     }
   }
 
+  // Each wave turns its tile through LDS, 16 * ER rows at a time, so that its 64
+  // lanes finish and store whole row segments; the loop keeps the epilogue's
+  // code (activation, residual) short
+  constexpr int WC = BN / WN, PITCH = WC + 4, ER = IM < 2 ? 1 : 2;
+  static_assert(IM % ER == 0, "rows of a turn");
+  float* turn = reinterpret_cast<float*>(smem) + wave * (16 * ER * PITCH);
 #pragma unroll
-  for (int i = 0; i < IM; ++i) {
-    const int row = m0 + wm + i * 16 + fr;
-    if (row >= P.m) continue;
+  for (int i0 = 0; i0 < IM; i0 += ER) {
 #pragma unroll
-    for (int j = 0; j < JN; ++j) {
-      const int col = n0 + wn + j * 16 + fc * 4;
-      if (col >= P.n) continue;
-      float z[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-      if (P.splits > 1) {
-        float* q = P.part + (((int64_t)split * P.G + g) * P.m + row) * P.n + col;
-        st4(q, z, P.n - col);
-      } else {
-        epilogue<EPI, TO>(P, g, row, col, z);
+    for (int i = 0; i < ER; ++i)
+#pragma unroll
+      for (int j = 0; j < JN; ++j)
+        *reinterpret_cast<f32x4*>(turn + (i * 16 + fr) * PITCH + j * 16 + fc * 4) = acc[i0 + i][j];
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    constexpr int LC = WC / 4, RS = 64 / LC;        // lanes a row, rows a step
+    const int col = n0 + wn + (lane % LC) * 4;
+    if (col < P.n) {
+#pragma unroll 2
+      for (int r = lane / LC; r < 16 * ER; r += RS) {
+        const int row = m0 + wm + i0 * 16 + r;
+        if (row >= P.m) break;
+        const f32x4 t = *reinterpret_cast<const f32x4*>(turn + r * PITCH + (lane % LC) * 4);
+        float z[4] = {t[0], t[1], t[2], t[3]};
+        if (P.splits > 1)
+          st4(P.part + (((int64_t)split * P.G + g) * P.m + row) * P.n + col, z, P.n - col);
+        else
+          epilogue<EPI, TO>(P, g, row, col, z);
       }
     }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   }
 }
 
@@ -606,47 +681,70 @@ __global__ __launch_bounds__(256) void dense_dbsum(const float* __restrict__ par
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
+enum { T_BIG, T_MID, T_SMALL, T_THIN };
+
 struct Plan {
-  int tile;      // 0: 256x256, 1: 128x128, 2: 64x64, 3: 32x64
-  int bm, bn, bk, tm, tn, splits, steps;
+  int tile, tm, tn, splits, steps;
 };
 
-// planes: of both operands together (2: bf16, 3: one fp32, 4: both fp32)
+// tile sizes by the planes of both operands together: 2 (bf16), 1 + DZ_PLANES
+// (dW of a bf16 layer with a smooth activation), 6 (fp32)
+constexpr int DZ_PLANES = 3;
+static constexpr int tile_m(int planes, int t) {
+  return t == T_BIG ? (planes == 2 || planes == 6 ? 256 : 128) : t == T_MID ? 128 : t == T_SMALL ? 64 : 32;
+}
+static constexpr int tile_n(int planes, int t) {
+  return t == T_BIG ? (planes == 6 ? 128 : 256) : t == T_MID ? (planes == 6 ? 64 : 128) : 64;
+}
+static constexpr int tile_k(int planes, int t) {
+  return t == T_THIN ? 64 : planes == 2 ? (t == T_MID ? 32 : 64) : 32;
+}
+// blocks of a CU (LDS and registers)
+static constexpr int tile_occ(int planes, int t) {
+  return t == T_BIG ? 1 : t == T_MID ? 2 : t == T_SMALL ? (planes == 2 ? 5 : 3) : 4;
+}
+
+// The tile and the split of the reduction with the least estimated time.  A
+// round is as many blocks as the chip holds; a step of a round costs the larger
+// of its MFMA cycles (at the share of the dense peak that the tile size reaches)
+// and its operand bytes (at the rate L2 delivers to a CU); partials cost a
+// launch and their traffic.
 static Plan make_plan(int64_t m, int64_t n, int64_t k, int G, int planes) {
-  static const int BMs[4] = {256, 128, 64, 32}, BNs[4] = {256, 128, 64, 64};
-  Plan p;
-  auto tiles = [&](int t) {
-    return (int64_t)G * ((m + BMs[t] - 1) / BMs[t]) * ((n + BNs[t] - 1) / BNs[t]);
-  };
-  int t;
-  if (m <= 32) t = 3;
-  else if (planes == 2 && tiles(0) >= 192) t = 0;
-  else if (tiles(1) >= 192) t = 1;
-  else t = 2;
-  p.tile = t;
-  p.bm = BMs[t];
-  p.bn = BNs[t];
-  p.bk = (t == 1 && planes > 2) ? 32 : 64;
-  p.tm = (int)((m + p.bm - 1) / p.bm);
-  p.tn = (int)((n + p.bn - 1) / p.bn);
-  const int64_t total = (k + p.bk - 1) / p.bk;
-  const int64_t nt = tiles(t);
-  int64_t s = 1;
-  if (nt < 512) {
-    s = (768 + nt - 1) / nt;
-    if (s > total / 4) s = total / 4;
-    if (s > 32) s = 32;
-    if (s < 1) s = 1;
+  const int passes = planes == 6 ? 6 : planes == 2 ? 1 : DZ_PLANES;
+  const int esz = planes == 2 ? 2 : 4;
+  static const double eff[4] = {0.5, 0.35, 0.25, 0.15};
+  Plan best = {};
+  double best_t = 1e30;
+  for (int t = T_BIG; t <= T_THIN; ++t) {
+    const int bm = tile_m(planes, t), bn = tile_n(planes, t), bk = tile_k(planes, t);
+    const int occ = tile_occ(planes, t);
+    const int64_t tm = (m + bm - 1) / bm, tn = (n + bn - 1) / bn;
+    const int64_t nt = G * tm * tn, total = (k + bk - 1) / bk;
+    const double mfma = 2.0 * bm * bn * bk * passes / 4096.0 / eff[t];
+    const double mem = (double)(bm + bn) * bk * esz / 16.0;
+    for (int64_t s = 1; s <= 32 && s <= (total + 3) / 4; s = s < 4 ? s + 1 : s * 2) {
+      const int64_t steps = (total + s - 1) / s, sp = (total + steps - 1) / steps;
+      const double blocks = (double)nt * sp, slots = 256.0 * occ;
+      const double rounds = ceil(blocks / slots);
+      // blocks share their CU: a part-filled round runs as fast as its fullest CU
+      const double share = rounds > 1 ? occ : ceil(blocks / 256.0);
+      double us = rounds * ((steps + 2) * share * (mfma > mem ? mfma : mem) / 2400.0 + 1.5);
+      if (sp > 1) us += 3.0 + (sp + 1.0) * G * m * n * 4.0 / 4e6;
+      if (us < best_t) {
+        best_t = us;
+        best.tile = t;
+        best.tm = (int)tm;
+        best.tn = (int)tn;
+        best.splits = (int)sp;
+        best.steps = (int)steps;
+      }
+    }
   }
-  p.steps = (int)((total + s - 1) / s);
-  if (p.steps < 1) p.steps = 1;
-  p.splits = (int)((total + p.steps - 1) / p.steps);
-  if (p.splits < 1) p.splits = 1;
-  return p;
+  return best;
 }
 
 template <typename SA, typename SB, int PA, int PB, bool KA, bool KB, int BM, int BN, int BK, int WM,
-          int WN, int EPI, typename TO>
+          int WN, int PF, int EPI, typename TO>
 static int launch_gemm(GemmP& P, const Plan& p, hipStream_t st) {
   P.tm = p.tm;
   P.tn = p.tn;
@@ -654,11 +752,21 @@ static int launch_gemm(GemmP& P, const Plan& p, hipStream_t st) {
   P.steps = p.steps;
   const int64_t blocks = (int64_t)P.G * p.tm * p.tn * p.splits;
   if (blocks > 0x7fffffff) return (int)hipErrorInvalidValue;
-  constexpr int lds = 2 * (PA * BM + PB * BN) * BK * 2;
-  auto kern = dense_gemm<SA, SB, PA, PB, KA, KB, BM, BN, BK, WM, WN, EPI, TO>;
+  constexpr int stage = 2 * (PA * BM + PB * BN) * BK * 2;
+  constexpr int turn = WM * WN * (BM / WM < 32 ? 16 : 32) * (BN / WN + 4) * 4;   // the epilogue's
+  constexpr int lds = stage > turn ? stage : turn;
+  static_assert(lds <= 160 * 1024, "LDS of a CU");
+  auto kern = dense_gemm<SA, SB, PA, PB, KA, KB, BM, BN, BK, WM, WN, PF, EPI, TO>;
   if (lds > 64 * 1024) {
-    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
-                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    // once per device
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e == hipSuccess && !(done.load() >> (dev & 63) & 1)) {
+      e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+      if (e == hipSuccess) done.fetch_or((uint64_t)1 << (dev & 63));
+    }
     if (e != hipSuccess) return (int)e;
   }
   kern<<<(int)blocks, WM * WN * 64, lds, st>>>(P);
@@ -673,22 +781,22 @@ static int launch_gemm(GemmP& P, const Plan& p, hipStream_t st) {
 
 template <typename SA, typename SB, int PA, int PB, bool KA, bool KB, int EPI, typename TO>
 static int run_gemm(GemmP& P, const Plan& p, hipStream_t st) {
-  constexpr int BK1 = (PA + PB > 2) ? 32 : 64;
+  constexpr int PL = PA + PB;
+#define CER_TILE(T, WM, WN, PF)                                                                   \
+  launch_gemm<SA, SB, PA, PB, KA, KB, tile_m(PL, T), tile_n(PL, T), tile_k(PL, T), WM, WN, PF, EPI, \
+              TO>(P, p, st)
   switch (p.tile) {
-    case 0:
-      if constexpr (PA + PB == 2)
-        return launch_gemm<SA, SB, PA, PB, KA, KB, 256, 256, 64, 2, 4, EPI, TO>(P, p, st);
-      else
-        return (int)hipErrorInvalidValue;
-    case 1: return launch_gemm<SA, SB, PA, PB, KA, KB, 128, 128, BK1, 2, 2, EPI, TO>(P, p, st);
-    case 2: return launch_gemm<SA, SB, PA, PB, KA, KB, 64, 64, 64, 2, 2, EPI, TO>(P, p, st);
-    default: return launch_gemm<SA, SB, PA, PB, KA, KB, 32, 64, 64, 1, 4, EPI, TO>(P, p, st);
+    case T_BIG: return CER_TILE(T_BIG, (PL == 6 ? 4 : 2), (PL == 6 ? 2 : 4), 1);
+    case T_MID: return CER_TILE(T_MID, 2, 2, 1);
+    case T_SMALL: return CER_TILE(T_SMALL, 2, 2, 1);
+    default: return CER_TILE(T_THIN, 1, 4, 3);
   }
+#undef CER_TILE
 }
 
 static inline int planes_of(int kind, int is_bf16, int act) {
-  if (!is_bf16) return 4;
-  return kind == 2 && act_smooth(act) ? 3 : 2;
+  if (!is_bf16) return 6;
+  return kind == 2 && act_smooth(act) ? 1 + DZ_PLANES : 2;
 }
 
 static inline Plan plan_of(int kind, int M, int N, int K, int G, int is_bf16, int act) {
@@ -742,7 +850,7 @@ static int dense_fwd(const T* x, int64_t ldx, const T* w, int64_t ws, const T* b
   P.act = act;
   P.part = part;
   const Plan p = plan_of(0, M, N, K, G, is_bf16, act);
-  constexpr int PL = is_bf16 ? 1 : 2;
+  constexpr int PL = is_bf16 ? 1 : 3;
   return run_gemm<T, T, PL, PL, false, false, EPI_FWD, T>(P, p, st);
 }
 
@@ -783,9 +891,9 @@ static int dense_bwd(const T* dy, const void* d, void* dz, const T* x, int64_t l
     P.part = part;
     const Plan p = plan_of(2, M, N, K, G, is_bf16, act);
     if constexpr (!is_bf16)
-      rc = run_gemm<float, float, 2, 2, true, true, EPI_F32, float>(P, p, st);
+      rc = run_gemm<float, float, 3, 3, true, true, EPI_F32, float>(P, p, st);
     else if (smooth)
-      rc = run_gemm<float, bf16_t, 2, 1, true, true, EPI_F32, float>(P, p, st);
+      rc = run_gemm<float, bf16_t, DZ_PLANES, 1, true, true, EPI_F32, float>(P, p, st);
     else
       rc = run_gemm<bf16_t, bf16_t, 1, 1, true, true, EPI_F32, float>(P, p, st);
     if (rc) return rc;
@@ -799,7 +907,7 @@ static int dense_bwd(const T* dy, const void* d, void* dz, const T* x, int64_t l
   P.part = part;
   const Plan p = plan_of(1, M, N, K, G, is_bf16, act);
   if constexpr (!is_bf16)
-    return run_gemm<float, float, 2, 2, false, true, EPI_T, float>(P, p, st);
+    return run_gemm<float, float, 3, 3, false, true, EPI_T, float>(P, p, st);
   else if (smooth)
     return run_gemm<float, bf16_t, 1, 1, false, true, EPI_T, bf16_t>(P, p, st);
   else

@@ -3,8 +3,8 @@
 Tolerances are element by element.  With S = |x| |w|^T (the sum of absolute
 products) a result of T terms may be off by
 
-* fp32: 3 * 2^-16 S (two bf16 planes per factor: the rounding of each low
-  plane and the dropped low * low, 2^-16 of a product each) + T 2^-24 S,
+* fp32: (6 T + 2) 2^-24 S (three bf16 planes per factor, 2^-8 and 2^-16 of it:
+  six exact products a term in fp32 sums, the dropped ones below 2^-23),
 * bf16: T 2^-24 S (exact products, fp32 sums),
 
 plus half a step of the output's type, and through the activation times its
@@ -32,9 +32,8 @@ def _hip_backend():
     yield
 
 
-def _eps(dtype, terms, planes=2):
-    e = terms * 2.0 ** -24
-    return e + (3 * 2.0 ** -16 if dtype == torch.float32 else 0.0)
+def _eps(dtype, terms):
+    return (6 * terms + 2 if dtype == torch.float32 else terms) * 2.0 ** -24
 
 
 def _within(got, want, tol, what):
@@ -96,20 +95,18 @@ def check(G, M, K, N, dtype, act, bias=True, residual=True, train=True, grid=Fal
         dz = dys * dz1
         edz = (dys.abs() * (1.1 * ez + 2.0 ** -20 * (1 + z.abs())) + 2.0 ** -22 * dz.abs()
                if act in SMOOTH else 0 * dz)
-        # dW = dz^T x: dz enters with two planes, in bf16 mode x with one exact
-        planes = 3 * 2.0 ** -16 if dtype == torch.float32 else (
-            2.0 ** -16 if act in SMOOTH else 0.0)
+        # dW = dz^T x: in bf16 mode dz of a smooth activation has two planes
+        planes = 2.0 ** -16 if dtype == torch.bfloat16 and act in SMOOTH else 0.0
         dw, sw = dz.t() @ xs, dz.abs().t() @ xs.abs()
-        _within(w.grad()[g], dw, (planes + (M + 1) * 2.0 ** -24) * sw + edz.t() @ xs.abs()
-                + 2.0 ** -24 * dw.abs(), ("dw", g))
+        _within(w.grad()[g], dw, (planes + 2 * _eps(dtype, M + 1)) * sw
+                + (1 + 2.0 ** -8) * (edz.t() @ xs.abs()) + 2.0 ** -24 * dw.abs(), ("dw", g))
         if bias:
             db = dz.sum(0)
             _within(b.grad()[g], db, edz.sum(0) + (M + 1) * 2.0 ** -24 * dz.abs().sum(0), ("db", g))
         # dx = dz W: in bf16 mode dz of a smooth activation is rounded once
-        planes = 3 * 2.0 ** -16 if dtype == torch.float32 else (
-            2.0 ** -8 if act in SMOOTH else 0.0)
+        planes = 2.0 ** -8 if dtype == torch.bfloat16 and act in SMOOTH else 0.0
         dx, sx = dz @ ws, dz.abs() @ ws.abs()
-        ex = (planes + (N + 1) * 2.0 ** -24) * sx + 1.01 * (edz @ ws.abs())
+        ex = (planes + _eps(dtype, N + 1)) * sx + 1.01 * (edz @ ws.abs())
         _within(grads[0][:, g * K:(g + 1) * K], dx, ex + eo * (dx.abs() + ex), ("dx", g))
     if train:
         if residual:
