@@ -17,6 +17,7 @@ run as 3-pass split-bf16 MFMA GEMMs with fp32 accumulation, csrc/hip/conv.hip).
 
 import contextlib
 import ctypes
+import functools
 import os
 
 import torch
@@ -1652,60 +1653,86 @@ _RET_I64 |= {"cer_dense_ws"}
 IMPLEMENTED |= {"linear_act"}
 
 
-def _on(t):
-    """Launches inside go to ``t``'s device (and that device's current stream)."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+def _on_device(fn):
+    """``fn(t, ...)`` launches on ``t``'s device and that device's current stream."""
+    @functools.wraps(fn)
+    def call(t, *args):
+        if t.get_device() == torch.cuda.current_device():
+            return fn(t, *args)
+        with torch.cuda.device(t.device):
+            return fn(t, *args)
+    return call
 
 
-def _dense_ws(kind, M, N, K, G, x, act):
-    n = lib().cer_dense_ws(kind, M, N, K, G, int(x.dtype == torch.bfloat16), act)
-    if n < 0:
-        raise ValueError("linear_act: M={} N={} K={} G={} is beyond the kernels' 32-bit tile "
-                         "offsets".format(M, N, K, G))
-    ws = torch.empty(n, dtype=torch.float32, device=x.device) if n else None
-    return ws, n
+def _raw_stream(t):
+    """The current stream of ``t``'s device."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
+_DENSE_WS = {}      # (kind, M, N, K, G, bf16, act) -> floats of workspace
+
+
+def _dense_ws(*key):
+    n = _DENSE_WS.get(key)
+    if n is None:
+        n = lib().cer_dense_ws(*key)
+        if n < 0:
+            raise ValueError("linear_act: M={1} N={2} K={3} G={4} is beyond the kernels' 32-bit "
+                             "tile offsets".format(*key))
+        if len(_DENSE_WS) >= 4096:
+            _DENSE_WS.clear()
+        _DENSE_WS[key] = n
+    return n
+
+
+@_on_device
 def linear_act_fwd(x, wref, bref, act, residual, train):
     """x [M, G*K] (rows may be pitched) -> (y [M, G*N], act'(z) or None)."""
-    with _on(x):
-        M, G = x.shape[0], wref.G
-        N, K = wref.spec.shape
-        y = torch.empty((M, G * N), dtype=x.dtype, device=x.device)
-        d = None
-        if train and act:
-            d = torch.empty((M, G * N), dtype=torch.float32 if act > 6 else torch.uint8,
-                            device=x.device)
-        ws, n = _dense_ws(0, M, N, K, G, x, act)
-        wp, wst = wref.work_ptr()
-        bp, bst = bref.work_ptr() if bref is not None else (0, 0)
-        rc = _fn("cer_dense_fwd", x)(
-            _ptr(x), x.stride(0), c_p(wp), wst, c_p(bp), bst, _ptr(residual),
-            residual.stride(0) if residual is not None else 0, _ptr(y), _ptr(d), M, N, K, G, act,
-            _ptr(ws), n, _stream())
+    dt, dev = x.dtype, x.device
+    bf16 = dt is torch.bfloat16
+    M, G = x.shape[0], wref.arena.G
+    N, K = wref.spec.shape
+    n = _dense_ws(0, M, N, K, G, bf16, act)
+    y = torch.empty((M, G * N), dtype=dt, device=dev)
+    d = (torch.empty((M, G * N), dtype=torch.float32 if act > 6 else torch.uint8, device=dev)
+         if train and act else None)
+    ws = torch.empty(n, dtype=torch.float32, device=dev) if n else None
+    wp, wst = wref.work_ptr()
+    bp, bst = bref.work_ptr() if bref is not None else (None, 0)
+    L = lib()
+    rc = (L.cer_dense_fwd if bf16 else L.cer_dense_fwd_f32)(
+        x.data_ptr(), x.stride(0), wp, wst, bp, bst,
+        None if residual is None else residual.data_ptr(),
+        0 if residual is None else residual.stride(0), y.data_ptr(),
+        None if d is None else d.data_ptr(), M, N, K, G, act, None if ws is None else ws.data_ptr(),
+        n, _raw_stream(x))
+    if rc:
         _check(rc, "cer_dense_fwd")
     return y, d
 
 
-def linear_act_bwd(dy, d, x, wref, bref, act, need_dx):
+@_on_device
+def linear_act_bwd(x, dy, d, wref, bref, act, need_dx):
     """dx (or None); the weight and bias gradients go to the arena."""
-    with _on(x):
-        M, G = x.shape[0], wref.G
-        N, K = wref.spec.shape
-        dx = torch.empty((M, G * K), dtype=x.dtype, device=x.device) if need_dx else None
-        dz = None
-        if act:
-            dz = torch.empty((M, G * N), dtype=torch.float32 if act > 6 else x.dtype,
-                             device=x.device)
-        ws, n = _dense_ws(1, M, N, K, G, x, act)
-        wp, wst = wref.work_ptr()
-        gp, gst = wref.grad_ptr()
-        bp, bst = bref.grad_ptr() if bref is not None else (0, 0)
-        rc = _fn("cer_dense_bwd", x)(
-            _ptr(dy), _ptr(d), _ptr(dz), _ptr(x), x.stride(0), c_p(wp), wst, _ptr(dx), c_p(gp), gst,
-            c_p(bp), bst, M, N, K, G, act, _ptr(ws), n, _stream())
+    dt, dev = x.dtype, x.device
+    bf16 = dt is torch.bfloat16
+    M, G = x.shape[0], wref.arena.G
+    N, K = wref.spec.shape
+    n = _dense_ws(1, M, N, K, G, bf16, act)
+    dx = torch.empty((M, G * K), dtype=dt, device=dev) if need_dx else None
+    # one temporary: the workspace and dz (fp32 for the smooth activations)
+    nz = M * G * N if act else 0
+    tmp = torch.empty(n + nz, dtype=torch.float32, device=dev) if n + nz else None
+    tp = None if tmp is None else tmp.data_ptr()
+    wp, wst = wref.work_ptr()
+    gp, gst = wref.grad_ptr()
+    bp, bst = bref.grad_ptr() if bref is not None else (None, 0)
+    L = lib()
+    rc = (L.cer_dense_bwd if bf16 else L.cer_dense_bwd_f32)(
+        dy.data_ptr(), None if d is None else d.data_ptr(), tp + 4 * n if act else None,
+        x.data_ptr(), x.stride(0), wp, wst, None if dx is None else dx.data_ptr(), gp, gst, bp, bst,
+        M, N, K, G, act, tp if n else None, n, _raw_stream(x))
+    if rc:
         _check(rc, "cer_dense_bwd")
     return dx
 
@@ -1713,13 +1740,12 @@ def linear_act_bwd(dy, d, x, wref, bref, act, need_dx):
 # ---------------------------------------------------------------------------
 # distillation loss (csrc/hip/distill.hip), top logits (csrc/hip/toplogits.hip)
 # ---------------------------------------------------------------------------
-_TEACHER = [c_p, c_i, c_i64, c_i64, c_p, c_i64, c_i64]
+_TEACHER = [c_p, c_i, c_i64, c_i64, c_p, c_i64, c_i64, c_p, c_f, c_p, c_f]
 _SIGS.update({
     "cer_distill_ws": [c_i, c_i, c_i, c_i],
-    "cer_distill_fwd": [c_p, c_i64, c_p] + _TEACHER + [c_p, c_p, c_p, c_p, c_p, c_p, c_i, c_i, c_i,
-                                                       c_i, c_p, c_i64, c_p],
-    "cer_distill_bwd": [c_p, c_i64, c_p] + _TEACHER + [c_p, c_p, c_p, c_p, c_p, c_i, c_i, c_i, c_i,
-                                                       c_p],
+    "cer_distill_fwd": [c_p, c_i64, c_p] + _TEACHER + [c_p, c_p, c_p, c_p, c_i, c_i, c_i, c_i, c_p,
+                                                       c_i64, c_p],
+    "cer_distill_bwd": [c_p, c_i64, c_p] + _TEACHER + [c_p, c_p, c_p, c_i, c_i, c_i, c_i, c_p],
     "cer_top_ws": [c_i, c_i, c_i, c_i, c_i],
     "cer_top_logits": [c_p, c_i64, c_p, c_p, c_i, c_i, c_i, c_i, c_p, c_i64, c_p],
 })
@@ -1727,53 +1753,66 @@ _RET_I64 |= {"cer_distill_ws", "cer_top_ws"}
 IMPLEMENTED |= {"distill", "top_logits"}
 
 
-def _teacher(val, idx):
-    """Arguments of a teacher's entries [G, B, K], entries adjacent."""
-    return (_ptr(val), int(val.dtype == torch.float32), val.stride(0), val.stride(1), _ptr(idx),
-            idx.stride(0), idx.stride(1))
+def _weight(x):
+    """A per-config hyper-parameter as (device pointer or None, number)."""
+    return (x.data_ptr(), 0.0) if isinstance(x, torch.Tensor) else (None, x)
 
 
+def _teacher(val, idx, alpha, tau):
+    """Arguments of a teacher's entries [G, B, K], entries adjacent, and their weights."""
+    return (val.data_ptr(), val.dtype is torch.float32, val.stride(0), val.stride(1),
+            idx.data_ptr(), idx.stride(0), idx.stride(1)) + _weight(alpha) + _weight(tau)
+
+
+@_on_device
 def distill_fwd(logits, labels, acc, G, val, idx, alpha, tau, need_grad):
     """(loss [G], stats for ``distill_bwd``, gradient for a loss gradient of
     ones or None)."""
-    with _on(logits):
-        B, GN = logits.shape
-        N, K = GN // G, val.shape[2]
-        dev = logits.device
-        n = lib().cer_distill_ws(B, G, N, int(logits.dtype == torch.bfloat16))
-        # loss, stats and workspace in one allocation
-        buf = torch.empty(G + 4 * G * B + n, dtype=torch.float32, device=dev)
-        loss, stats, ws = buf[:G], buf[G:G + 4 * G * B], buf[G + 4 * G * B:]
-        d = torch.empty((B, GN), dtype=logits.dtype, device=dev) if need_grad else None
-        rc = _fn("cer_distill_fwd", logits)(
-            _ptr(logits), logits.stride(0), _ptr(labels), *_teacher(val, idx), _ptr(alpha),
-            _ptr(tau), _ptr(stats), _ptr(d), _ptr(loss), _ptr(acc), B, G, N, K, _ptr(ws), n,
-            _stream())
+    B, GN = logits.shape
+    dt, dev = logits.dtype, logits.device
+    bf16 = dt is torch.bfloat16
+    L = lib()
+    n = L.cer_distill_ws(B, G, GN // G, bf16)
+    loss = torch.empty(G, dtype=torch.float32, device=dev)
+    buf = torch.empty(4 * G * B + n, dtype=torch.float32, device=dev)      # stats, workspace
+    d = torch.empty((B, GN), dtype=dt, device=dev) if need_grad else None
+    p = buf.data_ptr()
+    rc = (L.cer_distill_fwd if bf16 else L.cer_distill_fwd_f32)(
+        logits.data_ptr(), logits.stride(0), labels.data_ptr(), *_teacher(val, idx, alpha, tau), p,
+        None if d is None else d.data_ptr(), loss.data_ptr(), acc.data_ptr(), B, G, GN // G,
+        val.shape[2], p + 16 * G * B, n, _raw_stream(logits))
+    if rc:
         _check(rc, "cer_distill_fwd")
-    return loss, stats, d
+    return loss, buf, d
 
 
+@_on_device
 def distill_bwd(logits, labels, G, val, idx, alpha, tau, dloss, stats):
-    with _on(logits):
-        B, GN = logits.shape
-        d = torch.empty((B, GN), dtype=logits.dtype, device=logits.device)
-        rc = _fn("cer_distill_bwd", logits)(
-            _ptr(logits), logits.stride(0), _ptr(labels), *_teacher(val, idx), _ptr(alpha),
-            _ptr(tau), _ptr(dloss), _ptr(stats), _ptr(d), B, G, GN // G, val.shape[2], _stream())
+    B, GN = logits.shape
+    d = torch.empty((B, GN), dtype=logits.dtype, device=logits.device)
+    L = lib()
+    rc = (L.cer_distill_bwd if logits.dtype is torch.bfloat16 else L.cer_distill_bwd_f32)(
+        logits.data_ptr(), logits.stride(0), labels.data_ptr(), *_teacher(val, idx, alpha, tau),
+        dloss.data_ptr(), stats.data_ptr(), d.data_ptr(), B, G, GN // G, val.shape[2],
+        _raw_stream(logits))
+    if rc:
         _check(rc, "cer_distill_bwd")
     return d
 
 
+@_on_device
 def top_logits(logits, G, k):
-    with _on(logits):
-        B, GN = logits.shape
-        N = GN // G
-        dev = logits.device
-        val = torch.empty((G, B, k), dtype=logits.dtype, device=dev)
-        idx = torch.empty((G, B, k), dtype=torch.int32, device=dev)
-        n = lib().cer_top_ws(B, G, N, k, int(logits.dtype == torch.bfloat16))
-        ws = torch.empty(n, dtype=torch.int64, device=dev) if n > 0 else None
-        rc = _fn("cer_top_logits", logits)(_ptr(logits), logits.stride(0), _ptr(val), _ptr(idx), B,
-                                           G, N, k, _ptr(ws), max(n, 0), _stream())
+    B, GN = logits.shape
+    dt, dev = logits.dtype, logits.device
+    bf16 = dt is torch.bfloat16
+    L = lib()
+    val = torch.empty((G, B, k), dtype=dt, device=dev)
+    idx = torch.empty((G, B, k), dtype=torch.int32, device=dev)
+    n = L.cer_top_ws(B, G, GN // G, k, bf16)
+    ws = torch.empty(n, dtype=torch.int64, device=dev) if n > 0 else None
+    rc = (L.cer_top_logits if bf16 else L.cer_top_logits_f32)(
+        logits.data_ptr(), logits.stride(0), val.data_ptr(), idx.data_ptr(), B, G, GN // G, k,
+        None if ws is None else ws.data_ptr(), max(n, 0), _raw_stream(logits))
+    if rc:
         _check(rc, "cer_top_logits")
     return val, idx

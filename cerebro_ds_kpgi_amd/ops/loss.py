@@ -143,7 +143,11 @@ class DistillCE(torch.autograd.Function):
                 if unit:
                     ctx.save_for_backward(d)
                 else:
-                    ctx.save_for_backward(logits, labels, val, idx, alpha, tau, stats)
+                    # alpha and tau are numbers or tensors
+                    ctx.nums = tuple(x if not isinstance(x, torch.Tensor) else None
+                                     for x in (alpha, tau))
+                    ctx.save_for_backward(logits, labels, val, idx, stats,
+                                          *(x for x in (alpha, tau) if isinstance(x, torch.Tensor)))
             return loss
         loss, d = _distill_torch(logits, labels, acc, G, val, idx, alpha, tau)
         if train:
@@ -158,7 +162,8 @@ class DistillCE(torch.autograd.Function):
             return (ctx.saved_tensors[0],) + none
         if ctx.hip:
             from . import _hip
-            logits, labels, val, idx, alpha, tau, stats = ctx.saved_tensors
+            logits, labels, val, idx, stats, *rest = ctx.saved_tensors
+            alpha, tau = (rest.pop(0) if x is None else x for x in ctx.nums)
             return (_hip.distill_bwd(logits, labels, ctx.G, val, idx, alpha, tau,
                                      dloss.contiguous(), stats),) + none
         d, = ctx.saved_tensors
@@ -174,7 +179,8 @@ def _distill_torch(logits, labels, acc, G, val, idx, alpha, tau):
     z = logits.detach().reshape(B, G, N).float()
     lab = labels.t().long()                                             # [B, G]
     v, i = val.transpose(0, 1).float(), idx.transpose(0, 1).long()      # [B, G, K]
-    a, ta = alpha.view(1, G), tau.view(1, G)
+    a, ta = (x.view(1, G) if isinstance(x, torch.Tensor) else
+             torch.full((1, G), x, dtype=torch.float32, device=z.device) for x in (alpha, tau))
     hard_on = (lab >= 0) & (a != 1)
     there = (i >= 0) & (v != -inf) & (a != 0).unsqueeze(2)
     bad = (lab >= N) | ((i >= N) & (a != 0).unsqueeze(2)).any(2)
@@ -215,15 +221,33 @@ def _distill_torch(logits, labels, acc, G, val, idx, alpha, tau):
 
 
 def _per_config(what, x, G, device, lo, hi):
-    """A hyper-parameter as an fp32 [G] tensor; numbers are range-checked."""
+    """A hyper-parameter: a range-checked number or an fp32 [G] tensor."""
     if isinstance(x, torch.Tensor):
         if tuple(x.shape) != (G,) or x.dtype != torch.float32 or x.device != device:
             raise ValueError("distill_ce: {} must be a number or an fp32 [{}] tensor on {}".format(
                 what, G, device))
-        return x.detach().contiguous()
-    if not lo <= float(x) <= hi:
+        x = x.detach() if x.requires_grad else x
+        return x if x.is_contiguous() else x.contiguous()
+    x = float(x)
+    if not lo <= x <= hi:
         raise ValueError("distill_ce: {} = {} is not in [{}, {}]".format(what, x, lo, hi))
-    return torch.full((G,), float(x), dtype=torch.float32, device=device)
+    return x
+
+
+def _refuse_teacher(G, B, dev, **tensors):
+    K = tensors["top_val"].shape[-1]
+    f32, i32 = torch.float32, torch.int32
+    for name, dt, shape in (("labels", (i32,), (G, B)), ("acc", (f32,), (G, 4)),
+                            ("top_val", (f32, torch.bfloat16), (G, B, K)),
+                            ("top_idx", (i32,), (G, B, K))):
+        t = tensors[name]
+        if tuple(t.shape) != shape or t.dtype not in dt or t.device != dev:
+            raise ValueError("distill_ce: {} is {} {} on {}, not {} {} on {}".format(
+                name, tuple(t.shape), t.dtype, t.device, shape,
+                " or ".join(str(d) for d in dt), dev))
+    if K > MAX_TOP:
+        raise ValueError("distill_ce: {} teacher entries, at most {}".format(K, MAX_TOP))
+    raise ValueError("distill_ce: acc must be contiguous")
 
 
 def distill_ce(logits, labels, acc, G, top_val, top_idx, alpha=0.5, tau=1.0, unit=False):
@@ -257,25 +281,22 @@ def distill_ce(logits, labels, acc, G, top_val, top_idx, alpha=0.5, tau=1.0, uni
         top_val = top_val.unsqueeze(0).expand(G, -1, -1)
     if top_idx.dim() == 2:
         top_idx = top_idx.unsqueeze(0).expand(G, -1, -1)
-    for name, t, dt, shape in (
-            ("labels", labels, (torch.int32,), (G, B)), ("acc", acc, (torch.float32,), (G, 4)),
-            ("top_val", top_val, (torch.float32, torch.bfloat16), (G, B, top_val.shape[-1])),
-            ("top_idx", top_idx, (torch.int32,), (G, B, top_val.shape[-1]))):
-        if tuple(t.shape) != shape or t.dtype not in dt or t.device != dev:
-            raise ValueError("distill_ce: {} is {} {} on {}, not {} {} on {}".format(
-                name, tuple(t.shape), t.dtype, t.device, shape,
-                " or ".join(str(d) for d in dt), dev))
-    if top_val.shape[2] > MAX_TOP:
-        raise ValueError("distill_ce: {} teacher entries, at most {}".format(top_val.shape[2],
-                                                                             MAX_TOP))
-    if not acc.is_contiguous():
-        raise ValueError("distill_ce: acc must be contiguous")
+    K = top_val.shape[-1]
+    if (labels.shape != (G, B) or labels.dtype is not torch.int32 or labels.device != dev
+            or acc.shape != (G, 4) or acc.dtype is not torch.float32 or acc.device != dev
+            or not acc.is_contiguous() or top_val.shape != (G, B, K)
+            or top_val.dtype not in (torch.float32, torch.bfloat16) or top_val.device != dev
+            or top_idx.shape != (G, B, K) or top_idx.dtype is not torch.int32
+            or top_idx.device != dev or K > MAX_TOP):
+        _refuse_teacher(G, B, dev, labels=labels, acc=acc, top_val=top_val, top_idx=top_idx)
     alpha = _per_config("alpha", alpha, G, dev, 0.0, 1.0)
     tau = _per_config("tau", tau, G, dev, 1e-6, 1e6)
-    if top_val.shape[2] and top_val.stride(2) != 1:
+    if K and top_val.stride(2) != 1:
         top_val = top_val.contiguous()
-    if top_idx.shape[2] and top_idx.stride(2) != 1:
+    if K and top_idx.stride(2) != 1:
         top_idx = top_idx.contiguous()
+    if top_val.requires_grad:
+        top_val = top_val.detach()
     train = torch.is_grad_enabled() and z.requires_grad
-    return DistillCE.apply(z, labels.contiguous(), acc, G, top_val.detach(), top_idx, alpha, tau,
-                           unit, train)
+    return DistillCE.apply(z, labels.contiguous(), acc, G, top_val, top_idx, alpha, tau, unit,
+                           train)

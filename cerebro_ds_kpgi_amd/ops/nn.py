@@ -787,7 +787,7 @@ class PackedLinearAct(torch.autograd.Function):
             y = y.to(x.dtype)
         if train:
             ctx.save_for_backward(x2, d)
-        return y.view(*lead, G * N)
+        return y if len(lead) == 1 else y.view(*lead, G * N)
 
     @staticmethod
     def backward(ctx, dy):
@@ -803,9 +803,11 @@ class PackedLinearAct(torch.autograd.Function):
             if bref is not None:
                 bref.grad().zero_()
             return dy.new_empty(ctx.shape) if need_dx else None, None, dr, None, None, None, None
-        dy2 = dy.contiguous().view(M, G * N)
+        dy2 = dy.contiguous()
+        if dy2.dim() != 2:
+            dy2 = dy2.view(M, G * N)
         if ctx.hip:
-            dx = _hip().linear_act_bwd(dy2, d, x2, wref, bref, ctx.act, need_dx)
+            dx = _hip().linear_act_bwd(x2, dy2, d, wref, bref, ctx.act, need_dx)
         else:
             dz = dy2.view(M, G, N).transpose(0, 1).float() * d              # [G, M, N]
             xg = x2.reshape(M, G, K).transpose(0, 1).float()                # [G, M, K]
@@ -816,7 +818,9 @@ class PackedLinearAct(torch.autograd.Function):
             if need_dx:
                 dx = torch.bmm(dz, wref.work().float())
                 dx = dx.transpose(0, 1).reshape(M, G * K).to(x2.dtype)
-        return dx.view(ctx.shape) if need_dx else None, None, dr, None, None, None, None
+        if need_dx and len(ctx.shape) != 2:
+            dx = dx.view(ctx.shape)
+        return dx, None, dr, None, None, None, None
 
 
 def _rows(t, width):
@@ -843,36 +847,51 @@ def linear_act(x, wref, bref=None, act="none", residual=None, anchor=None):
     sums), bf16 products are exact with fp32 sums, and every output is rounded
     once; act'(z) is kept in fp32 between the passes.
     """
+    code = LINEAR_ACTS.get(act)
+    arena = wref.arena
+    shape, dtype = x.shape, x.dtype
+    # one test on the way, the reasons only when it fails
+    if (code is None or len(wref.spec.shape) != 2 or dtype is not arena.compute_dtype
+            or dtype not in (torch.float32, torch.bfloat16) or not shape
+            or shape[-1] != arena.G * wref.spec.shape[1] or x.device != arena.state.device
+            or (bref is not None and (bref.arena is not arena
+                                      or bref.spec.shape != wref.spec.shape[:1]))
+            or (residual is not None
+                and (residual.shape != shape[:-1] + (arena.G * wref.spec.shape[0],)
+                     or residual.dtype is not dtype or residual.device != x.device))):
+        _refuse_linear_act(x, wref, bref, act, residual)
+    train = torch.is_grad_enabled() and (
+        x.requires_grad or (anchor is not None and anchor.requires_grad)
+        or (residual is not None and residual.requires_grad))
+    if train and arena.grad is None:
+        raise ValueError("linear_act: this arena holds no gradients (trainable=False)")
+    return PackedLinearAct.apply(x, anchor, residual, wref, bref, code, train)
+
+
+def _refuse_linear_act(x, wref, bref, act, residual):
+    arena = wref.arena
     if act not in LINEAR_ACTS:
         raise ValueError("linear_act: act {!r} is not one of {}".format(act, sorted(LINEAR_ACTS)))
-    arena = wref.arena
     if len(wref.spec.shape) != 2:
         raise ValueError("linear_act: weight {} is not [N, K]".format(wref.spec.shape))
     N, K = wref.spec.shape
-    G = wref.G
+    G = arena.G
     if x.dtype != arena.compute_dtype or x.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError("linear_act: x is {}, the arena computes in {} (fp32 and bf16 are "
                         "supported)".format(x.dtype, arena.compute_dtype))
     if x.dim() < 1 or x.shape[-1] != G * K:
         raise ValueError("linear_act: x {} does not end in G*K = {}".format(tuple(x.shape), G * K))
-    if bref is not None and (bref.arena is not arena or tuple(bref.spec.shape) != (N,)):
-        raise ValueError("linear_act: the bias must be an [{}] parameter of the weight's arena"
-                         .format(N))
     if x.device != arena.state.device:
         raise ValueError("linear_act: x is on {}, the arena on {}".format(x.device,
                                                                           arena.state.device))
-    if residual is not None:
-        if tuple(residual.shape) != tuple(x.shape[:-1]) + (G * N,):
-            raise ValueError("linear_act: residual {} is not {}".format(
-                tuple(residual.shape), tuple(x.shape[:-1]) + (G * N,)))
-        if residual.dtype != x.dtype or residual.device != x.device:
-            raise TypeError("linear_act: residual is {} on {}, x is {} on {}".format(
-                residual.dtype, residual.device, x.dtype, x.device))
-    train = torch.is_grad_enabled() and any(
-        t is not None and t.requires_grad for t in (x, anchor, residual))
-    if train and arena.grad is None:
-        raise ValueError("linear_act: this arena holds no gradients (trainable=False)")
-    return PackedLinearAct.apply(x, anchor, residual, wref, bref, LINEAR_ACTS[act], train)
+    if bref is not None and (bref.arena is not arena or tuple(bref.spec.shape) != (N,)):
+        raise ValueError("linear_act: the bias must be an [{}] parameter of the weight's arena"
+                         .format(N))
+    if tuple(residual.shape) != tuple(x.shape[:-1]) + (G * N,):
+        raise ValueError("linear_act: residual {} is not {}".format(
+            tuple(residual.shape), tuple(x.shape[:-1]) + (G * N,)))
+    raise TypeError("linear_act: residual is {} on {}, x is {} on {}".format(
+        residual.dtype, residual.device, x.dtype, x.device))
 
 
 # ---------------------------------------------------------------------------

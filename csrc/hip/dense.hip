@@ -701,18 +701,25 @@ static constexpr int tile_k(int planes, int t) {
 }
 // blocks of a CU (LDS and registers)
 static constexpr int tile_occ(int planes, int t) {
-  return t == T_BIG ? 1 : t == T_MID ? 2 : t == T_SMALL ? (planes == 2 ? 5 : 3) : 4;
+  return t == T_BIG ? 1 : t == T_MID ? 2 : t == T_SMALL ? (planes == 2 ? 4 : 3) : planes == 2 ? 3 : 2;
 }
 
 // The tile and the split of the reduction with the least estimated time.  A
-// round is as many blocks as the chip holds; a step of a round costs the larger
-// of its MFMA cycles (at the share of the dense peak that the tile size reaches)
-// and its operand bytes (at the rate L2 delivers to a CU); partials cost a
-// launch and their traffic.
-static Plan make_plan(int64_t m, int64_t n, int64_t k, int G, int planes) {
+// round is as many blocks as the chip holds.  A step of a round costs the
+// largest of its MFMA cycles (at the share of the dense peak that the tile
+// reaches), its operand bytes (at the rate a CU is fed) and the latency of a
+// step; a round also costs its start and its stores, of which blocks that share
+// a CU hide half in each other; partials cost a launch and their traffic.  The
+// constants are fitted to 240 products (1 - 16 configurations, 1 - 8192 rows, 4
+// - 8192 columns, all three forms, both types), each timed under every tile
+// and 8 splits: the choice is on average 3 % slower than the best of them,
+// against 9 % for a rule by tile count.
+static Plan choose_plan(int64_t m, int64_t n, int64_t k, int G, int planes, int out_bytes) {
   const int passes = planes == 6 ? 6 : planes == 2 ? 1 : DZ_PLANES;
   const int esz = planes == 2 ? 2 : 4;
-  static const double eff[4] = {0.5, 0.35, 0.25, 0.15};
+  static const double eff_f32[4] = {0.48, 0.31, 0.31, 0.17}, eff_bf16[4] = {0.28, 0.47, 0.37, 0.09};
+  static const double latency[4] = {0.87, 0.73, 0.61, 0.37};       // us of a step
+  const double* eff = planes == 2 ? eff_bf16 : eff_f32;
   Plan best = {};
   double best_t = 1e30;
   for (int t = T_BIG; t <= T_THIN; ++t) {
@@ -720,16 +727,20 @@ static Plan make_plan(int64_t m, int64_t n, int64_t k, int G, int planes) {
     const int occ = tile_occ(planes, t);
     const int64_t tm = (m + bm - 1) / bm, tn = (n + bn - 1) / bn;
     const int64_t nt = G * tm * tn, total = (k + bk - 1) / bk;
-    const double mfma = 2.0 * bm * bn * bk * passes / 4096.0 / eff[t];
-    const double mem = (double)(bm + bn) * bk * esz / 16.0;
-    for (int64_t s = 1; s <= 32 && s <= (total + 3) / 4; s = s < 4 ? s + 1 : s * 2) {
+    const double mfma = 2.0 * bm * bn * bk * passes / 4096.0 / eff[t] / 2400.0;
+    const double mem = (double)(bm + bn) * bk * esz / 18.0 / 2400.0;
+    for (int64_t s = 1; s <= 16 && s <= (total + 1) / 2; s = s < 4 ? s + 1 : s + s / 3) {
       const int64_t steps = (total + s - 1) / s, sp = (total + steps - 1) / steps;
-      const double blocks = (double)nt * sp, slots = 256.0 * occ;
-      const double rounds = ceil(blocks / slots);
-      // blocks share their CU: a part-filled round runs as fast as its fullest CU
+      const double blocks = (double)nt * sp;
+      const double rounds = ceil(blocks / (256.0 * occ));
+      // a part-filled round runs as fast as its fullest CU
       const double share = rounds > 1 ? occ : ceil(blocks / 256.0);
-      double us = rounds * ((steps + 2) * share * (mfma > mem ? mfma : mem) / 2400.0 + 1.5);
-      if (sp > 1) us += 3.0 + (sp + 1.0) * G * m * n * 4.0 / 4e6;
+      double step = share * (mfma > mem ? mfma : mem);
+      if (step < latency[t]) step = latency[t];
+      const double start = 3.8 + share * bm * bn * (sp > 1 ? 4 : out_bytes) / 10.0 / 2400.0;
+      double us = rounds * (steps * step + start);
+      if (occ > 1) us -= 0.55 * (rounds - 1) * (steps * step < start ? steps * step : start);
+      if (sp > 1) us += 4.6 + (sp + 1.0) * G * m * n * 4.0 / 9.8e6;
       if (us < best_t) {
         best_t = us;
         best.tile = t;
@@ -741,6 +752,26 @@ static Plan make_plan(int64_t m, int64_t n, int64_t k, int G, int planes) {
     }
   }
   return best;
+}
+
+// the last choices of this thread, by sizes (choosing takes a microsecond)
+static Plan make_plan(int64_t m, int64_t n, int64_t k, int G, int planes, int out_bytes) {
+  struct Entry {
+    int64_t key[6];
+    Plan plan;
+  };
+  static thread_local Entry memo[64];
+  const int64_t key[6] = {m, n, k, G, planes, out_bytes};
+  uint64_t h = 0;
+  for (int64_t x : key) h = (h ^ (uint64_t)x) * 0x9e3779b97f4a7c15ull;
+  Entry& e = memo[h >> 58];
+  bool hit = true;
+  for (int i = 0; i < 6; ++i) hit = hit && e.key[i] == key[i];
+  if (!hit) {
+    e.plan = choose_plan(m, n, k, G, planes, out_bytes);
+    for (int i = 0; i < 6; ++i) e.key[i] = key[i];
+  }
+  return e.plan;
 }
 
 template <typename SA, typename SB, int PA, int PB, bool KA, bool KB, int BM, int BN, int BK, int WM,
@@ -801,9 +832,10 @@ static inline int planes_of(int kind, int is_bf16, int act) {
 
 static inline Plan plan_of(int kind, int M, int N, int K, int G, int is_bf16, int act) {
   const int pl = planes_of(kind, is_bf16, act);
-  if (kind == 0) return make_plan(M, N, K, G, pl);
-  if (kind == 1) return make_plan(M, K, N, G, pl);
-  return make_plan(N, K, M, G, pl);
+  const int out = is_bf16 ? 2 : 4;
+  if (kind == 0) return make_plan(M, N, K, G, pl, out);
+  if (kind == 1) return make_plan(M, K, N, G, pl, out);
+  return make_plan(N, K, M, G, pl, 4);
 }
 
 static inline bool sizes_ok(int M, int N, int K, int G, int64_t ldx) {

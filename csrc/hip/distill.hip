@@ -34,8 +34,9 @@ struct DistP {
   int64_t val_gs, val_bs;
   const int* idx;
   int64_t idx_gs, idx_bs;
-  const float* alpha;          // [G]
-  const float* tau;
+  const float* alpha;          // [G], or null: alpha0
+  const float* tau;            // [G], or null: tau0
+  float alpha0, tau0;
   const float* dloss;          // [G] or null (ones)
   void* dz;                    // [B][G N] or null
   float* rowloss;              // [G][B]
@@ -99,8 +100,8 @@ template <int TH>
 __device__ __forceinline__ RowW teacher(const DistP& P, int g, int b, int lab, int* ti, float* tp,
                                         float* sm, float& plogp, int& nthere) {
   RowW w;
-  w.a = P.alpha[g];
-  w.tau = P.tau[g];
+  w.a = P.alpha ? P.alpha[g] : P.alpha0;
+  w.tau = P.tau ? P.tau[g] : P.tau0;
   w.itau = 1.f / w.tau;
   const int64_t v0 = g * P.val_gs + b * P.val_bs;
   const int* ix = P.idx + g * P.idx_gs + b * P.idx_bs;
@@ -341,7 +342,7 @@ __global__ __launch_bounds__(SL_TH) void distill_stats(const DistP P) {
   const int lab = P.labels[(int64_t)g * P.B + b];
   const float zl = lab >= 0 && lab < P.N ? ld1(zr + lab) : 0.f;
   float mx, s1, s2, cnt;
-  row_stats<T, SL_TH, SL_R, true>(row, lo, lab, zl, true, true, 1.f / P.tau[g], sm, mx, s1, s2, cnt);
+  row_stats<T, SL_TH, SL_R, true>(row, lo, lab, zl, true, true, 1.f / (P.tau ? P.tau[g] : P.tau0), sm, mx, s1, s2, cnt);
   if (threadIdx.x == 0) {
     float* p = P.part + (((int64_t)s * P.G + g) * P.B + b) * 4;
     p[0] = mx;
@@ -468,7 +469,7 @@ static int64_t slice_of(int N) {
 
 template <typename T>
 static bool dist_ok(const DistP& P) {
-  return P.z && P.labels && P.alpha && P.tau && P.B > 0 && P.G > 0 &&
+  return P.z && P.labels && P.B > 0 && P.G > 0 &&
          P.G <= 65535 && P.N > 0 && P.K >= 0 && P.K <= KMAX && (P.K == 0 || (P.val && P.idx)) &&
          P.ldz >= (int64_t)P.G * P.N;
 }
@@ -523,13 +524,13 @@ static int dist_fwd(DistP P, float* loss, float* acc, int64_t ws_floats, float* 
 
 static DistP dist_params(const void* z, int64_t ldz, const int* labels, const void* val,
                          int val_f32, int64_t val_gs, int64_t val_bs, const int* idx, int64_t idx_gs,
-                         int64_t idx_bs, const float* alpha, const float* tau, const float* dloss,
-                         float* stats, void* dz, int B, int G, int N, int K) {
+                         int64_t idx_bs, const float* alpha, float alpha0, const float* tau,
+                         float tau0, const float* dloss, float* stats, void* dz, int B, int G, int N, int K) {
   DistP P = {};
   P.z = z; P.ldz = ldz; P.labels = labels;
   P.val = val; P.val_f32 = val_f32; P.val_gs = val_gs; P.val_bs = val_bs;
   P.idx = idx; P.idx_gs = idx_gs; P.idx_bs = idx_bs;
-  P.alpha = alpha; P.tau = tau; P.dloss = dloss;
+  P.alpha = alpha; P.alpha0 = alpha0; P.tau = tau; P.tau0 = tau0; P.dloss = dloss;
   P.stats = stats; P.dz = dz;
   P.B = B; P.G = G; P.N = N; P.K = K;
   return P;
@@ -547,11 +548,12 @@ CER_API int64_t cer_distill_ws(int B, int G, int N, int is_bf16) {
 #define CER_DISTILL_FWD(NAME, T)                                                                  \
   CER_API int NAME(const T* z, int64_t ldz, const int* labels, const void* val, int val_f32,      \
                    int64_t val_gs, int64_t val_bs, const int* idx, int64_t idx_gs, int64_t idx_bs,                \
-                   const float* alpha, const float* tau, float* stats, T* dz, float* loss,        \
+                   const float* alpha, float alpha0, const float* tau, float tau0, float* stats,  \
+                   T* dz, float* loss,                                                            \
                    float* acc, int B, int G, int N, int K, float* ws, int64_t ws_floats,          \
                    hipStream_t st) {                                                              \
     return dist_fwd<T>(dist_params(z, ldz, labels, val, val_f32, val_gs, val_bs, idx, idx_gs, idx_bs,      \
-                                   alpha, tau, nullptr, stats, dz, B, G, N, K),                   \
+                                   alpha, alpha0, tau, tau0, nullptr, stats, dz, B, G, N, K),                   \
                        loss, acc, ws_floats, ws, st);                                             \
   }
 CER_DISTILL_FWD(cer_distill_fwd, bf16_t)
@@ -561,10 +563,11 @@ CER_DISTILL_FWD(cer_distill_fwd_f32, float)
 #define CER_DISTILL_BWD(NAME, T)                                                                  \
   CER_API int NAME(const T* z, int64_t ldz, const int* labels, const void* val, int val_f32,      \
                    int64_t val_gs, int64_t val_bs, const int* idx, int64_t idx_gs, int64_t idx_bs,                \
-                   const float* alpha, const float* tau, const float* dloss, float* stats, T* dz, \
+                   const float* alpha, float alpha0, const float* tau, float tau0,                \
+                   const float* dloss, float* stats, T* dz,                                       \
                    int B, int G, int N, int K, hipStream_t st) {                                  \
-    DistP P = dist_params(z, ldz, labels, val, val_f32, val_gs, val_bs, idx, idx_gs, idx_bs, alpha, tau,   \
-                          dloss, stats, dz, B, G, N, K);                                          \
+    DistP P = dist_params(z, ldz, labels, val, val_f32, val_gs, val_bs, idx, idx_gs, idx_bs, alpha, alpha0, \
+                          tau, tau0, dloss, stats, dz, B, G, N, K);                                          \
     if (!dist_ok<T>(P) || !stats || !dz || !dloss) return (int)hipErrorInvalidValue;              \
     return launch_grad<T>(P, st);                                                                 \
   }

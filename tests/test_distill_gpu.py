@@ -124,6 +124,19 @@ def test_alpha_of_zero_and_one():
     assert torch.isfinite(loss).all()
 
 
+@pytest.mark.parametrize("unit", [True, False])
+@pytest.mark.parametrize("N", [50, 70001])
+def test_weights_as_numbers(N, unit):
+    z, lab, val, idx, _, _ = inputs(2, 3, N, 4, device=DEV)
+    outs = []
+    for a, t in ((0.25, 2.0), (torch.full((2,), 0.25, device=DEV), 2.0),
+                 (0.25, torch.full((2,), 2.0, device=DEV))):
+        x = z.clone().requires_grad_(True)
+        loss = L.distill_ce(x, lab, torch.zeros(2, 4, device=DEV), 2, val, idx, a, t, unit=unit)
+        outs.append((loss.detach(), torch.autograd.grad(loss, [x], torch.ones(2, device=DEV))[0]))
+    assert all(torch.equal(p, q) for o in outs[1:] for p, q in zip(o, outs[0]))
+
+
 def test_layouts_and_mixed_types():
     """Pitched logits, a shared teacher, fp32 values beside bf16 logits and the
     other way round, strided entries."""
