@@ -18,6 +18,7 @@ run as 3-pass split-bf16 MFMA GEMMs with fp32 accumulation, csrc/hip/conv.hip).
 import contextlib
 import ctypes
 import functools
+import importlib.util
 import os
 
 import torch
@@ -1640,17 +1641,34 @@ def embbag_bwd(dy, idx, y, wref, bref, relu):
 
 
 # ---------------------------------------------------------------------------
-# packed dense layer with bias, activation and residual (csrc/hip/dense.hip)
+# packed dense layer with bias, activation and residual (csrc/hip/dense.hip) and
+# distillation loss (csrc/hip/distill.hip), through the autograd nodes of
+# csrc/torch/nodes.cpp; top logits (csrc/hip/toplogits.hip)
 # ---------------------------------------------------------------------------
 _SIGS.update({
-    "cer_dense_ws": [c_i, c_i, c_i, c_i, c_i, c_i, c_i],
-    "cer_dense_fwd": [c_p, c_i64, c_p, c_i64, c_p, c_i64, c_p, c_i64, c_p, c_p, c_i, c_i, c_i,
-                      c_i, c_i, c_p, c_i64, c_p],
-    "cer_dense_bwd": [c_p, c_p, c_p, c_p, c_i64, c_p, c_i64, c_p, c_p, c_i64, c_p, c_i64, c_i,
-                      c_i, c_i, c_i, c_i, c_p, c_i64, c_p],
+    "cer_top_ws": [c_i, c_i, c_i, c_i, c_i],
+    "cer_top_logits": [c_p, c_i64, c_p, c_p, c_i, c_i, c_i, c_i, c_p, c_i64, c_p],
 })
-_RET_I64 |= {"cer_dense_ws"}
-IMPLEMENTED |= {"linear_act"}
+_RET_I64 |= {"cer_top_ws"}
+IMPLEMENTED |= {"linear_act", "distill", "top_logits"}
+
+_NODES = None
+
+
+def nodes():
+    """The module of autograd nodes (``_lib/cerebro_nodes.so``)."""
+    global _NODES
+    if _NODES is None:
+        lib()                   # its entry points resolve against this
+        path = os.path.join(os.path.dirname(LIB_PATH), "cerebro_nodes.so")
+        if not os.path.exists(path):
+            raise RuntimeError("autograd nodes missing: {} (run __graft_entry__.build())"
+                               .format(path))
+        spec = importlib.util.spec_from_file_location("cerebro_nodes", path)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        _NODES = mod
+    return _NODES
 
 
 def _on_device(fn):
@@ -1667,137 +1685,6 @@ def _on_device(fn):
 def _raw_stream(t):
     """The current stream of ``t``'s device."""
     return torch._C._cuda_getCurrentRawStream(t.get_device())
-
-
-_DENSE_WS = {}      # (kind, M, N, K, G, bf16, act) -> floats of workspace
-
-
-def _dense_ws(*key):
-    n = _DENSE_WS.get(key)
-    if n is None:
-        n = lib().cer_dense_ws(*key)
-        if n < 0:
-            raise ValueError("linear_act: M={1} N={2} K={3} G={4} is beyond the kernels' 32-bit "
-                             "tile offsets".format(*key))
-        if len(_DENSE_WS) >= 4096:
-            _DENSE_WS.clear()
-        _DENSE_WS[key] = n
-    return n
-
-
-@_on_device
-def linear_act_fwd(x, wref, bref, act, residual, train):
-    """x [M, G*K] (rows may be pitched) -> (y [M, G*N], act'(z) or None)."""
-    dt, dev = x.dtype, x.device
-    bf16 = dt is torch.bfloat16
-    M, G = x.shape[0], wref.arena.G
-    N, K = wref.spec.shape
-    n = _dense_ws(0, M, N, K, G, bf16, act)
-    y = torch.empty((M, G * N), dtype=dt, device=dev)
-    d = (torch.empty((M, G * N), dtype=torch.float32 if act > 6 else torch.uint8, device=dev)
-         if train and act else None)
-    ws = torch.empty(n, dtype=torch.float32, device=dev) if n else None
-    wp, wst = wref.work_ptr()
-    bp, bst = bref.work_ptr() if bref is not None else (None, 0)
-    L = lib()
-    rc = (L.cer_dense_fwd if bf16 else L.cer_dense_fwd_f32)(
-        x.data_ptr(), x.stride(0), wp, wst, bp, bst,
-        None if residual is None else residual.data_ptr(),
-        0 if residual is None else residual.stride(0), y.data_ptr(),
-        None if d is None else d.data_ptr(), M, N, K, G, act, None if ws is None else ws.data_ptr(),
-        n, _raw_stream(x))
-    if rc:
-        _check(rc, "cer_dense_fwd")
-    return y, d
-
-
-@_on_device
-def linear_act_bwd(x, dy, d, wref, bref, act, need_dx):
-    """dx (or None); the weight and bias gradients go to the arena."""
-    dt, dev = x.dtype, x.device
-    bf16 = dt is torch.bfloat16
-    M, G = x.shape[0], wref.arena.G
-    N, K = wref.spec.shape
-    n = _dense_ws(1, M, N, K, G, bf16, act)
-    dx = torch.empty((M, G * K), dtype=dt, device=dev) if need_dx else None
-    # one temporary: the workspace and dz (fp32 for the smooth activations)
-    nz = M * G * N if act else 0
-    tmp = torch.empty(n + nz, dtype=torch.float32, device=dev) if n + nz else None
-    tp = None if tmp is None else tmp.data_ptr()
-    wp, wst = wref.work_ptr()
-    gp, gst = wref.grad_ptr()
-    bp, bst = bref.grad_ptr() if bref is not None else (None, 0)
-    L = lib()
-    rc = (L.cer_dense_bwd if bf16 else L.cer_dense_bwd_f32)(
-        dy.data_ptr(), None if d is None else d.data_ptr(), tp + 4 * n if act else None,
-        x.data_ptr(), x.stride(0), wp, wst, None if dx is None else dx.data_ptr(), gp, gst, bp, bst,
-        M, N, K, G, act, tp if n else None, n, _raw_stream(x))
-    if rc:
-        _check(rc, "cer_dense_bwd")
-    return dx
-
-
-# ---------------------------------------------------------------------------
-# distillation loss (csrc/hip/distill.hip), top logits (csrc/hip/toplogits.hip)
-# ---------------------------------------------------------------------------
-_TEACHER = [c_p, c_i, c_i64, c_i64, c_p, c_i64, c_i64, c_p, c_f, c_p, c_f]
-_SIGS.update({
-    "cer_distill_ws": [c_i, c_i, c_i, c_i],
-    "cer_distill_fwd": [c_p, c_i64, c_p] + _TEACHER + [c_p, c_p, c_p, c_p, c_i, c_i, c_i, c_i, c_p,
-                                                       c_i64, c_p],
-    "cer_distill_bwd": [c_p, c_i64, c_p] + _TEACHER + [c_p, c_p, c_p, c_i, c_i, c_i, c_i, c_p],
-    "cer_top_ws": [c_i, c_i, c_i, c_i, c_i],
-    "cer_top_logits": [c_p, c_i64, c_p, c_p, c_i, c_i, c_i, c_i, c_p, c_i64, c_p],
-})
-_RET_I64 |= {"cer_distill_ws", "cer_top_ws"}
-IMPLEMENTED |= {"distill", "top_logits"}
-
-
-def _weight(x):
-    """A per-config hyper-parameter as (device pointer or None, number)."""
-    return (x.data_ptr(), 0.0) if isinstance(x, torch.Tensor) else (None, x)
-
-
-def _teacher(val, idx, alpha, tau):
-    """Arguments of a teacher's entries [G, B, K], entries adjacent, and their weights."""
-    return (val.data_ptr(), val.dtype is torch.float32, val.stride(0), val.stride(1),
-            idx.data_ptr(), idx.stride(0), idx.stride(1)) + _weight(alpha) + _weight(tau)
-
-
-@_on_device
-def distill_fwd(logits, labels, acc, G, val, idx, alpha, tau, need_grad):
-    """(loss [G], stats for ``distill_bwd``, gradient for a loss gradient of
-    ones or None)."""
-    B, GN = logits.shape
-    dt, dev = logits.dtype, logits.device
-    bf16 = dt is torch.bfloat16
-    L = lib()
-    n = L.cer_distill_ws(B, G, GN // G, bf16)
-    loss = torch.empty(G, dtype=torch.float32, device=dev)
-    buf = torch.empty(4 * G * B + n, dtype=torch.float32, device=dev)      # stats, workspace
-    d = torch.empty((B, GN), dtype=dt, device=dev) if need_grad else None
-    p = buf.data_ptr()
-    rc = (L.cer_distill_fwd if bf16 else L.cer_distill_fwd_f32)(
-        logits.data_ptr(), logits.stride(0), labels.data_ptr(), *_teacher(val, idx, alpha, tau), p,
-        None if d is None else d.data_ptr(), loss.data_ptr(), acc.data_ptr(), B, G, GN // G,
-        val.shape[2], p + 16 * G * B, n, _raw_stream(logits))
-    if rc:
-        _check(rc, "cer_distill_fwd")
-    return loss, buf, d
-
-
-@_on_device
-def distill_bwd(logits, labels, G, val, idx, alpha, tau, dloss, stats):
-    B, GN = logits.shape
-    d = torch.empty((B, GN), dtype=logits.dtype, device=logits.device)
-    L = lib()
-    rc = (L.cer_distill_bwd if logits.dtype is torch.bfloat16 else L.cer_distill_bwd_f32)(
-        logits.data_ptr(), logits.stride(0), labels.data_ptr(), *_teacher(val, idx, alpha, tau),
-        dloss.data_ptr(), stats.data_ptr(), d.data_ptr(), B, G, GN // G, val.shape[2],
-        _raw_stream(logits))
-    if rc:
-        _check(rc, "cer_distill_bwd")
-    return d
 
 
 @_on_device

@@ -131,44 +131,21 @@ def top_logits(logits, G, k):
 
 
 class DistillCE(torch.autograd.Function):
+    """The oracle."""
+
     @staticmethod
-    def forward(ctx, logits, labels, acc, G, val, idx, alpha, tau, unit, train):
-        ctx.unit, ctx.G, ctx.shape = unit, G, logits.shape
-        ctx.hip = use_hip("distill", logits)
-        if ctx.hip:
-            from . import _hip
-            loss, stats, d = _hip.distill_fwd(logits, labels, acc, G, val, idx, alpha, tau,
-                                              train and unit)
-            if train:
-                if unit:
-                    ctx.save_for_backward(d)
-                else:
-                    # alpha and tau are numbers or tensors
-                    ctx.nums = tuple(x if not isinstance(x, torch.Tensor) else None
-                                     for x in (alpha, tau))
-                    ctx.save_for_backward(logits, labels, val, idx, stats,
-                                          *(x for x in (alpha, tau) if isinstance(x, torch.Tensor)))
-            return loss
+    def forward(ctx, logits, labels, acc, G, val, idx, alpha, tau, unit):
+        ctx.unit, ctx.G, ctx.dtype = unit, G, logits.dtype
         loss, d = _distill_torch(logits, labels, acc, G, val, idx, alpha, tau)
-        if train:
-            ctx.save_for_backward(d.to(logits.dtype) if unit else d)
-            ctx.dtype = logits.dtype
+        ctx.save_for_backward(d)
         return loss
 
     @staticmethod
     def backward(ctx, dloss):
-        none = (None,) * 9
-        if ctx.unit:                    # dloss is ones by the caller's contract
-            return (ctx.saved_tensors[0],) + none
-        if ctx.hip:
-            from . import _hip
-            logits, labels, val, idx, stats, *rest = ctx.saved_tensors
-            alpha, tau = (rest.pop(0) if x is None else x for x in ctx.nums)
-            return (_hip.distill_bwd(logits, labels, ctx.G, val, idx, alpha, tau,
-                                     dloss.contiguous(), stats),) + none
         d, = ctx.saved_tensors
-        d = d.view(d.shape[0], ctx.G, -1) * dloss.view(1, ctx.G, 1)
-        return (d.reshape(ctx.shape).to(ctx.dtype),) + none
+        if not ctx.unit:                # else dloss is ones by the caller's contract
+            d = (d.view(d.shape[0], ctx.G, -1) * dloss.view(1, ctx.G, 1)).view(d.shape)
+        return (d.to(ctx.dtype),) + (None,) * 8
 
 
 def _distill_torch(logits, labels, acc, G, val, idx, alpha, tau):
@@ -297,6 +274,11 @@ def distill_ce(logits, labels, acc, G, top_val, top_idx, alpha=0.5, tau=1.0, uni
         top_idx = top_idx.contiguous()
     if top_val.requires_grad:
         top_val = top_val.detach()
-    train = torch.is_grad_enabled() and z.requires_grad
-    return DistillCE.apply(z, labels.contiguous(), acc, G, top_val, top_idx, alpha, tau, unit,
-                           train)
+    labels = labels.contiguous()
+    if use_hip("distill", z):
+        from . import _hip
+        a, a0 = (alpha, 0.0) if isinstance(alpha, torch.Tensor) else (None, alpha)
+        t, t0 = (tau, 0.0) if isinstance(tau, torch.Tensor) else (None, tau)
+        return _hip.nodes().distill_ce(z, labels, acc, G, top_val, top_idx, a, a0, t, t0, unit,
+                                       torch.is_grad_enabled() and z.requires_grad)
+    return DistillCE.apply(z, labels, acc, G, top_val, top_idx, alpha, tau, unit)

@@ -761,76 +761,52 @@ def _act_and_grad(z, code):
 
 
 class PackedLinearAct(torch.autograd.Function):
+    """The oracle (and the way of an empty batch); x [M, G*K], residual [M, G*N]."""
+
     @staticmethod
-    def forward(ctx, x, anchor, residual, wref, bref, act, train):
-        ctx.wref, ctx.bref, ctx.act, ctx.shape = wref, bref, act, x.shape
+    def forward(ctx, x, anchor, residual, wref, bref, act):
+        ctx.wref, ctx.bref = wref, bref
         G = wref.G
         N, K = wref.spec.shape
-        lead = x.shape[:-1]
-        x2 = _rows(x, G * K)
-        r2 = _rows(residual, G * N) if residual is not None else None
-        M = x2.shape[0]
-        ctx.hip = use_hip("linear_act", x)
-        if M == 0:
-            y, d = x2.new_empty(0, G * N), None
-        elif ctx.hip:
-            y, d = _hip().linear_act_fwd(x2, wref, bref, act, r2, train)
-        else:
-            z = torch.bmm(x2.reshape(M, G, K).transpose(0, 1).float(),
-                          wref.work().float().transpose(1, 2))              # [G, M, N]
-            if bref is not None:
-                z = z + bref.work().float().unsqueeze(1)
-            y, d = _act_and_grad(z, act)
-            y = y.transpose(0, 1).reshape(M, G * N)
-            if r2 is not None:
-                y = y + r2.float()
-            y = y.to(x.dtype)
-        if train:
-            ctx.save_for_backward(x2, d)
-        return y if len(lead) == 1 else y.view(*lead, G * N)
+        M = x.shape[0]
+        z = torch.bmm(x.reshape(M, G, K).transpose(0, 1).float(),
+                      wref.work().float().transpose(1, 2))                  # [G, M, N]
+        if bref is not None:
+            z = z + bref.work().float().unsqueeze(1)
+        y, d = _act_and_grad(z, act)
+        y = y.transpose(0, 1).reshape(M, G * N)
+        if residual is not None:
+            y = y + residual.float()
+        ctx.save_for_backward(x, d)
+        return y.to(x.dtype)
 
     @staticmethod
     def backward(ctx, dy):
-        x2, d = ctx.saved_tensors
+        x, d = ctx.saved_tensors
         wref, bref = ctx.wref, ctx.bref
         G = wref.G
         N, K = wref.spec.shape
-        M = x2.shape[0]
-        need_dx, _, need_dr = ctx.needs_input_grad[:3]
-        dr = dy if need_dr else None
-        if M == 0:
-            wref.grad().zero_()
-            if bref is not None:
-                bref.grad().zero_()
-            return dy.new_empty(ctx.shape) if need_dx else None, None, dr, None, None, None, None
-        dy2 = dy.contiguous()
-        if dy2.dim() != 2:
-            dy2 = dy2.view(M, G * N)
-        if ctx.hip:
-            dx = _hip().linear_act_bwd(x2, dy2, d, wref, bref, ctx.act, need_dx)
-        else:
-            dz = dy2.view(M, G, N).transpose(0, 1).float() * d              # [G, M, N]
-            xg = x2.reshape(M, G, K).transpose(0, 1).float()                # [G, M, K]
-            wref.grad().copy_(torch.bmm(dz.transpose(1, 2), xg))
-            if bref is not None:
-                bref.grad().copy_(dz.sum(1))
-            dx = None
-            if need_dx:
-                dx = torch.bmm(dz, wref.work().float())
-                dx = dx.transpose(0, 1).reshape(M, G * K).to(x2.dtype)
-        if need_dx and len(ctx.shape) != 2:
-            dx = dx.view(ctx.shape)
-        return dx, None, dr, None, None, None, None
+        M = x.shape[0]
+        dz = dy.reshape(M, G, N).transpose(0, 1).float() * d                # [G, M, N]
+        xg = x.reshape(M, G, K).transpose(0, 1).float()                     # [G, M, K]
+        wref.grad().copy_(torch.bmm(dz.transpose(1, 2), xg))
+        if bref is not None:
+            bref.grad().copy_(dz.sum(1))
+        dx = None
+        if ctx.needs_input_grad[0]:
+            dx = torch.bmm(dz, wref.work().float())
+            dx = dx.transpose(0, 1).reshape(M, G * K).to(x.dtype)
+        return dx, None, dy if ctx.needs_input_grad[2] else None, None, None, None
 
 
 def _rows(t, width):
     """``t`` as [rows, width] with neighbouring elements of a row adjacent;
     a row pitch is kept, any other layout is copied."""
     if getattr(t, "_cer_hl", False):
-        t = _hip().hl_to_fp32(t)
+        raise ValueError("linear_act: an operand is in the HL format that only convolutions read")
     if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= width:
         return t
-    return t.contiguous().view(-1, width)
+    return t.reshape(-1, width).contiguous()
 
 
 def linear_act(x, wref, bref=None, act="none", residual=None, anchor=None):
@@ -865,7 +841,16 @@ def linear_act(x, wref, bref=None, act="none", residual=None, anchor=None):
         or (residual is not None and residual.requires_grad))
     if train and arena.grad is None:
         raise ValueError("linear_act: this arena holds no gradients (trainable=False)")
-    return PackedLinearAct.apply(x, anchor, residual, wref, bref, code, train)
+    N, K = wref.spec.shape
+    x2 = _rows(x, arena.G * K)
+    r2 = _rows(residual, arena.G * N) if residual is not None else None
+    if use_hip("linear_act", x) and x2.shape[0]:
+        y = _hip().nodes().linear_act(
+            x2, anchor, r2, arena.work, arena.grad, wref.spec.offset,
+            -1 if bref is None else bref.spec.offset, N, K, code, train)
+    else:
+        y = PackedLinearAct.apply(x2, anchor, r2, wref, bref, code)
+    return y if len(shape) == 2 else y.view(shape[:-1] + (arena.G * N,))
 
 
 def _refuse_linear_act(x, wref, bref, act, residual):

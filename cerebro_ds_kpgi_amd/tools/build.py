@@ -3,6 +3,9 @@
 * ``libcerebro_hip.so`` — every ``csrc/hip/*.hip`` compiled for gfx950 with
   hipcc (``--offload-arch=gfx950``), loaded by ``ops._hip`` through ctypes
   *after* torch so it binds to the HIP runtime torch already loaded.
+* ``cerebro_nodes.so``   — autograd nodes (``csrc/torch/*.cpp``, g++ against
+  torch's C++ headers) that call ``libcerebro_hip.so``; a Python module, loaded
+  by ``ops._hip`` after it.
 * ``libcerebro_da.so``  — the C++ Direct-Access reader / pglz codec
   (``csrc/da/*.cpp``), host-only.
 
@@ -85,8 +88,30 @@ def build_da(jobs=8):
     return _build("da", srcs, headers, out, os.environ.get("CXX", "g++"), CXX_FLAGS, [], jobs)
 
 
+def build_nodes(jobs=8):
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension as ext
+    srcs = sorted(glob.glob(os.path.join(ROOT, "csrc", "torch", "*.cpp")))
+    inc = ext.include_paths() + [sysconfig.get_paths()["include"],
+                                 os.path.join(os.path.dirname(os.path.dirname(HIPCC)), "include")]
+    flags = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+             "-D_GLIBCXX_USE_CXX11_ABI={}".format(int(torch._C._GLIBCXX_USE_CXX11_ABI))]
+    for d in inc:
+        flags += ["-isystem", d]
+    # the entry points of libcerebro_hip.so stay open: ops._hip has loaded it
+    link = ["-L" + d for d in ext.library_paths()] + ["-lc10", "-lc10_hip", "-ltorch_cpu",
+                                                      "-ltorch", "-ltorch_python"]
+    out = os.path.join(LIBDIR, "cerebro_nodes.so")
+    return _build("nodes", srcs, [], out, os.environ.get("CXX", "g++"), flags, link, jobs)
+
+
 def build_all(jobs=8):
-    return build_hip(jobs), build_da(jobs)
+    with cf.ThreadPoolExecutor(max_workers=1) as ex:      # beside the HIP sources
+        nodes = ex.submit(build_nodes, jobs)
+        built = build_hip(jobs), build_da(jobs)
+        nodes.result()
+    return built
 
 
 if __name__ == "__main__":

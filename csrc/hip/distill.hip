@@ -48,7 +48,15 @@ struct DistP {
 
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// sums of two / three values over the block
+// 2^(k (z - m)); the difference first: a row (or slice) of the type's lowest
+// value has m k beyond the type
+struct Expo {
+  float k, m;
+  __device__ __forceinline__ Expo(float k_, float m_) : k(k_), m(m_) {}
+  __device__ __forceinline__ float operator()(float z) const { return ex2((z - m) * k); }
+};
+
+// sums of three values over the block
 template <int TH>
 __device__ __forceinline__ void block_sum3(float& a, float& b, float& c, float* sm) {
   a = warp_sum(a);
@@ -176,10 +184,12 @@ __device__ __forceinline__ void row_result(const DistP& P, int g, int b, int lab
   P.rowhit[o] = (lb && cnt < 1.f ? 1 : 0) | ((P.N > 2 ? (lb && cnt < 5.f) : true) ? 2 : 0);
 }
 
-// coefficients of a row's gradient
+// coefficients of a row's gradient: before the entries it is
+// sgn (2^((z - mx) k + o1) + 2^((z - mx) k2 + o2)), the factors c / sum in the
+// exponents
 struct GradW {
-  float mx, k2, c1, c2, ch, cs;   // dz = c1 exp(z - mx) + c2 exp((z - mx) / tau) - entries
-  bool hard, soft;
+  float mx, k2, o1, o2, sgn, ch, cs;
+  bool hard, soft, one;
 };
 
 __device__ __forceinline__ GradW grad_weights(const DistP& P, const RowW& w, int g, float mx,
@@ -189,21 +199,32 @@ __device__ __forceinline__ GradW grad_weights(const DistP& P, const RowW& w, int
   if (w.bad) sc = NAN;
   q.hard = w.hard || w.bad;
   q.soft = w.soft;
-  q.mx = mx;
   q.k2 = LOG2E * w.itau;
   q.ch = (1.f - w.a) * sc;
   q.cs = w.a * w.tau * sc;
-  q.c1 = q.ch / s1;
-  q.c2 = q.cs / s2;
+  q.sgn = sc < 0.f ? -1.f : 1.f;
+  q.mx = mx;
+  q.o1 = __log2f(q.ch * q.sgn / s1);
+  q.o2 = __log2f(q.cs * q.sgn / s2);
+  // at tau = 1 both terms have one exponential
+  q.one = q.hard && q.soft && w.tau == 1.f;
+  if (q.one) q.o1 = __log2f((q.ch + q.cs) * q.sgn / s1);
   return q;
 }
 
-__device__ __forceinline__ float grad_base(const GradW& q, float z) {
+template <bool HARD, bool SOFT>
+__device__ __forceinline__ float grad_of(const GradW& q, float z) {
   const float x = z - q.mx;
   float d = 0.f;
-  if (q.hard) d = q.c1 * ex2(x * LOG2E);
-  if (q.soft) d = fmaf(q.c2, ex2(x * q.k2), d);
+  if (HARD) d = ex2(fmaf(x, LOG2E, q.o1));
+  if (SOFT) d = HARD ? d + ex2(fmaf(x, q.k2, q.o2)) : ex2(fmaf(x, q.k2, q.o2));
   return d;
+}
+
+__device__ __forceinline__ float grad_base(const GradW& q, float z) {
+  const float d = q.hard ? (q.soft && !q.one ? grad_of<true, true>(q, z) : grad_of<true, false>(q, z))
+                         : (q.soft ? grad_of<false, true>(q, z) : 0.f);
+  return d * q.sgn;
 }
 
 // The label's and the teacher's classes in [lo, hi): written whole, after the
@@ -232,64 +253,86 @@ __device__ __forceinline__ void grad_entries(const DistP& P, const GradW& q, con
 // the gradient's rows need not have the logits' alignment
 typedef uint32_t u32x4_a __attribute__((ext_vector_type(4), aligned(2)));
 
-template <typename T, int TH, int R>
-__device__ __forceinline__ void grad_row(RowRegs<T, TH, R>& row, const GradW& q, T* dr) {
+template <typename T, int TH, int R, typename F>
+__device__ __forceinline__ void write_row(const RowRegs<T, TH, R>& row, T* dr, F f) {
   constexpr int V = RowRegs<T, TH, R>::V;
-  #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int i = threadIdx.x + r * TH;
-    if (i < row.nv) {
-      uint32_t w[4];
-      const uint4 u = row.fresh(r);
+  row.vecs(threadIdx.x, [&](int r, int, const float* z) {
+    uint32_t w[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if constexpr (V == 4) {
-          w[e] = __float_as_uint(grad_base(q, row.get(u, e)));
-        } else {
-          w[e] = cvt_pk_bf16(grad_base(q, row.get(u, 2 * e)), grad_base(q, row.get(u, 2 * e + 1)));
-        }
-      }
-      *reinterpret_cast<u32x4_a*>(dr + row.head + (int64_t)i * V) = u32x4_a{w[0], w[1], w[2], w[3]};
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (V == 4) w[e] = __float_as_uint(f(z[e]));
+      else w[e] = cvt_pk_bf16(f(z[2 * e]), f(z[2 * e + 1]));
     }
-  }
-  if (row.ej >= 0) st1(dr + row.ej, grad_base(q, row.edge));
+    const int i = threadIdx.x + r * TH;
+    if (i < row.nv)
+      *reinterpret_cast<u32x4_a*>(dr + row.head + (int64_t)i * V) = u32x4_a{w[0], w[1], w[2], w[3]};
+  });
+  if (row.ej >= 0) st1(dr + row.ej, f(row.edge));
+}
+
+template <typename T, int TH, int R>
+__device__ __forceinline__ void grad_row(const RowRegs<T, TH, R>& row, const GradW& q, T* dr) {
+  if (!q.hard && !q.soft)
+    write_row(row, dr, [&](float) { return 0.f; });
+  else if (q.sgn < 0.f)          // a negative loss gradient
+    write_row(row, dr, [&](float z) { return grad_base(q, z); });
+  else if (q.hard && q.soft && !q.one)
+    write_row(row, dr, [&](float z) { return grad_of<true, true>(q, z); });
+  else if (q.hard)
+    write_row(row, dr, [&](float z) { return grad_of<true, false>(q, z); });
+  else
+    write_row(row, dr, [&](float z) { return grad_of<false, true>(q, z); });
 }
 
 // maximum, both sums and the label's rank of the elements in `row`, which
 // start at class j0 of the logits row; all threads get them.  A whole row of
 // -inf has sums of NaN, a SLICE of nothing but -inf sums of zero.
 template <typename T, int TH, int R, bool SLICE>
-__device__ __forceinline__ void row_stats(RowRegs<T, TH, R>& row, int j0, int lab, float zl,
+__device__ __forceinline__ void row_stats(const RowRegs<T, TH, R>& row, int j0, int lab, float zl,
                                           bool hard, bool soft, float itau, float* sm, float& mx,
                                           float& s1, float& s2, float& cnt) {
-  float m = -INFINITY;
-  row.each(threadIdx.x, [&](int, float z) { m = fmaxf(m, z); });
-  mx = block_max1<TH>(m, sm);
-  s1 = s2 = cnt = 0.f;
-  const float k2 = LOG2E * itau, mm = SLICE && mx == -INFINITY ? 0.f : mx;
-  if (hard) row.each(threadIdx.x, [&](int, float z) { s1 += ex2((z - mm) * LOG2E); });
-  if (soft) row.each(threadIdx.x, [&](int, float z) { s2 += ex2((z - mm) * k2); });
+  constexpr int V = RowRegs<T, TH, R>::V;
+  float m = row.edge;
+  int before = 0;
   if (lab >= 0) {
-    // how many come before the label: counted a wave at a time in scalar
-    // registers; equal values are rare and looked at only where there are any
+    // the maximum, and how many come before the label: counted a wave at a time
+    // in scalar registers; equal values are rare and looked at only where there
+    // are any
     const int l = lab - j0;
-    int before = 0;
-    row.vecs(threadIdx.x, [&](int j, const float* z) {
+    row.vecs(threadIdx.x, [&](int, int j, const float* z) {
       uint64_t eq = 0;
 #pragma unroll
-      for (int e = 0; e < RowRegs<T, TH, R>::V; ++e) {
+      for (int e = 0; e < V; ++e) {
+        m = fmaxf(m, z[e]);
         before += __popcll(__ballot(z[e] > zl));
         eq |= __ballot(z[e] == zl);
       }
       if (eq) {
 #pragma unroll
-        for (int e = 0; e < RowRegs<T, TH, R>::V; ++e)
+        for (int e = 0; e < V; ++e)
           before += __popcll(__ballot((z[e] == zl) & (j + e < l)));
       }
     });
     const int je = row.ej >= 0 ? row.ej : 0x7fffffff;
     before += __popcll(__ballot((row.edge > zl) | ((row.edge == zl) & (je < l))));
-    if ((threadIdx.x & 63) == 0) cnt = (float)before;
+  } else {
+    row.each(threadIdx.x, [&](int, float z) { m = fmaxf(m, z); });
+  }
+  mx = block_max1<TH>(m, sm);
+  s1 = s2 = 0.f;
+  cnt = (threadIdx.x & 63) == 0 ? (float)before : 0.f;
+  const float mm = SLICE && mx == -INFINITY ? 0.f : mx;
+  const Expo q1(LOG2E, mm), q2(LOG2E * itau, mm);
+  if (hard && soft && itau != 1.f) {
+    row.each(threadIdx.x, [&](int, float z) {
+      s1 += q1(z);
+      s2 += q2(z);
+    });
+  } else if (hard || itau == 1.f) {
+    row.each(threadIdx.x, [&](int, float z) { s1 += q1(z); });
+    s2 = s1;                     // used where the soft term is there: tau is 1 then
+  } else if (soft) {
+    row.each(threadIdx.x, [&](int, float z) { s2 += q2(z); });
   }
   block_sum3<TH>(s1, s2, cnt, sm);
 }

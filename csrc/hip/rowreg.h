@@ -35,42 +35,48 @@ struct RowRegs {
     edge = ej >= 0 ? ld1(p + ej) : -INFINITY;
   }
 
-  static __device__ __forceinline__ float get(const uint4& u, int e) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-    if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
-    else return __uint_as_float((e & 1) ? (w[e >> 1] & 0xffff0000u) : (w[e >> 1] << 16));
-  }
-
-  // vector r as if just loaded: the compiler otherwise keeps unpacked or
-  // half-computed values of the whole row from one pass to the next
-  __device__ __forceinline__ uint4 fresh(int r) {
-    asm volatile("" : "+v"(v[r].x), "+v"(v[r].y), "+v"(v[r].z), "+v"(v[r].w));
-    return v[r];
-  }
+  // Unpacks the vectors of one pass over the row.  The shift and the mask are
+  // opaque to the compiler, which would otherwise keep every bf16 of the row
+  // unpacked, in twice the registers, from one pass to the next.
+  struct Unpack {
+    uint32_t shift, mask;
+    __device__ __forceinline__ Unpack() {
+      if constexpr (sizeof(T) == 2) {
+        asm volatile("s_mov_b32 %0, 16" : "=s"(shift));
+        asm volatile("s_mov_b32 %0, 0xffff0000" : "=s"(mask));
+      }
+    }
+    __device__ __forceinline__ float operator()(const uint4& u, int e) const {
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+      if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
+      else return __uint_as_float((e & 1) ? (w[e >> 1] & mask) : (w[e >> 1] << shift));
+    }
+  };
 
   // f(element, value) over this thread's slots; slots past the row have value
   // -inf and an element number beyond every row's
   template <typename F>
-  __device__ __forceinline__ void each(int tid, F f) {
-    vecs(tid, [&](int j, const float* z) {
+  __device__ __forceinline__ void each(int tid, F f) const {
+    vecs(tid, [&](int, int j, const float* z) {
 #pragma unroll
       for (int e = 0; e < V; ++e) f(j + e, z[e]);
     });
     f(ej >= 0 ? ej : 0x7fffffff, edge);
   }
 
-  // f(first element, V values) over this thread's vectors
+  // f(r, first element, V values) over this thread's vectors
   template <typename F>
-  __device__ __forceinline__ void vecs(int tid, F f) {
+  __device__ __forceinline__ void vecs(int tid, F f) const {
+    const Unpack get;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
+      if (r > 0 && r * TH >= nv) break;           // the same for all threads
       const int i = tid + r * TH;
       const int j = i < nv ? head + i * V : 0x7ffffff0;
-      const uint4 u = fresh(r);
       float z[V];
 #pragma unroll
-      for (int e = 0; e < V; ++e) z[e] = get(u, e);
-      f(j, z);
+      for (int e = 0; e < V; ++e) z[e] = get(v[r], e);
+      f(r, j, z);
     }
   }
 };

@@ -16,20 +16,20 @@
 //
 // What bounds it: the one read of the logits.  Rows longer than a block's
 // registers, and long rows that are too few to fill the chip, are cut into
-// chunks; the chunks' lists are merged.
+// chunks; a chunk hands on its candidates unordered (or its K largest, if those
+// are too many) and top_merge selects among them in the same way.
 #include "rowreg.h"
 
 constexpr int TOP_KMAX = 1024;
 constexpr int TOP_CAND = 4096;       // candidates in LDS
-constexpr int TOP_MERGE = 8192;      // numbers a merging block sorts
 
 struct TopP {
   const void* z;
   int64_t ldz;
   void* val;             // [G][B][K]
   int* idx;
-  uint64_t* list;        // chunked: [rows][chunks][K]
-  int B, G, N, K, chunks, chunk;
+  uint64_t* list;        // chunked: [rows][chunks][room]
+  int B, G, N, K, chunks, chunk, room;
 };
 
 __device__ __forceinline__ uint32_t key_of(float z) {
@@ -69,18 +69,32 @@ __device__ __forceinline__ void bitonic(uint64_t* s, int n) {
 // The C numbers in s (room for the next power of two, above 512) in descending
 // order to out(rank, number) for rank < K.
 template <int TH, typename F>
-__device__ __forceinline__ void ordered(uint64_t* s, int C, int K, F out) {
+__device__ __forceinline__ void ordered(uint64_t* s, int* rk, int C, int K, F out) {
   if (C <= 512) {
-    // few: every number counts the larger ones
-    const int c2 = (C + 1) & ~1;
-    if (threadIdx.x == 0 && c2 > C) s[C] = 0;
+    // few: every number counts the larger ones; several threads share a number
+    const int ce = (C + 1) & ~1;
+    if (threadIdx.x == 0 && ce > C) s[C] = 0;
+    int cp = 64;
+    while (cp < C) cp <<= 1;
+    if (cp > TH) cp = TH;
+    const int parts = TH / cp;
+    for (int i = threadIdx.x; i < C; i += TH) rk[i] = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < C; i += TH) {
+    const int part = threadIdx.x / cp, len = (ce / 2 + parts - 1) / parts * 2;
+    const int c0 = part * len, c1 = min(ce, c0 + len);
+    for (int i = threadIdx.x & (cp - 1); i < C; i += cp) {
       const uint64_t me = s[i];
-      int rank = 0;
-      for (int c = 0; c < c2; c += 2) rank += (s[c] > me ? 1 : 0) + (s[c + 1] > me ? 1 : 0);
-      if (rank < K) out(rank, me);
+      int larger = 0;
+#pragma unroll 4
+      for (int c = c0; c < c1; c += 2) {
+        const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(s + c);
+        larger += (x.x > me ? 1 : 0) + (x.y > me ? 1 : 0);
+      }
+      atomicAdd(&rk[i], larger);
     }
+    __syncthreads();
+    for (int i = threadIdx.x; i < C; i += TH)
+      if (rk[i] < K) out(rk[i], s[i]);
     return;
   }
   int n = 1024;
@@ -90,12 +104,27 @@ __device__ __forceinline__ void ordered(uint64_t* s, int C, int K, F out) {
   for (int i = threadIdx.x; i < K; i += TH) out(i, s[i]);
 }
 
-// Radix search of a row for its K-th largest number, 8 bits at a time from the
-// top, until what reaches the prefix fits `room`; those go to cand.  Reads the
-// row from memory (one of the last levels of cache has it).
-template <typename T, int TH>
-__device__ __noinline__ int radix_candidates(const T* zr, int n, int lo, int K, uint64_t* cand,
-                                             int room, int* hist, int* count) {
+// a lower bound (upper 20 bits) of the kw-th largest of a wave's 64 * GR keys
+template <int GR>
+__device__ __forceinline__ uint32_t wave_bound(const uint32_t* mk, int kw) {
+  uint32_t t = 0;
+  if (kw <= 64 * GR) {
+    for (int bit = 31; bit >= 12; --bit) {
+      const uint32_t c = t | (1u << bit);
+      int reach = 0;
+#pragma unroll
+      for (int q = 0; q < GR; ++q) reach += __popcll(__ballot(mk[q] >= c));
+      if (reach >= kw) t = c;
+    }
+  }
+  return t;
+}
+
+// Radix search for the K-th largest of number(0 .. n), 8 bits at a time from the
+// top, until what reaches the prefix fits `room`; those go to cand.
+template <int TH, typename F>
+__device__ __noinline__ int radix_candidates(F number, int n, int K, uint64_t* cand, int room,
+                                             int* hist, int* count) {
   const int tid = threadIdx.x;
   uint64_t prefix = 0;
   int above = 0;                       // elements above the prefix
@@ -104,7 +133,7 @@ __device__ __noinline__ int radix_candidates(const T* zr, int n, int lo, int K, 
     for (int i = tid; i < 256; i += TH) hist[i] = 0;
     __syncthreads();
     for (int j = tid; j < n; j += TH) {
-      const uint64_t x = number_of(ld1(zr + j), lo + j);
+      const uint64_t x = number(j);
       if (sh == 56 || (x >> (sh + 8)) == (prefix >> (sh + 8)))
         atomicAdd(&hist[(int)(x >> sh) & 255], 1);
     }
@@ -141,7 +170,7 @@ __device__ __noinline__ int radix_candidates(const T* zr, int n, int lo, int K, 
   if (tid == 0) *count = 0;
   __syncthreads();
   for (int j = tid; j < n; j += TH) {
-    const uint64_t x = number_of(ld1(zr + j), lo + j);
+    const uint64_t x = number(j);
     if (x >= prefix) cand[atomicAdd(count, 1)] = x;
   }
   __syncthreads();
@@ -157,7 +186,7 @@ __global__ __launch_bounds__(TH) void top_rows(const TopP P) {
   constexpr int ROOM = CAP <= 512 ? 514 : (CAP < TOP_CAND ? CAP : TOP_CAND);
   __shared__ __attribute__((aligned(16))) uint64_t cand[ROOM];
   __shared__ uint32_t bound[16];
-  __shared__ int hist[CAP > TOP_CAND ? 256 : 1], count, nanflag;
+  __shared__ int hist[CAP > TOP_CAND ? 256 : 1], rk[512], count, nanflag;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int row = blockIdx.x / P.chunks, ch = blockIdx.x - row * P.chunks;
   const int g = row / P.B, b = row - g * P.B;
@@ -179,18 +208,15 @@ __global__ __launch_bounds__(TH) void top_rows(const TopP P) {
   for (int q = 0; q < GR; ++q) m[q] = -INFINITY;
   bool nan = regs.edge != regs.edge;
   m[0] = fmaxf(m[0], regs.edge);
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const uint4 u = regs.fresh(r);
+  regs.vecs(tid, [&](int r, int, const float* z) {
     float t = -INFINITY;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const float z = regs.get(u, e);
-      nan |= z != z;
-      t = fmaxf(t, z);
+      nan |= z[e] != z[e];
+      t = fmaxf(t, z[e]);
     }
     m[r % GR] = fmaxf(m[r % GR], t);
-  }
+  });
   if (__ballot(nan) && lane == 0) nanflag = 1;
   if (GR > 1 && kw <= 16) {
 #pragma unroll
@@ -202,17 +228,7 @@ __global__ __launch_bounds__(TH) void top_rows(const TopP P) {
   uint32_t mk[GR];
 #pragma unroll
   for (int q = 0; q < GR; ++q) mk[q] = key_of(m[q]);
-  // this wave's kw-th largest maximum, its upper 20 bits
-  uint32_t t = 0;
-  if (kw <= 64 * GR) {
-    for (int bit = 31; bit >= 12; --bit) {
-      const uint32_t c = t | (1u << bit);
-      int reach = 0;
-#pragma unroll
-      for (int q = 0; q < GR; ++q) reach += __popcll(__ballot(mk[q] >= c));
-      if (reach >= kw) t = c;
-    }
-  }
+  const uint32_t t = wave_bound<GR>(mk, kw);
   if (lane == 0) bound[wave] = t;
   __syncthreads();
   uint32_t lim = bound[0];
@@ -229,7 +245,7 @@ __global__ __launch_bounds__(TH) void top_rows(const TopP P) {
         if (at < ROOM) cand[at] = number_of(z, lo + j);
       }
     };
-    regs.vecs(tid, [&](int j, const float* z) {
+    regs.vecs(tid, [&](int, int j, const float* z) {
       bool any = false;
 #pragma unroll
       for (int e = 0; e < V; ++e) any |= !(z[e] < fl);
@@ -243,50 +259,79 @@ __global__ __launch_bounds__(TH) void top_rows(const TopP P) {
     C = count;
   }
   if constexpr (CAP > TOP_CAND) {
-    if (C > ROOM) C = radix_candidates<T, TH>(zr, n, lo, K, cand, ROOM, hist, &count);
+    // from memory: one of the last levels of cache has the row
+    if (C > ROOM)
+      C = radix_candidates<TH>([=](int j) { return number_of(ld1(zr + j), lo + j); }, n, K, cand,
+                               ROOM, hist, &count);
   }
   if (P.chunks == 1) {
     T* val = reinterpret_cast<T*>(P.val) + (int64_t)row * P.K;
     int* idx = P.idx + (int64_t)row * P.K;
-    ordered<TH>(cand, C, K, [&](int k, uint64_t x) {
+    ordered<TH>(cand, rk, C, K, [&](int k, uint64_t x) {
       const int j = (int)~(uint32_t)x;
       idx[k] = j;
       val[k] = zr[j];
     });
   } else {
-    uint64_t* out = P.list + (int64_t)blockIdx.x * P.K;
-    ordered<TH>(cand, C, K, [&](int k, uint64_t x) { out[k] = x; });
-    for (int k = K + tid; k < P.K; k += TH) out[k] = 0;     // a last chunk shorter than K
+    uint64_t* out = P.list + (int64_t)blockIdx.x * P.room;
+    int filled = C;
+    if (C <= P.room) {
+      for (int k = tid; k < C; k += TH) out[k] = cand[k];
+    } else {
+      ordered<TH>(cand, rk, C, K, [&](int k, uint64_t x) { out[k] = x; });
+      filled = K;
+    }
+    for (int k = filled + tid; k < P.room; k += TH) out[k] = 0;
   }
 }
 
-// `per` lists of K numbers into one; the last merge writes the result
-template <typename T, int TH>
-__global__ __launch_bounds__(TH) void top_merge(const TopP P, const uint64_t* __restrict__ in,
-                                                uint64_t* __restrict__ out, int lists, int per,
-                                                int last) {
-  extern __shared__ __attribute__((aligned(16))) uint64_t s[];
-  const int groups = (lists + per - 1) / per;
-  const int row = blockIdx.x / groups, gr = blockIdx.x - row * groups;
-  const int l0 = gr * per, nl = min(per, lists - l0);
-  const int C = nl * P.K;
-  int n = 2;
-  while (n < C) n <<= 1;
-  const uint64_t* src = in + ((int64_t)row * lists + l0) * P.K;
-  for (int i = threadIdx.x; i < n; i += TH) s[i] = i < C ? src[i] : 0;
-  bitonic<TH>(s, n);
-  if (!last) {
-    uint64_t* o = out + ((int64_t)row * groups + gr) * P.K;
-    for (int k = threadIdx.x; k < P.K; k += TH) o[k] = s[k];
-    return;
+// the chunks' lists of a row (zeros are no entries) to its result
+constexpr int TM_TH = 1024;
+template <typename T>
+__global__ __launch_bounds__(TM_TH) void top_merge(const TopP P) {
+  constexpr int W = TM_TH / 64, GR = 4;
+  __shared__ __attribute__((aligned(16))) uint64_t cand[TOP_CAND];
+  __shared__ uint32_t bound[W];
+  __shared__ int hist[256], rk[512], count;
+  const int tid = threadIdx.x, row = blockIdx.x;
+  const int n = P.chunks * P.room, K = P.K, kw = (K + W - 1) / W;
+  const uint64_t* src = P.list + (int64_t)row * n;
+  if (tid == 0) count = 0;
+  uint32_t mk[GR] = {0, 0, 0, 0};
+  for (int i = tid; i < n; i += GR * TM_TH) {
+#pragma unroll
+    for (int q = 0; q < GR; ++q) {
+      const int j = i + q * TM_TH;
+      if (j < n) mk[q] = max(mk[q], (uint32_t)(src[j] >> 32));
+    }
   }
+  const uint32_t t = wave_bound<GR>(mk, kw);
+  if ((tid & 63) == 0) bound[tid >> 6] = t;
+  __syncthreads();
+  uint32_t lim = bound[0];
+#pragma unroll
+  for (int w = 1; w < W; ++w) lim = min(lim, bound[w]);
+  if (lim == 0) lim = 1;                       // zeros stay out
+  for (int i = tid; i < n; i += TM_TH) {
+    const uint64_t x = src[i];
+    if ((uint32_t)(x >> 32) >= lim) {
+      const int at = atomicAdd(&count, 1);
+      if (at < TOP_CAND) cand[at] = x;
+    }
+  }
+  __syncthreads();
+  int C = count;
+  if (C > TOP_CAND)
+    C = radix_candidates<TM_TH>([=](int j) { return src[j]; }, n, K, cand, TOP_CAND, hist, &count);
   const int g = row / P.B, b = row - g * P.B;
   const T* zr = reinterpret_cast<const T*>(P.z) + (int64_t)b * P.ldz + (int64_t)g * P.N;
-  for (int k = threadIdx.x; k < P.K; k += TH) {
-    const int j = (int)~(uint32_t)s[k];
-    P.idx[(int64_t)row * P.K + k] = j;
-    reinterpret_cast<T*>(P.val)[(int64_t)row * P.K + k] = zr[j];
-  }
+  T* val = reinterpret_cast<T*>(P.val) + (int64_t)row * K;
+  int* idx = P.idx + (int64_t)row * K;
+  ordered<TM_TH>(cand, rk, C, K, [&](int k, uint64_t x) {
+    const int j = (int)~(uint32_t)x;
+    idx[k] = j;
+    val[k] = zr[j];
+  });
 }
 
 template <typename T>
@@ -295,7 +340,8 @@ static int top_chunk(int64_t rows, int N, int K) {
   int c = N;
   if (N > 1024 * 16 * V) c = 1024 * 16 * V;
   // few rows: shorter chunks put more of the chip to work
-  if (rows < 128 && N > 256 * 8 * V) c = 256 * 8 * V;
+  const int few = K <= 256 ? 256 * 8 * V : 512 * 16 * V;
+  if (rows < 128 && N > few && few < c) c = few;
   return c;
 }
 
@@ -303,6 +349,8 @@ static inline bool top_sizes(int B, int G, int N, int K) {
   return B > 0 && G > 0 && N > 0 && N < 0x7ffffff0 && K > 0 && K <= N && K <= TOP_KMAX &&
          (int64_t)B * G <= 0x7fffffff;
 }
+
+static inline int top_room(int K) { return K < 32 ? 64 : 2 * K; }
 
 // 64-bit numbers of workspace, -1 for sizes out of range
 template <typename T>
@@ -312,7 +360,7 @@ static int64_t top_ws(int B, int G, int N, int K) {
   const int c = top_chunk<T>(rows, N, K);
   const int64_t chunks = (N + c - 1) / c;
   if (rows * chunks > 0x7fffffff) return -1;
-  return chunks > 1 ? 2 * rows * chunks * K : 0;
+  return chunks > 1 ? rows * chunks * top_room(K) : 0;
 }
 
 CER_API int64_t cer_top_ws(int B, int G, int N, int K, int is_bf16) {
@@ -332,6 +380,7 @@ static int top_launch(const T* z, int64_t ldz, T* val, int* idx, int B, int G, i
   P.chunk = top_chunk<T>(rows, N, K);
   P.chunks = (N + P.chunk - 1) / P.chunk;
   P.list = ws;
+  P.room = top_room(K);
   const int grid = (int)(rows * P.chunks);
   const int n = P.chunk;
   constexpr int V = 16 / (int)sizeof(T);
@@ -342,25 +391,7 @@ static int top_launch(const T* z, int64_t ldz, T* val, int* idx, int B, int G, i
   else if (n <= 512 * 8 * V) top_rows<T, 512, 8><<<grid, 512, 0, st>>>(P);
   else if (n <= 512 * 16 * V) top_rows<T, 512, 16><<<grid, 512, 0, st>>>(P);
   else top_rows<T, 1024, 16><<<grid, 1024, 0, st>>>(P);
-  if (P.chunks > 1) {
-    int per = TOP_MERGE / K;
-    const uint64_t* in = ws;
-    uint64_t* out = ws + rows * P.chunks * K;
-    int lists = P.chunks;
-    while (true) {
-      const int groups = (lists + per - 1) / per;
-      const int nl = lists < per ? lists : per;
-      int p2 = 2;
-      while (p2 < nl * K) p2 <<= 1;
-      const int last = groups == 1;
-      top_merge<T, 512><<<(int)(rows * groups), 512, p2 * 8, st>>>(P, in, out, lists, per, last);
-      if (last) break;
-      lists = groups;
-      uint64_t* t = const_cast<uint64_t*>(in);
-      in = out;
-      out = t;
-    }
-  }
+  if (P.chunks > 1) top_merge<T><<<(int)rows, TM_TH, 0, st>>>(P);
   return (int)hipGetLastError();
 }
 

@@ -54,6 +54,7 @@ def test_masked_classes_and_extremes(dtype, N, unit):
     zz[:, :, N // 2:N // 2 + N // 4] = torch.finfo(dtype).min
     zz[:, :, -(N // 4):] = -math.inf
     zz[2] *= 1000
+    zz[3] = torch.finfo(dtype).min                # nothing but the lowest value
     lab.clamp_(max=N // 2 - 1)
     idx = idx % (N // 2)
     val[0, 0, 0] = -math.inf                      # an entry that is none
@@ -107,6 +108,23 @@ def test_every_entry_the_same_class(dtype):
     idx[:] = 11
     lab[0] = 11
     check(2, 4, 30, 9, dtype, device=DEV, args=(z, lab, val, idx, alpha, tau))
+
+
+@pytest.mark.parametrize("N", [30, 5000, 70001])
+@DTYPES
+def test_negative_and_zero_loss_gradients_and_tau_of_one(dtype, N):
+    z, lab, val, idx, alpha, tau = inputs(3, 6, N, 5, dtype, device=DEV)
+    tau = torch.tensor([1.0, 2.0, 1.0], device=DEV)
+    dloss = torch.tensor([-2.0, 0.0, 0.7], device=DEV)
+    x = z.clone().requires_grad_(True)
+    loss = L.distill_ce(x, lab, torch.zeros(3, 4, device=DEV), 3, val, idx, alpha, tau)
+    d, = torch.autograd.grad(loss, [x], dloss)
+    _, _, want, mag = reference(z, lab, val, idx, alpha, tau, dloss)
+    half = 2.0 ** -24 if dtype == torch.float32 else 2.0 ** -8
+    tol = 2.0 ** -20 * 40 * mag
+    tol = tol + half * (want.abs() + tol) + 1e-30
+    assert ((d.double() - want).abs() <= tol).all()
+    check(3, 6, N, 5, dtype, True, device=DEV, args=(z, lab, val, idx, alpha, tau))
 
 
 def test_alpha_of_zero_and_one():

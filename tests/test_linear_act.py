@@ -91,6 +91,10 @@ def test_refusals():
         P.linear_act(x, w, w)
     with pytest.raises(ValueError, match="\\[N, K\\]"):
         P.linear_act(x, b)
+    hl = x.clone()
+    hl._cer_hl = True
+    with pytest.raises(ValueError, match="HL"):
+        P.linear_act(hl, w, b)
     _, w2, b2 = make(trainable=False)
     with pytest.raises(ValueError, match="no gradients"):
         P.linear_act(x.clone().requires_grad_(True), w2, b2)
