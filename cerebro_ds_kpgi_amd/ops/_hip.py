@@ -17,7 +17,6 @@ run as 3-pass split-bf16 MFMA GEMMs with fp32 accumulation, csrc/hip/conv.hip).
 
 import contextlib
 import ctypes
-import functools
 import importlib.util
 import os
 
@@ -1642,21 +1641,17 @@ def embbag_bwd(dy, idx, y, wref, bref, relu):
 
 # ---------------------------------------------------------------------------
 # packed dense layer with bias, activation and residual (csrc/hip/dense.hip) and
-# distillation loss (csrc/hip/distill.hip), through the autograd nodes of
-# csrc/torch/nodes.cpp; top logits (csrc/hip/toplogits.hip)
+# distillation loss (csrc/hip/distill.hip), top logits (csrc/hip/toplogits.hip):
+# called by csrc/torch/nodes.cpp, which holds their autograd nodes
 # ---------------------------------------------------------------------------
-_SIGS.update({
-    "cer_top_ws": [c_i, c_i, c_i, c_i, c_i],
-    "cer_top_logits": [c_p, c_i64, c_p, c_p, c_i, c_i, c_i, c_i, c_p, c_i64, c_p],
-})
-_RET_I64 |= {"cer_top_ws"}
 IMPLEMENTED |= {"linear_act", "distill", "top_logits"}
 
 _NODES = None
 
 
 def nodes():
-    """The module of autograd nodes (``_lib/cerebro_nodes.so``)."""
+    """The module with linear_act, distill_ce and top_logits
+    (``_lib/cerebro_nodes.so``); arguments are checked by ``ops.nn`` / ``ops.loss``."""
     global _NODES
     if _NODES is None:
         lib()                   # its entry points resolve against this
@@ -1669,37 +1664,3 @@ def nodes():
         spec.loader.exec_module(mod)
         _NODES = mod
     return _NODES
-
-
-def _on_device(fn):
-    """``fn(t, ...)`` launches on ``t``'s device and that device's current stream."""
-    @functools.wraps(fn)
-    def call(t, *args):
-        if t.get_device() == torch.cuda.current_device():
-            return fn(t, *args)
-        with torch.cuda.device(t.device):
-            return fn(t, *args)
-    return call
-
-
-def _raw_stream(t):
-    """The current stream of ``t``'s device."""
-    return torch._C._cuda_getCurrentRawStream(t.get_device())
-
-
-@_on_device
-def top_logits(logits, G, k):
-    B, GN = logits.shape
-    dt, dev = logits.dtype, logits.device
-    bf16 = dt is torch.bfloat16
-    L = lib()
-    val = torch.empty((G, B, k), dtype=dt, device=dev)
-    idx = torch.empty((G, B, k), dtype=torch.int32, device=dev)
-    n = L.cer_top_ws(B, G, GN // G, k, bf16)
-    ws = torch.empty(n, dtype=torch.int64, device=dev) if n > 0 else None
-    rc = (L.cer_top_logits if bf16 else L.cer_top_logits_f32)(
-        logits.data_ptr(), logits.stride(0), val.data_ptr(), idx.data_ptr(), B, G, GN // G, k,
-        None if ws is None else ws.data_ptr(), max(n, 0), _raw_stream(logits))
-    if rc:
-        _check(rc, "cer_top_logits")
-    return val, idx

@@ -120,12 +120,14 @@ def top_logits(logits, G, k):
     class number (+0 equals -0, NaN counts as largest); 1 <= k <= min(N, 1024).
     No gradient: this is what a teacher hands to ``distill_ce``.
     """
-    z, N = _logit_rows("top_logits", logits.detach(), G)
+    if logits.requires_grad:
+        logits = logits.detach()
+    z, N = _logit_rows("top_logits", logits, G)
     if not 1 <= k <= min(N, MAX_TOP):
         raise ValueError("top_logits: k = {} is not in 1 .. min(N = {}, {})".format(k, N, MAX_TOP))
     if use_hip("top_logits", z):
         from . import _hip
-        return _hip.top_logits(z, G, k)
+        return _hip.nodes().top_logits(z, G, k)
     v, i = torch.sort(z.reshape(-1, G, N).transpose(0, 1), dim=2, descending=True, stable=True)
     return v[:, :, :k].contiguous(), i[:, :, :k].to(torch.int32)
 

@@ -498,14 +498,20 @@ static int64_t slice_of(int N) {
   return N <= RowRegs<T, 1024, 16>::CAP ? 0 : RowRegs<T, SL_TH, SL_R>::CAP;
 }
 
-// blocks for a row of N: calls f(threads, vectors)
+// Threads and vectors of the block for a row of N.  Few waves with long rows
+// rather than many with short ones: the row's reductions are barriers, and
+// blocks of 256 leave several of them on a CU (8192 x 16000 bf16: 512 x 8 253 us,
+// 256 x 8 150 us; 4096 x 30000: 512 x 8 186 us, 256 x 16 141 us; 4096 x 49999:
+// 512 x 16 251 us, 256 x 26 229 us).
 #define CER_ROW_DISPATCH(T, N, LAUNCH)                  \
   do {                                                  \
     constexpr int V_ = 16 / sizeof(T);                  \
     if ((N) <= 64 * V_) LAUNCH(64, 1);                  \
     else if ((N) <= 256 * V_) LAUNCH(256, 1);           \
-    else if ((N) <= 256 * 4 * V_) LAUNCH(256, 4);       \
-    else if ((N) <= 512 * 8 * V_) LAUNCH(512, 8);       \
+    else if ((N) <= 256 * 3 * V_) LAUNCH(256, 3);       \
+    else if ((N) <= 256 * 8 * V_) LAUNCH(256, 8);       \
+    else if ((N) <= 256 * 16 * V_) LAUNCH(256, 16);     \
+    else if ((N) <= 256 * 26 * V_) LAUNCH(256, 26);     \
     else if ((N) <= 512 * 16 * V_) LAUNCH(512, 16);     \
     else LAUNCH(1024, 16);                              \
   } while (0)

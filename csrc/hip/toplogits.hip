@@ -21,7 +21,7 @@
 #include "rowreg.h"
 
 constexpr int TOP_KMAX = 1024;
-constexpr int TOP_CAND = 4096;       // candidates in LDS
+constexpr int TOP_CAND = 4096;       // most candidates in LDS
 
 struct TopP {
   const void* z;
@@ -30,6 +30,7 @@ struct TopP {
   int* idx;
   uint64_t* list;        // chunked: [rows][chunks][room]
   int B, G, N, K, chunks, chunk, room;
+  int cand;              // candidates in LDS
 };
 
 __device__ __forceinline__ uint32_t key_of(float z) {
@@ -104,12 +105,12 @@ __device__ __forceinline__ void ordered(uint64_t* s, int* rk, int C, int K, F ou
   for (int i = threadIdx.x; i < K; i += TH) out(i, s[i]);
 }
 
-// a lower bound (upper 20 bits) of the kw-th largest of a wave's 64 * GR keys
+// a lower bound (upper 16 bits: all of a bf16) of the kw-th largest of a wave's 64 * GR keys
 template <int GR>
 __device__ __forceinline__ uint32_t wave_bound(const uint32_t* mk, int kw) {
   uint32_t t = 0;
   if (kw <= 64 * GR) {
-    for (int bit = 31; bit >= 12; --bit) {
+    for (int bit = 31; bit >= 16; --bit) {
       const uint32_t c = t | (1u << bit);
       int reach = 0;
 #pragma unroll
@@ -181,12 +182,10 @@ template <typename T, int TH, int R>
 __global__ __launch_bounds__(TH) void top_rows(const TopP P) {
   constexpr int W = TH / 64, V = RowRegs<T, TH, R>::V, CAP = RowRegs<T, TH, R>::CAP;
   constexpr int GR = R >= 4 ? 4 : 1;          // maxima a thread keeps for larger K
-  // candidates: a short row fits whole (up to 512 are ranked, which needs one
-  // more place; above that the size is a power of two for the sort)
-  constexpr int ROOM = CAP <= 512 ? 514 : (CAP < TOP_CAND ? CAP : TOP_CAND);
-  __shared__ __attribute__((aligned(16))) uint64_t cand[ROOM];
+  constexpr bool SHORT = CAP <= 512;          // the whole row fits: no search is ever needed
+  extern __shared__ __attribute__((aligned(16))) uint64_t cand[];
   __shared__ uint32_t bound[16];
-  __shared__ int hist[CAP > TOP_CAND ? 256 : 1], rk[512], count, nanflag;
+  __shared__ int hist[SHORT ? 1 : 256], rk[512], count, nanflag;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int row = blockIdx.x / P.chunks, ch = blockIdx.x - row * P.chunks;
   const int g = row / P.B, b = row - g * P.B;
@@ -235,14 +234,14 @@ __global__ __launch_bounds__(TH) void top_rows(const TopP P) {
 #pragma unroll
   for (int w = 1; w < W; ++w) lim = min(lim, bound[w]);
   const bool has_nan = nanflag != 0;
-  int C = ROOM + 1;
-  if (!has_nan || CAP <= TOP_CAND) {
+  int C = P.cand + 1;
+  if (!has_nan || SHORT) {
     // a bound below -inf's key takes every element; so does a short row with NaN
     const float fl = has_nan || lim <= 0x007fffffu ? -INFINITY : key_value(lim);
     auto push = [&](int j, float z) {
       if (!(z < fl) && j < n) {
         const int at = atomicAdd(&count, 1);
-        if (at < ROOM) cand[at] = number_of(z, lo + j);
+        if (at < P.cand) cand[at] = number_of(z, lo + j);
       }
     };
     regs.vecs(tid, [&](int, int j, const float* z) {
@@ -258,11 +257,11 @@ __global__ __launch_bounds__(TH) void top_rows(const TopP P) {
     __syncthreads();
     C = count;
   }
-  if constexpr (CAP > TOP_CAND) {
+  if constexpr (!SHORT) {
     // from memory: one of the last levels of cache has the row
-    if (C > ROOM)
+    if (C > P.cand)
       C = radix_candidates<TH>([=](int j) { return number_of(ld1(zr + j), lo + j); }, n, K, cand,
-                               ROOM, hist, &count);
+                               P.cand, hist, &count);
   }
   if (P.chunks == 1) {
     T* val = reinterpret_cast<T*>(P.val) + (int64_t)row * P.K;
@@ -384,13 +383,18 @@ static int top_launch(const T* z, int64_t ldz, T* val, int* idx, int B, int G, i
   const int grid = (int)(rows * P.chunks);
   const int n = P.chunk;
   constexpr int V = 16 / (int)sizeof(T);
-  if (n <= 64 * V) top_rows<T, 64, 1><<<grid, 64, 0, st>>>(P);
-  else if (n <= 256 * V) top_rows<T, 256, 1><<<grid, 256, 0, st>>>(P);
-  else if (n <= 256 * 4 * V) top_rows<T, 256, 4><<<grid, 256, 0, st>>>(P);
-  else if (n <= 256 * 8 * V) top_rows<T, 256, 8><<<grid, 256, 0, st>>>(P);
-  else if (n <= 512 * 8 * V) top_rows<T, 512, 8><<<grid, 512, 0, st>>>(P);
-  else if (n <= 512 * 16 * V) top_rows<T, 512, 16><<<grid, 512, 0, st>>>(P);
-  else top_rows<T, 1024, 16><<<grid, 1024, 0, st>>>(P);
+  // room for a multiple of K, a power of two above 512 for the sort (a short row
+  // is ranked and takes one place more); little LDS leaves more blocks on a CU
+  P.cand = n <= 64 * V ? 514 : K <= 256 ? 1024 : TOP_CAND;
+#define CER_TOP(TH, R) top_rows<T, TH, R><<<grid, TH, P.cand * sizeof(uint64_t), st>>>(P)
+  if (n <= 64 * V) CER_TOP(64, 1);
+  else if (n <= 256 * V) CER_TOP(256, 1);
+  else if (n <= 256 * 4 * V) CER_TOP(256, 4);
+  else if (n <= 256 * 8 * V) CER_TOP(256, 8);
+  else if (n <= 512 * 8 * V) CER_TOP(512, 8);
+  else if (n <= 512 * 16 * V) CER_TOP(512, 16);
+  else CER_TOP(1024, 16);
+#undef CER_TOP
   if (P.chunks > 1) top_merge<T><<<(int)rows, TM_TH, 0, st>>>(P);
   return (int)hipGetLastError();
 }

@@ -1,4 +1,5 @@
-// Autograd nodes of linear_act and distill_ce (ops.nn, ops.loss).
+// Autograd nodes of linear_act and distill_ce, and the call of top_logits
+// (ops.nn, ops.loss).
 //
 // The kernels of both take tens of microseconds at the sizes of a classifier's
 // head.  As Python autograd functions their host path took longer than that: the
@@ -40,6 +41,12 @@ extern "C" {
            int64_t val_gs, int64_t val_bs, const int* idx, int64_t idx_gs, int64_t idx_bs,        \
            const float* alpha, float alpha0, const float* tau, float tau0, const float* dloss,    \
            float* stats, void* dz, int B, int G, int N, int K, void* st);
+#define TOP_LOGITS(NAME)                                                                          \
+  int NAME(const void* z, int64_t ldz, void* val, int* idx, int B, int G, int N, int K,           \
+           int64_t* ws, int64_t ws_n, void* st);
+TOP_LOGITS(cer_top_logits)
+TOP_LOGITS(cer_top_logits_f32)
+int64_t cer_top_ws(int B, int G, int N, int K, int is_bf16);
 DENSE_FWD(cer_dense_fwd)
 DENSE_FWD(cer_dense_fwd_f32)
 DENSE_BWD(cer_dense_bwd)
@@ -54,6 +61,11 @@ int64_t cer_distill_ws(int B, int G, int N, int is_bf16);
 
 static void* stream_of(const Tensor& t) {
   return c10::hip::getCurrentHIPStream(t.device().index()).stream();
+}
+
+// row counts go to the kernels as int
+static void rows_fit(const char* name, int64_t rows) {
+  TORCH_CHECK_VALUE(rows <= INT32_MAX, name, ": ", rows, " rows are more than 2^31 - 1");
 }
 
 static void done(int rc, const char* name) {
@@ -119,6 +131,7 @@ static Tensor linear_act(const Tensor& x, const std::optional<Tensor>& anchor,
                          const std::optional<Tensor>& residual, const Tensor& work,
                          const std::optional<Tensor>& grad, int64_t w_off, int64_t b_off, int64_t N,
                          int64_t K, int64_t act, bool train) {
+  rows_fit("linear_act", x.size(0));
   const c10::OptionalDeviceGuard guard(x.device());
   Dense p{work, grad.value_or(Tensor()), w_off, b_off, x.size(0), N, K, work.size(0), act,
           x.scalar_type() == at::kBFloat16};
@@ -195,6 +208,7 @@ static Tensor distill_ce(const Tensor& z, const Tensor& labels, const Tensor& ac
                          const Tensor& val, const Tensor& idx, const std::optional<Tensor>& alpha,
                          double alpha0, const std::optional<Tensor>& tau, double tau0, bool unit,
                          bool train) {
+  rows_fit("distill_ce", z.size(0));
   const c10::OptionalDeviceGuard guard(z.device());
   const bool bf16 = z.scalar_type() == at::kBFloat16;
   const int64_t B = z.size(0), N = z.size(1) / G;
@@ -227,7 +241,25 @@ static Tensor distill_ce(const Tensor& z, const Tensor& labels, const Tensor& ac
   return loss;
 }
 
+// ---------------------------------------------------------------------------
+static std::tuple<Tensor, Tensor> top_logits(const Tensor& z, int64_t G, int64_t k) {
+  rows_fit("top_logits", z.size(0) * G);
+  const c10::OptionalDeviceGuard guard(z.device());
+  const bool bf16 = z.scalar_type() == at::kBFloat16;
+  const int64_t B = z.size(0), N = z.size(1) / G;
+  Tensor val = at::empty({G, B, k}, z.options());
+  Tensor idx = at::empty({G, B, k}, z.options().dtype(at::kInt));
+  const int64_t n = cer_top_ws(B, G, N, k, bf16);
+  Tensor ws = n > 0 ? at::empty({n}, z.options().dtype(at::kLong)) : Tensor();
+  done((bf16 ? cer_top_logits : cer_top_logits_f32)(
+           z.data_ptr(), z.stride(0), val.data_ptr(), idx.data_ptr<int>(), B, G, N, k,
+           ws.defined() ? ws.data_ptr<int64_t>() : nullptr, n > 0 ? n : 0, stream_of(z)),
+       "cer_top_logits");
+  return {val, idx};
+}
+
 PYBIND11_MODULE(cerebro_nodes, m) {
+  m.def("top_logits", &top_logits);
   m.def("linear_act", &linear_act);
   m.def("distill_ce", &distill_ce);
 }
