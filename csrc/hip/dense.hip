@@ -24,8 +24,8 @@
 // 2^-24 of |x||w| a term, so the result is that of an fp32 product (measured
 // against 64 bits: as near as the library's) at 6/16 of the time of fp32 MFMA.
 // In bf16 mode dz = dy * act'(z) has more than 8 bits: it is kept in fp32,
-// enters dW as DZ_PLANES planes (dW is an fp32 tensor) and dx as one (dx is
-// rounded to bf16 anyway).  A non-finite fp32 factor gives a non-finite result,
+// enters dW as DZ_PLANES planes (dW is an fp32 tensor) and dx rounded to bf16 (as
+// dx itself is).  A non-finite fp32 factor gives a non-finite result,
 // NaN where a single fp32 product would give an infinity; |x| above 3.39e38
 // rounds to infinity.
 #include <atomic>
@@ -653,12 +653,13 @@ __global__ __launch_bounds__(256) void dense_join(const GemmP P) {
 // ---------------------------------------------------------------------------
 constexpr int DA_COLS = 64, DA_ROWS = 128;
 
-// D: 0 none (dz is dy, only db is made), 1 u8 mask, 2 fp32 derivative
+// D: 0 none (dz is dy, only db is made), 1 u8 mask, 2 fp32 derivative.  dzr (or
+// null): dz rounded to bf16, the operand of dx; dW takes the fp32 one.
 template <typename T, int D, typename TZ>
 __global__ __launch_bounds__(256) void dense_dact(const T* __restrict__ dy, const void* __restrict__ d,
-                                                  TZ* __restrict__ dz, float* __restrict__ db,
-                                                  int64_t db_gs, float* __restrict__ part, int M,
-                                                  int C, int N) {
+                                                  TZ* __restrict__ dz, bf16_t* __restrict__ dzr,
+                                                  float* __restrict__ db, int64_t db_gs,
+                                                  float* __restrict__ part, int M, int C, int N) {
   __shared__ float sm[4][DA_COLS];
   const int c = blockIdx.x * DA_COLS + (threadIdx.x & 63), w = threadIdx.x >> 6;
   const int r0 = blockIdx.y * DA_ROWS, r1 = min(M, r0 + DA_ROWS);
@@ -671,6 +672,7 @@ __global__ __launch_bounds__(256) void dense_dact(const T* __restrict__ dy, cons
       if constexpr (D == 1) v = reinterpret_cast<const uint8_t*>(d)[i] ? v : 0.f;
       if constexpr (D == 2) v *= reinterpret_cast<const float*>(d)[i];
       if constexpr (D != 0) st1(dz + i, v);
+      if constexpr (D == 2 && sizeof(T) == 2) dzr[i] = f2bf(v);
       s += v;
     }
   }
@@ -729,17 +731,17 @@ static constexpr int tile_occ(int planes, int t) {
 // round is as many blocks as the chip holds.  A step of a round costs the
 // largest of its MFMA cycles (at the share of the dense peak that the tile
 // reaches), its operand bytes (at the rate a CU is fed) and the latency of a
-// step; a round also costs its start and its stores, of which blocks that share
-// a CU hide half in each other; partials cost a launch and their traffic.  The
-// constants are fitted to 240 products (1 - 16 configurations, 1 - 8192 rows, 4
-// - 8192 columns, all three forms, both types), each timed under every tile
-// and 8 splits: the choice is on average 3 % slower than the best of them,
-// against 9 % for a rule by tile count.
+// step; a round also costs its start and its stores, which blocks that share a
+// CU hide in each other; partials cost a launch and their traffic.  The
+// constants are fitted to 282 products (1 - 16 configurations, 1 - 16384 rows, 2
+// - 8192 columns, all three forms, both types), each timed under every tile and
+// up to 8 splits: the choice is on average 2 % slower than the best of them,
+// against 9 % for the constants that a first guess gave.
 static Plan choose_plan(int64_t m, int64_t n, int64_t k, int G, int planes, int out_bytes) {
   const int passes = planes == 6 ? 6 : planes == 2 ? 1 : DZ_PLANES;
   const int esz = planes == 2 ? 2 : 4;
-  static const double eff_f32[4] = {0.48, 0.31, 0.31, 0.17}, eff_bf16[4] = {0.28, 0.47, 0.37, 0.09};
-  static const double latency[4] = {0.87, 0.73, 0.61, 0.37};       // us of a step
+  static const double eff_f32[4] = {0.56, 0.33, 0.33, 0.17}, eff_bf16[4] = {0.40, 0.43, 0.19, 0.09};
+  static const double latency[4] = {0.76, 0.69, 0.60, 0.35};       // us of a step
   const double* eff = planes == 2 ? eff_bf16 : eff_f32;
   Plan best = {};
   double best_t = 1e30;
@@ -749,7 +751,7 @@ static Plan choose_plan(int64_t m, int64_t n, int64_t k, int G, int planes, int 
     const int64_t tm = (m + bm - 1) / bm, tn = (n + bn - 1) / bn;
     const int64_t nt = G * tm * tn, total = (k + bk - 1) / bk;
     const double mfma = 2.0 * bm * bn * bk * passes / 4096.0 / eff[t] / 2400.0;
-    const double mem = (double)(bm + bn) * bk * esz / 18.0 / 2400.0;
+    const double mem = (double)(bm + bn) * bk * esz / 23.0 / 2400.0;
     for (int64_t s = 1; s <= 16 && s <= (total + 1) / 2; s = s < 4 ? s + 1 : s + s / 3) {
       const int64_t steps = (total + s - 1) / s, sp = (total + steps - 1) / steps;
       const double blocks = (double)nt * sp;
@@ -758,10 +760,11 @@ static Plan choose_plan(int64_t m, int64_t n, int64_t k, int G, int planes, int 
       const double share = rounds > 1 ? occ : ceil(blocks / 256.0);
       double step = share * (mfma > mem ? mfma : mem);
       if (step < latency[t]) step = latency[t];
-      const double start = 3.8 + share * bm * bn * (sp > 1 ? 4 : out_bytes) / 10.0 / 2400.0;
-      double us = rounds * (steps * step + start);
-      if (occ > 1) us -= 0.55 * (rounds - 1) * (steps * step < start ? steps * step : start);
-      if (sp > 1) us += 4.6 + (sp + 1.0) * G * m * n * 4.0 / 9.8e6;
+      const double run = steps * step + 3.9;
+      const double store = share * bm * bn * (sp > 1 ? 4 : out_bytes) / 9.4 / 2400.0;
+      const double hide = occ > 1 && rounds > 1 ? 0.9 : 0.0;
+      double us = rounds * (run + store - hide * (run < store ? run : store));
+      if (sp > 1) us += 4.1 + (sp + 1.0) * G * m * n * 4.0 / 7.7e6;
       if (us < best_t) {
         best_t = us;
         best.tile = t;
@@ -908,8 +911,9 @@ static int dense_fwd(const T* x, int64_t ldx, const T* w, int64_t ws, const T* b
 }
 
 // gradients: dx (or null) [M][G K], dW -> gw (fp32, config stride gs),
-// db -> gb (or null).  d: act'(z) of the forward; dz: scratch [M][G N] (fp32
-// for the smooth activations, else T; unused for act none).
+// db -> gb (or null).  d: act'(z) of the forward; dz: scratch [M][G N] (T for
+// relu / relu6; fp32 for the smooth activations, and in bf16 mode [M][G N] bf16
+// behind it; unused for act none).
 template <typename T>
 static int dense_bwd(const T* dy, const void* d, void* dz, const T* x, int64_t ldx, const T* w,
                      int64_t ws, T* dx, float* gw, int64_t gs, float* gb, int64_t gbs, int M, int N,
@@ -921,15 +925,16 @@ static int dense_bwd(const T* dy, const void* d, void* dz, const T* x, int64_t l
   if (part_floats < cer_dense_ws(1, M, N, K, G, is_bf16, act)) return (int)hipErrorInvalidValue;
   const int C = G * N;
   const bool smooth = act_smooth(act);
+  bf16_t* dzr = is_bf16 && smooth ? (bf16_t*)((float*)dz + (int64_t)M * C) : nullptr;
   if (act != ACT_NONE || gb) {
     const dim3 grid((C + DA_COLS - 1) / DA_COLS, (M + DA_ROWS - 1) / DA_ROWS);
     if (grid.y > 65535) return (int)hipErrorInvalidValue;
     if (act == ACT_NONE)
-      dense_dact<T, 0, T><<<grid, 256, 0, st>>>(dy, nullptr, nullptr, gb, gbs, part, M, C, N);
+      dense_dact<T, 0, T><<<grid, 256, 0, st>>>(dy, nullptr, nullptr, nullptr, gb, gbs, part, M, C, N);
     else if (smooth)
-      dense_dact<T, 2, float><<<grid, 256, 0, st>>>(dy, d, (float*)dz, gb, gbs, part, M, C, N);
+      dense_dact<T, 2, float><<<grid, 256, 0, st>>>(dy, d, (float*)dz, dzr, gb, gbs, part, M, C, N);
     else
-      dense_dact<T, 1, T><<<grid, 256, 0, st>>>(dy, d, (T*)dz, gb, gbs, part, M, C, N);
+      dense_dact<T, 1, T><<<grid, 256, 0, st>>>(dy, d, (T*)dz, nullptr, gb, gbs, part, M, C, N);
     if (gb && grid.y > 1)
       dense_dbsum<<<grid.x, 256, 0, st>>>(part, grid.y, gb, gbs, C, N);
   }
@@ -953,18 +958,14 @@ static int dense_bwd(const T* dy, const void* d, void* dz, const T* x, int64_t l
   }
   if (!dx) return 0;
   GemmP P = {};
-  P.a = z; P.lda = C; P.a_gs = N;
+  P.a = dzr ? dzr : z; P.lda = C; P.a_gs = N;
   P.b = w; P.ldb = K; P.b_gs = ws;
   P.m = M; P.n = K; P.k = N; P.G = G;
   P.c = dx; P.ldc = (int64_t)G * K; P.c_gs = K;
   P.part = part;
   const Plan p = plan_of(1, M, N, K, G, is_bf16, act);
-  if constexpr (!is_bf16)
-    return run_gemm<float, float, 3, 3, false, true, EPI_T, float>(P, p, st);
-  else if (smooth)
-    return run_gemm<float, bf16_t, 1, 1, false, true, EPI_T, bf16_t>(P, p, st);
-  else
-    return run_gemm<bf16_t, bf16_t, 1, 1, false, true, EPI_T, bf16_t>(P, p, st);
+  constexpr int PL = is_bf16 ? 1 : 3;
+  return run_gemm<T, T, PL, PL, false, true, EPI_T, T>(P, p, st);
 }
 
 CER_API int cer_dense_fwd(const bf16_t* x, int64_t ldx, const bf16_t* w, int64_t ws,
