@@ -651,7 +651,9 @@ __global__ __launch_bounds__(256) void dense_join(const GemmP P) {
 // range of rows; the partial sums of several row ranges meet in dense_dbsum in
 // a fixed order.
 // ---------------------------------------------------------------------------
-constexpr int DA_COLS = 64, DA_ROWS = 128;
+constexpr int DA_COLS = 64;
+// rows of a block: 128, more where that keeps the ranges to 4096
+static inline int dact_rows(int M) { return M <= 128 * 4096 ? 128 : (M + 4095) / 4096; }
 
 // D: 0 none (dz is dy, only db is made), 1 u8 mask, 2 fp32 derivative.  dzr (or
 // null): dz rounded to bf16, the operand of dx; dW takes the fp32 one.
@@ -659,10 +661,11 @@ template <typename T, int D, typename TZ>
 __global__ __launch_bounds__(256) void dense_dact(const T* __restrict__ dy, const void* __restrict__ d,
                                                   TZ* __restrict__ dz, bf16_t* __restrict__ dzr,
                                                   float* __restrict__ db, int64_t db_gs,
-                                                  float* __restrict__ part, int M, int C, int N) {
+                                                  float* __restrict__ part, int M, int C, int N,
+                                                  int rows) {
   __shared__ float sm[4][DA_COLS];
   const int c = blockIdx.x * DA_COLS + (threadIdx.x & 63), w = threadIdx.x >> 6;
-  const int r0 = blockIdx.y * DA_ROWS, r1 = min(M, r0 + DA_ROWS);
+  const int r0 = blockIdx.y * rows, r1 = min(M, r0 + rows);
   float s = 0.f;
   if (c < C) {
 #pragma unroll 8
@@ -863,8 +866,9 @@ static inline Plan plan_of(int kind, int M, int N, int K, int G, int is_bf16, in
 }
 
 static inline bool sizes_ok(int M, int N, int K, int G, int64_t ldx) {
-  // byte offsets inside a tile are 32-bit: 256 rows of the longest row
-  const int64_t most = ((int64_t)1 << 31) / (256 * 4);
+  // byte offsets inside a tile are 32-bit: 255 rows of the longest pitch and a
+  // chunk
+  const int64_t most = ((int64_t)1 << 32) / (256 * 4);
   return M > 0 && N > 0 && K > 0 && G > 0 && (int64_t)G * N < most && (int64_t)G * K < most &&
          N < most && K < most && ldx >= (int64_t)G * K && ldx < most;
 }
@@ -879,7 +883,7 @@ CER_API int64_t cer_dense_ws(int kind, int M, int N, int K, int G, int is_bf16, 
   };
   if (kind == 0) return need(0, M, N);
   const int64_t a = need(1, M, K), b = need(2, N, K);
-  const int64_t nb = (M + DA_ROWS - 1) / DA_ROWS;
+  const int64_t nb = (M + dact_rows(M) - 1) / dact_rows(M);
   const int64_t c = nb > 1 ? nb * G * N : 0;
   return a > b ? (a > c ? a : c) : (b > c ? b : c);
 }
@@ -927,14 +931,17 @@ static int dense_bwd(const T* dy, const void* d, void* dz, const T* x, int64_t l
   const bool smooth = act_smooth(act);
   bf16_t* dzr = is_bf16 && smooth ? (bf16_t*)((float*)dz + (int64_t)M * C) : nullptr;
   if (act != ACT_NONE || gb) {
-    const dim3 grid((C + DA_COLS - 1) / DA_COLS, (M + DA_ROWS - 1) / DA_ROWS);
-    if (grid.y > 65535) return (int)hipErrorInvalidValue;
+    const int rows = dact_rows(M);
+    const dim3 grid((C + DA_COLS - 1) / DA_COLS, (M + rows - 1) / rows);
     if (act == ACT_NONE)
-      dense_dact<T, 0, T><<<grid, 256, 0, st>>>(dy, nullptr, nullptr, nullptr, gb, gbs, part, M, C, N);
+      dense_dact<T, 0, T><<<grid, 256, 0, st>>>(dy, nullptr, nullptr, nullptr, gb, gbs, part, M, C, N,
+                                                  rows);
     else if (smooth)
-      dense_dact<T, 2, float><<<grid, 256, 0, st>>>(dy, d, (float*)dz, dzr, gb, gbs, part, M, C, N);
+      dense_dact<T, 2, float><<<grid, 256, 0, st>>>(dy, d, (float*)dz, dzr, gb, gbs, part, M, C, N,
+                                                      rows);
     else
-      dense_dact<T, 1, T><<<grid, 256, 0, st>>>(dy, d, (T*)dz, nullptr, gb, gbs, part, M, C, N);
+      dense_dact<T, 1, T><<<grid, 256, 0, st>>>(dy, d, (T*)dz, nullptr, gb, gbs, part, M, C, N,
+                                                  rows);
     if (gb && grid.y > 1)
       dense_dbsum<<<grid.x, 256, 0, st>>>(part, grid.y, gb, gbs, C, N);
   }

@@ -414,3 +414,31 @@ def test_teacher_to_student_step(dtype):
         torch.cuda.synchronize()
         assert torch.equal(out, want)
     assert torch.equal(sar.state, after)
+
+
+def test_more_than_two_to_the_31_elements():
+    """17 000 rows of 131 072 classes (2.2e9 logits): loss, gradient and top
+    logits of the last rows."""
+    B, N, K = 17_000, 131_072, 8
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    z = torch.empty(B, N, dtype=torch.bfloat16, device=DEV)
+    for i in range(0, B, 1000):
+        z[i:i + 1000] = (torch.randn(1000, N, generator=gen, device=DEV) * 3).bfloat16()
+    val, idx = L.top_logits(z, 1, K)
+    tail = slice(B - 40, B)
+    vr, ir = top_reference(z[tail], 1, K)
+    assert torch.equal(idx[:, tail].cpu(), ir) and torch.equal(val[:, tail].cpu(), vr)
+    lab = torch.randint(0, N, (1, B), generator=gen, device=DEV, dtype=torch.int32)
+    alpha, tau = torch.tensor([0.4], device=DEV), torch.tensor([2.0], device=DEV)
+    z.requires_grad_(True)
+    grads = []
+    for unit in (True, False):
+        loss = L.distill_ce(z, lab, torch.zeros(1, 4, device=DEV), 1, val, idx, alpha, tau, unit=unit)
+        grads.append(torch.autograd.grad(loss, [z], torch.ones(1, device=DEV))[0])
+        del loss
+    assert torch.equal(grads[0], grads[1])
+    one = torch.ones(1, device=DEV)
+    _, _, d, dm = reference(z.detach()[tail], lab[:, tail], val[:, tail], idx[:, tail], alpha, tau, one)
+    d, dm = d * 40 / B, dm * 40 / B
+    tol = 2.0 ** -20 * 40 * dm
+    assert ((grads[0][tail].double() - d).abs() <= tol + 2.0 ** -8 * (d.abs() + tol) + 1e-30).all()

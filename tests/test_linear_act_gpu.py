@@ -317,3 +317,41 @@ def test_two_streams_at_once():
                 outs.append(P.linear_act(x, w, b, "silu"))
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+
+
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_more_than_two_to_the_31_elements(act):
+    """600 000 rows of 4096 outputs (2.4e9 elements): the last rows, the input
+    gradient there and the weight gradient of everything."""
+    M, K, N = 600_000, 8, 4096
+    arena, w, b = make(1, N, K, torch.bfloat16, device=DEV)
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.randn(M, K, generator=gen, device=DEV).bfloat16().requires_grad_(True)
+    y = P.linear_act(x, w, b, act)
+    dy = torch.empty_like(y)
+    for i in range(0, M, 50_000):
+        dy[i:i + 50_000] = torch.randn(50_000, N, generator=gen, device=DEV).bfloat16()
+    dx, = torch.autograd.grad(y, [x], dy)
+    dw = torch.zeros(N, K, dtype=torch.float64, device=DEV)
+    sw = torch.zeros_like(dw)
+    ws = w.work()[0].double()
+    for i in range(0, M, 50_000):
+        xs = x.detach()[i:i + 50_000].double()
+        z = (xs @ ws.t() + b.work()[0].double()).requires_grad_(True)
+        a = ACT64[act](z)
+        dz, = torch.autograd.grad(a, [z], dy[i:i + 50_000].double())
+        a = a.detach()
+        S = xs.abs() @ ws.abs().t() + b.work()[0].double().abs()
+        if i + 50_000 == M or i == 0:
+            # y: 9 exact terms in fp32, the activation, bf16; dx: dz rounded to
+            # bf16 where there is an activation, 4096 terms in fp32, bf16
+            ea = 1.13 * 9 * 2.0 ** -24 * S + 2.0 ** -20 * (1 + z.abs())
+            _within(y.detach()[i:i + 50_000], a, ea + (2.0 ** -8 + 2.0 ** -20) * (a.abs() + ea), "y")
+            want, sx = dz @ ws, dz.abs() @ ws.abs()
+            ex = (2.0 ** -8 + 4097 * 2.0 ** -24) * sx + 2.0 ** -18 * (
+                (dy[i:i + 50_000].double().abs() * (1 + S)) @ ws.abs())
+            _within(dx[i:i + 50_000], want, ex + 2.0 ** -8 * (want.abs() + ex), "dx")
+        dw += dz.t() @ xs
+        sw += (dy[i:i + 50_000].double().abs() * (1 + S)).t() @ xs.abs()
+    # three exact planes of dz; fp32 sums of 3 M terms
+    _within(w.grad()[0], dw, ((3 * M + 1) * 2.0 ** -24) * sw, "dw")
