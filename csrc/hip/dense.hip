@@ -172,10 +172,10 @@ __device__ __forceinline__ void ld4(const T* p, float* v, int nv) {
   }
 }
 
-// finished sums of row `row`, columns col .. col + 3 of config g
+// finished sums of row `row`, columns col .. col + nv - 1 of config g (at most 4)
 template <int EPI, typename T>
-__device__ __forceinline__ void epilogue(const GemmP& P, int g, int row, int col, float* z) {
-  const int nv = P.n - col;
+__device__ __forceinline__ void epilogue(const GemmP& P, int g, int row, int col, int nv,
+                                         float* z) {
   const int64_t o = (int64_t)g * P.c_gs + (int64_t)row * P.ldc + col;
   if constexpr (EPI == EPI_FWD) {
     if (P.bias) {
@@ -613,13 +613,139 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void dense_gemm(const GemmP P) {
         if (P.splits > 1)
           st4(P.part + (((int64_t)split * P.G + g) * P.m + row) * P.n + col, z, P.n - col);
         else
-          epilogue<EPI, TO>(P, g, row, col, z);
+          epilogue<EPI, TO>(P, g, row, col, P.n - col, z);
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   }
+}
+
+// ---------------------------------------------------------------------------
+// The forward of a few rows (serving: one row), M <= 8.  One pass over the
+// weights, which bound it: lanes along k, 16 B of each of NC weight rows per
+// step, products and sums in fp32 (no planes), one launch -- the MFMA tiles need
+// the reduction split over blocks to fill the chip and a second launch to join
+// it.  KW waves share a column's k where there are few columns.
+//
+// us, this kernel / the MFMA tiles (weights in turn from 3 copies):
+//                      M 1          M 2          M 4          M 8
+//   4096 x 4096 bf16    7.3 / 13.4   7.6 / 13.3  12.8 / 13.2  15.8 / 13.4
+//   4096 x 4096 fp32   12.4 / 21.5  12.5 / 21.5  14.6 / 21.4  28.8 / 22.0
+//   8 x 4608 x 4096 b  47.0 / 44.7  46.3 / 44.3  83.6 / 44.3  83.4 / 44.5
+//   8 x 4608 x 4096 f   101 / 110    105 / 109    107 / 109    177 / 109
+//   2048 x 1000 bf16    5.1 /  8.9   4.5 /  9.1   4.9 /  9.3   6.0 /  9.7
+//   8192 x 64 fp32      4.6 / 16.9   5.0 / 15.7   5.1 / 16.6   6.3 / 16.4
+//   100 x 8000 bf16     5.5 /  5.2   6.0 /  5.2   7.5 /  5.1  11.1 /  5.3
+// With more rows the products on the vector units weigh more than the second
+// launch, the sooner the more weights there are: gemv_better.
+// ---------------------------------------------------------------------------
+constexpr int GEMV_ROWS = 8;
+
+static inline bool gemv_better(int M, int N, int K, int G, int is_bf16) {
+  const int64_t bytes = (int64_t)G * N * K * (is_bf16 ? 2 : 4);
+  if (M <= 2) return true;
+  if (M <= 4) return K >= 512 && (!is_bf16 || bytes <= (32 << 20));
+  return M <= GEMV_ROWS && K >= 512 && bytes <= (8 << 20);
+}
+
+template <typename T, int MT, int NC, int KW>
+__global__ __launch_bounds__(256) void dense_gemv(const GemmP P) {
+  constexpr int V = 16 / sizeof(T), CW = 4 / KW;        // column groups of a block
+  __shared__ float sm[KW > 1 ? 4 * NC * MT : 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int per = (P.n + CW * NC - 1) / (CW * NC);
+  const int g = blockIdx.x / per, blk = blockIdx.x - g * per;
+  const int col = (blk * CW + wave / KW) * NC;
+  const T* x = reinterpret_cast<const T*>(P.a) + g * P.a_gs;
+  const T* w[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c)       // columns past the last: the last one's weights
+    w[c] = reinterpret_cast<const T*>(P.b) + g * P.b_gs + (int64_t)min(col + c, P.n - 1) * P.ldb;
+  float acc[MT][NC];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int c = 0; c < NC; ++c) acc[m][c] = 0.f;
+
+  auto step = [&](int k, auto ld) {
+    float wv[NC][V];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) ld(w[c] + k, wv[c]);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      float xv[V];
+      ld(x + min(m, P.m - 1) * P.lda + k, xv);
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[m][c] = fmaf(xv[e], wv[c][e], acc[m][c]);
+    }
+  };
+  auto whole = [](const T* p, float* v) {
+#pragma unroll
+    for (int e = 0; e < V; e += 4) ld4(p + e, v + e, 4);
+  };
+  int k = ((wave % KW) * 64 + lane) * V;
+#pragma unroll 2
+  for (; k + V <= P.k; k += KW * 64 * V) step(k, whole);
+  if (k < P.k)
+    step(k, [&](const T* p, float* v) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = k + e < P.k ? ld1(p + e) : 0.f;
+    });
+
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int c = 0; c < NC; ++c) acc[m][c] = warp_sum(acc[m][c]);
+  if constexpr (KW > 1) {
+    if (lane == 0) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) sm[(wave * MT + m) * NC + c] = acc[m][c];
+    }
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        float s = 0.f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) s += sm[(q * MT + m) * NC + c];
+        acc[m][c] = s;
+      }
+  }
+  // lane m finishes row m
+  if (col >= P.n || lane >= P.m) return;
+  float z[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+    if (lane == m) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) z[c] = acc[m][c];
+    }
+  epilogue<EPI_FWD, T>(P, g, lane, col, min(NC, P.n - col), z);
+}
+
+template <typename T, int MT>
+static int launch_gemv(const GemmP& P, hipStream_t st) {
+  // columns of a wave: as many as leave 512 waves; where even one leaves fewer
+  // than 256 blocks and k is long, the four waves of a block share it
+  const int64_t cols = (int64_t)P.G * P.n;
+  auto go = [&](auto kern, int per_block) {
+    const int64_t blocks = (int64_t)P.G * ((P.n + per_block - 1) / per_block);
+    if (blocks > 0x7fffffff) return (int)hipErrorInvalidValue;
+    kern<<<(int)blocks, 256, 0, st>>>(P);
+    return (int)hipGetLastError();
+  };
+  constexpr int NM = MT > 4 ? 2 : 4;          // registers: MT * NC sums
+  if (cols >= 4 * 512 * NM) return go(dense_gemv<T, MT, NM, 1>, 4 * NM);
+  if (cols < 4 * 256 && P.k >= 1024) return go(dense_gemv<T, MT, 1, 4>, 1);
+  return go(dense_gemv<T, MT, 1, 1>, 4);
 }
 
 // sums the split-K partials in split order (the result does not depend on
@@ -642,7 +768,7 @@ __global__ __launch_bounds__(256) void dense_join(const GemmP P) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) z[e] += v[e];
     }
-    epilogue<EPI, TO>(P, g, row, col, z);
+    epilogue<EPI, TO>(P, g, row, col, P.n - col, z);
   }
 }
 
@@ -881,7 +1007,7 @@ CER_API int64_t cer_dense_ws(int kind, int M, int N, int K, int G, int is_bf16, 
     const Plan p = plan_of(kd, M, N, K, G, is_bf16, act);
     return p.splits > 1 ? (int64_t)p.splits * G * m * n : 0;
   };
-  if (kind == 0) return need(0, M, N);
+  if (kind == 0) return gemv_better(M, N, K, G, is_bf16) ? 0 : need(0, M, N);
   const int64_t a = need(1, M, K), b = need(2, N, K);
   const int64_t nb = (M + dact_rows(M) - 1) / dact_rows(M);
   const int64_t c = nb > 1 ? nb * G * N : 0;
@@ -909,6 +1035,12 @@ static int dense_fwd(const T* x, int64_t ldx, const T* w, int64_t ws, const T* b
   P.d = act == ACT_NONE ? nullptr : d;
   P.act = act;
   P.part = part;
+  if (gemv_better(M, N, K, G, is_bf16)) {
+    if (M == 1) return launch_gemv<T, 1>(P, st);
+    if (M == 2) return launch_gemv<T, 2>(P, st);
+    if (M <= 4) return launch_gemv<T, 4>(P, st);
+    return launch_gemv<T, GEMV_ROWS>(P, st);
+  }
   const Plan p = plan_of(0, M, N, K, G, is_bf16, act);
   constexpr int PL = is_bf16 ? 1 : 3;
   return run_gemm<T, T, PL, PL, false, false, EPI_FWD, T>(P, p, st);

@@ -161,6 +161,18 @@ def test_long_reduction_is_split(dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 5, 8, 9])
+@pytest.mark.parametrize("size", [(1, 512, 7), (1, 4099, 30), (2, 1031, 1100), (3, 40, 50)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_few_rows(size, M, dtype):
+    """Either side of the rule for few rows, columns short of a wave's share,
+    reductions that end inside a vector."""
+    G, K, N = size
+    check(G, M, K, N, dtype, "gelu_tanh", train=False)
+    check(G, M, K, N, dtype, "none", residual=False)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
 def test_pitched_and_odd_aligned_rows(dtype):
     G, M, K, N = 2, 45, 33, 21
     big = torch.randn(M, G * K + 7, device=DEV).to(dtype)
