@@ -48,12 +48,22 @@ __device__ __forceinline__ uint64_t number_of(float z, int j) {
   return ((uint64_t)key_of(z) << 32) | (uint32_t)~j;
 }
 
-// s[0 .. n) in descending order; n a power of two, all TH threads
+// s[0 .. n) in descending order; n a power of two, all TH threads.  At a distance
+// of up to 64 a wave's pairs stay inside its own 128 numbers, step after step:
+// those steps need no barrier of the block.
 template <int TH>
 __device__ __forceinline__ void bitonic(uint64_t* s, int n) {
+  bool wide = true;
   for (int k = 2; k <= n; k <<= 1) {
     for (int j = k >> 1; j > 0; j >>= 1) {
-      __syncthreads();
+      if (wide || j > 64) {
+        __syncthreads();
+      } else {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      }
+      wide = j > 64;
       for (int i = threadIdx.x; i < n / 2; i += TH) {
         const int a = 2 * i - (i & (j - 1)), b = a + j;
         const uint64_t x = s[a], y = s[b];
@@ -67,11 +77,11 @@ __device__ __forceinline__ void bitonic(uint64_t* s, int n) {
   __syncthreads();
 }
 
-// The C numbers in s (room for the next power of two, above 512) in descending
+// The C numbers in s (room for the next power of two, above 256) in descending
 // order to out(rank, number) for rank < K.
 template <int TH, typename F>
 __device__ __forceinline__ void ordered(uint64_t* s, int* rk, int C, int K, F out) {
-  if (C <= 512) {
+  if (C <= 256) {
     // few: every number counts the larger ones; several threads share a number
     const int ce = (C + 1) & ~1;
     if (threadIdx.x == 0 && ce > C) s[C] = 0;
@@ -98,25 +108,37 @@ __device__ __forceinline__ void ordered(uint64_t* s, int* rk, int C, int K, F ou
       if (rk[i] < K) out(rk[i], s[i]);
     return;
   }
-  int n = 1024;
+  int n = 512;
   while (n < C) n <<= 1;
   for (int i = C + threadIdx.x; i < n; i += TH) s[i] = 0;
   bitonic<TH>(s, n);
   for (int i = threadIdx.x; i < K; i += TH) out(i, s[i]);
 }
 
-// a lower bound (upper 16 bits: all of a bf16) of the kw-th largest of a wave's 64 * GR keys
-template <int GR>
-__device__ __forceinline__ uint32_t wave_bound(const uint32_t* mk, int kw) {
+// a lower bound (upper 16 bits: all of a bf16) of the kw-th largest of a wave's
+// keys, kw <= 64
+__device__ __forceinline__ uint32_t wave_bound(uint32_t mk, int kw) {
   uint32_t t = 0;
-  if (kw <= 64 * GR) {
-    for (int bit = 31; bit >= 16; --bit) {
-      const uint32_t c = t | (1u << bit);
-      int reach = 0;
+  for (int bit = 31; bit >= 16; --bit) {
+    const uint32_t c = t | (1u << bit);
+    if (__popcll(__ballot(mk >= c)) >= kw) t = c;
+  }
+  return t;
+}
+
+// the same of the K-th largest of a block's GR keys a thread; cnt: 16 zeros,
+// ordered before by a barrier
+template <int GR>
+__device__ __forceinline__ uint32_t block_bound(const uint32_t* mk, int K, int* cnt) {
+  uint32_t t = 0;
+  for (int bit = 31; bit >= 16; --bit) {
+    const uint32_t c = t | (1u << bit);
+    int reach = 0;
 #pragma unroll
-      for (int q = 0; q < GR; ++q) reach += __popcll(__ballot(mk[q] >= c));
-      if (reach >= kw) t = c;
-    }
+    for (int q = 0; q < GR; ++q) reach += __popcll(__ballot(mk[q] >= c));
+    if ((threadIdx.x & 63) == 0 && reach) atomicAdd(&cnt[bit - 16], reach);
+    __syncthreads();
+    if (cnt[bit - 16] >= K) t = c;
   }
   return t;
 }
@@ -181,11 +203,13 @@ __device__ __noinline__ int radix_candidates(F number, int n, int K, uint64_t* c
 template <typename T, int TH, int R>
 __global__ __launch_bounds__(TH) void top_rows(const TopP P) {
   constexpr int W = TH / 64, V = RowRegs<T, TH, R>::V, CAP = RowRegs<T, TH, R>::CAP;
-  constexpr int GR = R >= 4 ? 4 : 1;          // maxima a thread keeps for larger K
+  // keys a thread brings to the bound: one maximum, or for larger K the maxima of
+  // 4 parts of its elements, or all of them where it has one vector
+  constexpr int GR = R == 1 ? V : R >= 4 ? 4 : 1;
   constexpr bool SHORT = CAP <= 512;          // the whole row fits: no search is ever needed
   extern __shared__ __attribute__((aligned(16))) uint64_t cand[];
   __shared__ uint32_t bound[16];
-  __shared__ int hist[SHORT ? 1 : 256], rk[512], count, nanflag;
+  __shared__ int hist[SHORT ? 1 : 256], rk[256], cnt[16], count, nanflag;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int row = blockIdx.x / P.chunks, ch = blockIdx.x - row * P.chunks;
   const int g = row / P.B, b = row - g * P.B;
@@ -196,6 +220,7 @@ __global__ __launch_bounds__(TH) void top_rows(const TopP P) {
     count = 0;
     nanflag = 0;
   }
+  if (tid < 16) cnt[tid] = 0;
   regs.load(zr, n, tid);
   const int K = min(P.K, n);
   const int kw = (K + W - 1) / W;
@@ -212,27 +237,31 @@ __global__ __launch_bounds__(TH) void top_rows(const TopP P) {
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       nan |= z[e] != z[e];
-      t = fmaxf(t, z[e]);
+      if constexpr (R == 1) m[e] = fmaxf(m[e], z[e]);
+      else t = fmaxf(t, z[e]);
     }
-    m[r % GR] = fmaxf(m[r % GR], t);
+    if constexpr (R > 1) m[r % GR] = fmaxf(m[r % GR], t);
   });
   if (__ballot(nan) && lane == 0) nanflag = 1;
-  if (GR > 1 && kw <= 16) {
+  // A small share per wave: the smallest of the waves' own bounds, which lets
+  // some more through but needs one barrier.  A large one: the block's bound,
+  // found with a barrier a bit (K 256 of 1000: 258 candidates, not all 1000).
+  uint32_t lim;
+  if (kw <= 16) {
 #pragma unroll
-    for (int q = 1; q < GR; ++q) {
-      m[0] = fmaxf(m[0], m[q]);
-      m[q] = -INFINITY;
-    }
+    for (int q = 1; q < GR; ++q) m[0] = fmaxf(m[0], m[q]);
+    const uint32_t t = wave_bound(key_of(m[0]), kw);
+    if (lane == 0) bound[wave] = t;
+    __syncthreads();
+    lim = bound[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) lim = min(lim, bound[w]);
+  } else {
+    uint32_t mk[GR];
+#pragma unroll
+    for (int q = 0; q < GR; ++q) mk[q] = key_of(m[q]);
+    lim = block_bound<GR>(mk, K, cnt);
   }
-  uint32_t mk[GR];
-#pragma unroll
-  for (int q = 0; q < GR; ++q) mk[q] = key_of(m[q]);
-  const uint32_t t = wave_bound<GR>(mk, kw);
-  if (lane == 0) bound[wave] = t;
-  __syncthreads();
-  uint32_t lim = bound[0];
-#pragma unroll
-  for (int w = 1; w < W; ++w) lim = min(lim, bound[w]);
   const bool has_nan = nanflag != 0;
   int C = P.cand + 1;
   if (!has_nan || SHORT) {
@@ -288,14 +317,14 @@ __global__ __launch_bounds__(TH) void top_rows(const TopP P) {
 constexpr int TM_TH = 1024;
 template <typename T>
 __global__ __launch_bounds__(TM_TH) void top_merge(const TopP P) {
-  constexpr int W = TM_TH / 64, GR = 4;
+  constexpr int GR = 4;
   __shared__ __attribute__((aligned(16))) uint64_t cand[TOP_CAND];
-  __shared__ uint32_t bound[W];
-  __shared__ int hist[256], rk[512], count;
+  __shared__ int hist[256], rk[256], cnt[16], count;
   const int tid = threadIdx.x, row = blockIdx.x;
-  const int n = P.chunks * P.room, K = P.K, kw = (K + W - 1) / W;
+  const int n = P.chunks * P.room, K = P.K;
   const uint64_t* src = P.list + (int64_t)row * n;
   if (tid == 0) count = 0;
+  if (tid < 16) cnt[tid] = 0;
   uint32_t mk[GR] = {0, 0, 0, 0};
   for (int i = tid; i < n; i += GR * TM_TH) {
 #pragma unroll
@@ -304,12 +333,8 @@ __global__ __launch_bounds__(TM_TH) void top_merge(const TopP P) {
       if (j < n) mk[q] = max(mk[q], (uint32_t)(src[j] >> 32));
     }
   }
-  const uint32_t t = wave_bound<GR>(mk, kw);
-  if ((tid & 63) == 0) bound[tid >> 6] = t;
   __syncthreads();
-  uint32_t lim = bound[0];
-#pragma unroll
-  for (int w = 1; w < W; ++w) lim = min(lim, bound[w]);
+  uint32_t lim = block_bound<GR>(mk, K, cnt);
   if (lim == 0) lim = 1;                       // zeros stay out
   for (int i = tid; i < n; i += TM_TH) {
     const uint64_t x = src[i];
@@ -383,9 +408,9 @@ static int top_launch(const T* z, int64_t ldz, T* val, int* idx, int B, int G, i
   const int grid = (int)(rows * P.chunks);
   const int n = P.chunk;
   constexpr int V = 16 / (int)sizeof(T);
-  // room for a multiple of K, a power of two above 512 for the sort (a short row
-  // is ranked and takes one place more); little LDS leaves more blocks on a CU
-  P.cand = n <= 64 * V ? 514 : K <= 256 ? 1024 : TOP_CAND;
+  // room for a multiple of K, a power of two for the sort; little LDS leaves more
+  // blocks on a CU
+  P.cand = n <= 64 * V ? 512 : K <= 256 ? 1024 : TOP_CAND;
 #define CER_TOP(TH, R) top_rows<T, TH, R><<<grid, TH, P.cand * sizeof(uint64_t), st>>>(P)
   if (n <= 64 * V) CER_TOP(64, 1);
   else if (n <= 256 * V) CER_TOP(256, 1);
