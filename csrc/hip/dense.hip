@@ -864,12 +864,12 @@ static constexpr int tile_occ(int planes, int t) {
 // CU hide in each other; partials cost a launch and their traffic.  The
 // constants are fitted to 282 products (1 - 16 configurations, 1 - 16384 rows, 2
 // - 8192 columns, all three forms, both types), each timed under every tile and
-// up to 8 splits: the choice is on average 2 % slower than the best of them,
+// up to 8 splits: the choice is on average 3 % slower than the best of them,
 // against 9 % for the constants that a first guess gave.
 static Plan choose_plan(int64_t m, int64_t n, int64_t k, int G, int planes, int out_bytes) {
   const int passes = planes == 6 ? 6 : planes == 2 ? 1 : DZ_PLANES;
   const int esz = planes == 2 ? 2 : 4;
-  static const double eff_f32[4] = {0.56, 0.33, 0.33, 0.17}, eff_bf16[4] = {0.40, 0.43, 0.19, 0.09};
+  static const double eff_f32[4] = {0.56, 0.33, 0.34, 0.17}, eff_bf16[4] = {0.40, 0.43, 0.19, 0.09};
   static const double latency[4] = {0.76, 0.69, 0.60, 0.35};       // us of a step
   const double* eff = planes == 2 ? eff_bf16 : eff_f32;
   Plan best = {};
