@@ -252,7 +252,7 @@ def distill_ce(logits, labels, acc, G, top_val, top_idx, alpha=0.5, tau=1.0, uni
     ``softmax_ce``; unlabelled rows are no hits (with N == 2 every row is a top-5
     hit).  Gradient in ``logits`` only.  ``unit=True``: the caller
     back-propagates a gradient of ones, and the forward writes the gradient in
-    the same pass over the logits.
+    the same pass over the logits.  (Capturing a backward: see ``nn.linear_act``.)
     """
     z, N = _logit_rows("distill_ce", logits, G)
     B, dev = z.shape[0], z.device

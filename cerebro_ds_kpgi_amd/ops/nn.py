@@ -800,11 +800,12 @@ class PackedLinearAct(torch.autograd.Function):
 
 
 def _rows(t, width):
-    """``t`` as [rows, width] with neighbouring elements of a row adjacent;
-    a row pitch is kept, any other layout is copied."""
+    """``t`` as [rows, width] with neighbouring elements of a row adjacent; a row
+    pitch that the kernels' 32-bit tile offsets reach is kept, any other layout
+    is copied."""
     if getattr(t, "_cer_hl", False):
         raise ValueError("linear_act: an operand is in the HL format that only convolutions read")
-    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= width:
+    if t.dim() == 2 and t.stride(1) == 1 and width <= t.stride(0) < 1 << 22:
         return t
     return t.reshape(-1, width).contiguous()
 
@@ -819,8 +820,8 @@ def linear_act(x, wref, bref=None, act="none", residual=None, anchor=None):
     them, or ``anchor``, requiring a gradient the backward writes the weight and
     bias gradients into the arena as every op of this module does -- it writes,
     it does not add, so a parameter is used once per step.  Rounding: fp32
-    products run on the two-plane split (16 significand bits per factor, fp32
-    sums), bf16 products are exact with fp32 sums, and every output is rounded
+    products run on three bf16 planes per factor (as near to the exact sum as
+    fp32 products), bf16 products are exact with fp32 sums, and every output is rounded
     once; act'(z) is kept in fp32 between the passes.
     """
     code = LINEAR_ACTS.get(act)
@@ -829,6 +830,7 @@ def linear_act(x, wref, bref=None, act="none", residual=None, anchor=None):
     # one test on the way, the reasons only when it fails
     if (code is None or len(wref.spec.shape) != 2 or dtype is not arena.compute_dtype
             or dtype not in (torch.float32, torch.bfloat16) or not shape
+            or arena.work.dtype is not dtype
             or shape[-1] != arena.G * wref.spec.shape[1] or x.device != arena.state.device
             or (bref is not None and (bref.arena is not arena
                                       or bref.spec.shape != wref.spec.shape[:1]))
@@ -864,6 +866,9 @@ def _refuse_linear_act(x, wref, bref, act, residual):
     if x.dtype != arena.compute_dtype or x.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError("linear_act: x is {}, the arena computes in {} (fp32 and bf16 are "
                         "supported)".format(x.dtype, arena.compute_dtype))
+    if arena.work.dtype != x.dtype:
+        raise ValueError("linear_act: a {} arena that only parks states (trainable=False) has no "
+                         "{} weights".format(arena.compute_dtype, x.dtype))
     if x.dim() < 1 or x.shape[-1] != G * K:
         raise ValueError("linear_act: x {} does not end in G*K = {}".format(tuple(x.shape), G * K))
     if x.device != arena.state.device:

@@ -72,6 +72,11 @@ static void done(int rc, const char* name) {
   TORCH_CHECK(rc == 0, name, " failed with hipError ", rc);
 }
 
+static void once(const char* name) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), name,
+              " has no second derivative (its backward ran with create_graph=True)");
+}
+
 static Tensor floats(const Tensor& like, int64_t n) {
   return n > 0 ? at::empty({n}, like.options().dtype(at::kFloat)) : Tensor();
 }
@@ -99,6 +104,7 @@ struct LinearActBackward : public Node {
     variable_list out(3);
     const Tensor g0 = grads[0];
     if (!g0.defined()) return out;
+    once("linear_act");
     const Tensor xv = x.unpack();
     const c10::OptionalDeviceGuard guard(xv.device());
     const Tensor dy = g0.contiguous();
@@ -174,11 +180,15 @@ struct DistillBackward : public Node {
   SavedVariable z;
   Tensor stats, d;              // d: the finished gradient of a unit loss gradient
   int64_t G;
+  bool unit;
 
   variable_list apply(variable_list&& grads) override {
     variable_list out(1);
     if (!grads[0].defined()) return out;
-    if (d.defined()) {
+    once("distill_ce");
+    if (unit) {
+      TORCH_CHECK(d.defined(), "distill_ce: backward through the graph a second time; its gradient "
+                               "was freed (retain_graph=True keeps it)");
       out[0] = d;
       return out;
     }
@@ -230,6 +240,7 @@ static Tensor distill_ce(const Tensor& z, const Tensor& labels, const Tensor& ac
     auto node = std::shared_ptr<DistillBackward>(new DistillBackward(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(z));
     node->G = G;
+    node->unit = unit;
     if (unit) {
       node->d = std::move(d);
     } else {

@@ -187,6 +187,39 @@ def test_layouts_and_mixed_types():
         assert not L.distill_ce(z.requires_grad_(True), lab, want[2], 2, val, idx).requires_grad
 
 
+@DTYPES
+def test_no_teacher_entries_at_all(dtype):
+    """K = 0: the hard term alone, its metrics as softmax_ce counts them."""
+    for N in (11, 70001):
+        check(2, 4, N, 0, dtype, device=DEV)
+    z, lab, val, idx, _, _ = inputs(2, 6, 40, 0, torch.float32, ragged=False, device=DEV)
+    a1, a2 = torch.zeros(2, 4, device=DEV), torch.zeros(2, 4, device=DEV)
+    one = L.distill_ce(z, lab, a1, 2, val, idx, alpha=0.0)
+    two = L.softmax_ce(z, lab, a2, 2)
+    # both sum six rows' lse - z_y of size below 20 in fp32
+    assert (one - two).abs().max() <= 20 * 2.0 ** -20
+    assert torch.equal(a1[:, 1:], a2[:, 1:])
+
+
+@pytest.mark.parametrize("unit", [True, False])
+def test_backward_twice_and_second_derivatives(unit):
+    z, lab, val, idx, alpha, tau = inputs(1, 3, 20, 4, device=DEV)
+    z.requires_grad_(True)
+
+    def loss():
+        return L.distill_ce(z, lab, torch.zeros(1, 4, device=DEV), 1, val, idx, alpha, tau,
+                            unit=unit)
+    y = loss()
+    y.sum().backward(retain_graph=True)
+    first = z.grad.clone()
+    y.sum().backward()
+    assert torch.equal(z.grad, first + first)
+    with pytest.raises(RuntimeError, match="second time"):
+        y.sum().backward()
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(loss().sum(), [z], create_graph=True)
+
+
 def test_gradient_against_differences():
     z, lab, val, idx, alpha, tau = inputs(2, 3, 12, 4, device=DEV, scale=1.0)
 

@@ -100,3 +100,6 @@ def test_refusals():
         P.linear_act(x.clone().requires_grad_(True), w2, b2)
     with torch.no_grad():
         assert P.linear_act(x, w2, b2).shape == (4, 6)
+    _, w3, b3 = make(dtype=torch.bfloat16, trainable=False)
+    with pytest.raises(ValueError, match="parks"):
+        P.linear_act(x.bfloat16(), w3, b3)

@@ -367,3 +367,47 @@ def test_more_than_two_to_the_31_elements(act):
         sw += (dy[i:i + 50_000].double().abs() * (1 + S)).t() @ xs.abs()
     # three exact planes of dz; fp32 sums of 3 M terms
     _within(w.grad()[0], dw, ((3 * M + 1) * 2.0 ** -24) * sw, "dw")
+
+
+def test_backward_twice_and_second_derivatives():
+    arena, w, b = make(1, 6, 5, device=DEV)
+    x = torch.randn(4, 5, device=DEV, requires_grad=True)
+    y = P.linear_act(x, w, b, "silu")
+    y.sum().backward(retain_graph=True)
+    first = x.grad.clone()
+    y.sum().backward()
+    assert torch.equal(x.grad, first + first)
+    with pytest.raises(RuntimeError, match="second time"):
+        y.sum().backward()
+    y = P.linear_act(x, w, b, "silu")
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(y.sum(), [x], create_graph=True)
+    # an input that was overwritten since is refused
+    h = x * 1.0
+    y = P.linear_act(h, w, b, "silu")
+    h.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_widths_out_of_reach_and_far_pitches():
+    arena, w, b = make(1, (1 << 22) + 8, 2, device=DEV)
+    with pytest.raises(ValueError, match="32-bit"):
+        P.linear_act(torch.zeros(1, 2, device=DEV), w, b)
+    # a pitch beyond the tile offsets is copied away
+    arena, w, b = make(1, 9, 7, device=DEV)
+    big = torch.randn(5, (1 << 22) + 1, device=DEV)
+    y = P.linear_act(big[:, 3:10], w, b, "gelu", big[:, 20:29])
+    assert torch.equal(y, P.linear_act(big[:, 3:10].contiguous(), w, b, "gelu",
+                                       big[:, 20:29].contiguous()))
+
+
+def test_residual_is_the_input():
+    """h + act(h W^T): both gradients meet in h."""
+    arena, w, b = make(2, 12, 12, device=DEV)
+    x = torch.randn(7, 24, device=DEV, requires_grad=True)
+    dy = torch.randn(7, 24, device=DEV)
+    gx, = torch.autograd.grad(P.linear_act(x, w, b, "gelu", x), [x], dy)
+    r = x.detach().clone().requires_grad_(True)
+    g1, g2 = torch.autograd.grad(P.linear_act(x, w, b, "gelu", r), [x, r], dy)
+    assert torch.equal(gx, g1 + g2)
