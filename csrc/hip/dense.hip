@@ -253,25 +253,38 @@ struct Stage {
   int64_t step_bytes;         // uniform: bytes from one step to the next
   uint32_t ldb;               // row pitch in bytes
   int row0, rows, kc;         // tile origin, operand extent; this thread's k chunk
-  bool colfull;
+  // k-strided operands, V > 1 columns a load.  Where no tile fits in the columns a
+  // vector that crosses the last one is loaded V columns back from it and shifted
+  // into place (a bf16 training pass of 8192 x 101 x 8192: 877 -> 600 us).  Not in
+  // the tile of BK 64: the code of it alone spills 18 registers more there and
+  // costs the bf16 dgrad 440 us against 298 at 8192 x 4096 x 4096.  bf16 rows that
+  // start inside a dword are loaded as they lie; taking them from their dwords by
+  // shifts instead costs 219 us against 207 at 2047^3.
+  static constexpr bool SHIFT = KS && V > 1 && BK == 32;
+  bool aligned;               // no vector of the tile crosses
+  bool single;                // element by element
 
   __device__ __forceinline__ void init(const void* src, int64_t ld, int r0, int nrows, int tid) {
     rows = nrows;
     row0 = r0;
     ldb = (uint32_t)(ld * sizeof(S));
     if constexpr (KS) {
-      base = reinterpret_cast<const char*>(src) + (int64_t)r0 * sizeof(S);
+      // V columns before the tile: offsets of vectors that start there stay
+      // positive
+      base = reinterpret_cast<const char*>(src) + ((int64_t)r0 - V) * (int)sizeof(S);
       step_bytes = (int64_t)BK * ld * sizeof(S);
       kc = tid / (R / V);
       int c = (tid % (R / V)) * V;
-      colfull = r0 + R <= nrows || nrows % V == 0;
-      if (colfull && r0 + c + V > nrows) c = nrows - V - r0;   // wholly outside: any columns
-      off[0] = (uint32_t)(kc * 8) * ldb + (uint32_t)(c * (int)sizeof(S));
+      aligned = r0 + R <= nrows || nrows % V == 0;
+      single = nrows < V || (!SHIFT && !aligned);
+      if (r0 + c + V > nrows) c = nrows - V - r0;       // wholly outside: any columns
+      off[0] = (uint32_t)(kc * 8) * ldb + (uint32_t)((c + V) * (int)sizeof(S));
     } else {
       base = reinterpret_cast<const char*>(src) + (int64_t)r0 * ld * sizeof(S);
       step_bytes = (int64_t)BK * sizeof(S);
       kc = tid % CH;
-      colfull = true;
+      aligned = true;
+      single = false;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         int row = tid / CH + i * (T / CH);
@@ -358,7 +371,7 @@ struct Stage {
       const int c = (tid % (R / V)) * V;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const char* q = p + (uint64_t)(kc * 8 + e) * ldb + c * (int)sizeof(S);
+        const char* q = p + (uint64_t)(kc * 8 + e) * ldb + (c + V) * (int)sizeof(S);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           uint32_t w = 0;
@@ -371,13 +384,43 @@ struct Stage {
     }
   }
 
-  __device__ __forceinline__ bool full(int step, int k) const {
-    return k - step * BK >= BK && colfull;
+  // moves the vectors that cross the last column into place
+  __device__ __forceinline__ void shift(Regs& q_, int tid) const {
+    uint32_t* r = q_.r;
+    const int over = row0 + (tid % (R / V)) * V + V - rows;
+    const int sh = over > 0 && over < V ? over : 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (F32) {
+#pragma unroll
+        for (int b = 1; b < V; b <<= 1)
+#pragma unroll
+          for (int v = 0; v + b < V; ++v) r[V * e + v] = sh & b ? r[V * e + v + b] : r[V * e + v];
+      } else if constexpr (V == 2) {
+        r[e] >>= 16 * sh;
+      } else if constexpr (V == 4) {
+        uint64_t w = ((uint64_t)r[2 * e + 1] << 32) | r[2 * e];
+        w >>= 16 * sh;
+        r[2 * e] = (uint32_t)w;
+        r[2 * e + 1] = (uint32_t)(w >> 32);
+      }
+    }
+  }
+
+  // a step that load_full alone serves
+  __device__ __forceinline__ bool plain(int step, int k) const {
+    return k - step * BK >= BK && aligned && !single;
   }
 
   __device__ __forceinline__ void load(Regs& q_, int step, int k, int tid) const {
-    if (full(step, k)) load_full(q_, step);
-    else load_edge(q_, step, k - step * BK, tid);
+    if (k - step * BK < BK || single) {
+      load_edge(q_, step, k - step * BK, tid);
+      return;
+    }
+    load_full(q_, step);
+    if constexpr (SHIFT) {
+      if (!aligned) shift(q_, tid);
+    }
   }
 
   // the 8 k of chunk i as PL bf16 planes into LDS
@@ -459,7 +502,13 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void dense_gemm(const GemmP P) {
   const int band = w / (4 * P.tn), in = w - band * 4 * P.tn;
   const int bh = min(4, P.tm - band * 4);
   const int tm = band * 4 + in % bh, tn = in / bh;
-  const int m0 = tm * BM, n0 = tn * BN;
+  // The last tile of a k-strided operand whose extent is no multiple of the vector
+  // is moved back to end with it: whole loads, and the rows or columns it shares
+  // with its neighbour get the same sums from both.  With single elements for
+  // these tiles a bf16 training pass of 2047^3 takes 313 us, so 175, 2048^3 155.
+  int m0 = tm * BM, n0 = tn * BN;
+  if (KA && P.m >= BM && P.m % StA::V) m0 = min(m0, P.m - BM);
+  if (KB && P.n >= BN && P.n % StB::V) n0 = min(n0, P.n - BN);
 
   StA sa;
   StB sb;
@@ -530,7 +579,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void dense_gemm(const GemmP P) {
     char *cur = smem, *nxt = smem + BUF;
     // steps whose requests stay inside both operands: no branch between the
     // multiplications, the stores and the requests
-    for (; s + 2 * PF < s1 && sa.full(s + 2 * PF, P.k) && sb.full(s + 2 * PF, P.k); s += PF) {
+    for (; s + 2 * PF < s1 && sa.plain(s + 2 * PF, P.k) && sb.plain(s + 2 * PF, P.k); s += PF) {
 #pragma unroll
       for (int u = 0; u < PF; ++u) {
         mma(cur, 0);

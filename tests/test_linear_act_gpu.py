@@ -155,6 +155,18 @@ def test_largest_tiles(act, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("act", ["none", "gelu"])
+@pytest.mark.parametrize("size", [(1, 515, 1001, 1031), (1, 4099, 2049, 4101), (1, 2051, 2053, 101),
+                                  (1, 4098, 101, 4098), (2, 700, 257, 130), (1, 9001, 131, 135),
+                                  (3, 200, 67, 65), (1, 4100, 254, 4093)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_last_tiles_of_odd_widths(size, act, dtype):
+    """Backward products whose last tile overlaps its neighbour, or whose operand
+    is narrower than a tile and no multiple of a vector."""
+    check(*size, dtype, act)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
 def test_long_reduction_is_split(dtype):
     check(1, 3, 8192, 130, dtype, "silu")
     check(1, 8192, 40, 24, dtype, "silu")
