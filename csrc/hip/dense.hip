@@ -256,15 +256,16 @@ struct Stage {
   // k-strided operands, V > 1 columns a load.  Where no tile fits in the columns a
   // vector that crosses the last one is loaded V columns back from it and shifted
   // into place (a bf16 training pass of 8192 x 101 x 8192: 877 -> 600 us).  Not in
-  // the tile of BK 64: the code of it alone spills 18 registers more there and
-  // costs the bf16 dgrad 440 us against 298 at 8192 x 4096 x 4096.  bf16 rows that
-  // start inside a dword are loaded as they lie; taking them from their dwords by
-  // shifts instead costs 219 us against 207 at 2047^3.
+  // the tile of BK 64, where the code of it alone spills 40 registers instead of 2:
+  // with 66 the bf16 dgrad of 8192 x 4096 x 4096 took 440 us, with 48 298, with 2
+  // 290.  bf16 rows that start inside a dword are loaded as they lie; taking them
+  // from their dwords by shifts costs 219 us against 207 at 2047^3.
   static constexpr bool SHIFT = KS && V > 1 && BK == 32;
   bool aligned;               // no vector of the tile crosses
   bool single;                // element by element
 
-  __device__ __forceinline__ void init(const void* src, int64_t ld, int r0, int nrows, int tid) {
+  __device__ __forceinline__ void init(const void* src, int64_t ld, int r0, int nrows, int k,
+                                       int tid) {
     rows = nrows;
     row0 = r0;
     ldb = (uint32_t)(ld * sizeof(S));
@@ -284,7 +285,7 @@ struct Stage {
       step_bytes = (int64_t)BK * sizeof(S);
       kc = tid % CH;
       aligned = true;
-      single = false;
+      single = k < 8;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         int row = tid / CH + i * (T / CH);
@@ -294,53 +295,98 @@ struct Stage {
     }
   }
 
+  // chunk i of a row-strided operand: 8 k from p
+  __device__ __forceinline__ void chunk(uint32_t* r, int i, const char* p) const {
+    if constexpr (F32) {
+      const f32x4_a4 a = *reinterpret_cast<const f32x4_a4*>(p);
+      const f32x4_a4 b = *reinterpret_cast<const f32x4_a4*>(p + 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        r[8 * i + e] = __float_as_uint(a[e]);
+        r[8 * i + 4 + e] = __float_as_uint(b[e]);
+      }
+    } else {
+      const u32x4_a2 a = *reinterpret_cast<const u32x4_a2*>(p);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[4 * i + e] = a[e];
+    }
+  }
+
+  // k number e of a k-strided operand: V columns from p
+  __device__ __forceinline__ void vec(uint32_t* r, int e, const char* p) const {
+    if constexpr (F32) {
+      if constexpr (V == 1) {
+        r[e] = *reinterpret_cast<const uint32_t*>(p);
+      } else if constexpr (V == 2) {
+        const f32x2_a4 a = *reinterpret_cast<const f32x2_a4*>(p);
+        r[2 * e] = __float_as_uint(a.x);
+        r[2 * e + 1] = __float_as_uint(a.y);
+      } else {
+        const f32x4_a4 a = *reinterpret_cast<const f32x4_a4*>(p);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) r[4 * e + v] = __float_as_uint(a[v]);
+      }
+    } else {
+      if constexpr (V == 1) {
+        r[e] = *reinterpret_cast<const bf16_t*>(p);
+      } else if constexpr (V == 2) {
+        r[e] = *reinterpret_cast<const u32_a2*>(p);
+      } else {
+        const u32x2_a2 a = *reinterpret_cast<const u32x2_a2*>(p);
+        r[2 * e] = a.x;
+        r[2 * e + 1] = a.y;
+      }
+    }
+  }
+
   __device__ __forceinline__ void load_full(Regs& q_, int step) const {
     uint32_t* r = q_.r;
     const char* p = base + step * step_bytes;
     if constexpr (!KS) {
 #pragma unroll
+      for (int i = 0; i < V; ++i) chunk(r, i, p + off[i]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) vec(r, e, p + (uint64_t)e * ldb + off[0]);
+    }
+  }
+
+  // the last step, with kleft < BK: zeros behind.  A chunk that crosses the last k
+  // is loaded from the 8 k that end there and shifted; k behind the last one are
+  // loaded from it and dropped.  (bf16 forward of 2048 x 2047 x 2048: 44.3 us,
+  // element by element 48.7; of 8192 x 4095 x 4096: 334 and 354.)
+  __device__ __forceinline__ void load_tail(Regs& q_, int step, int kleft) const {
+    uint32_t* r = q_.r;
+    const char* p = base + step * step_bytes;
+    if constexpr (!KS) {
+      const int back = max(0, kc * 8 + 8 - kleft);
+#pragma unroll
       for (int i = 0; i < V; ++i) {
-        if constexpr (F32) {
-          const f32x4_a4 a = *reinterpret_cast<const f32x4_a4*>(p + off[i]);
-          const f32x4_a4 b = *reinterpret_cast<const f32x4_a4*>(p + off[i] + 16);
+        chunk(r, i, p + off[i] - (int64_t)back * (int)sizeof(S));
+        constexpr int D = F32 ? 8 : 4;                // dwords of a chunk
+        uint32_t* c = r + D * i;
+        if constexpr (!F32) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            r[8 * i + e] = __float_as_uint(a[e]);
-            r[8 * i + 4 + e] = __float_as_uint(b[e]);
-          }
-        } else {
-          const u32x4_a2 a = *reinterpret_cast<const u32x4_a2*>(p + off[i]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) r[4 * i + e] = a[e];
+          for (int d = 0; d < D; ++d)
+            c[d] = back & 1 ? __builtin_amdgcn_alignbit(d + 1 < D ? c[d + 1] : 0, c[d], 16) : c[d];
         }
+#pragma unroll
+        for (int b = 1; b < D; b <<= 1) {
+          const bool on = back & (F32 ? b : 2 * b);
+#pragma unroll
+          for (int d = 0; d < D; ++d) c[d] = on ? (d + b < D ? c[d + b] : 0) : c[d];
+        }
+#pragma unroll
+        for (int d = 0; d < D; ++d) c[d] = back < 8 ? c[d] : 0;
       }
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const char* q = p + (uint64_t)e * ldb + off[0];
-        if constexpr (F32) {
-          if constexpr (V == 1) {
-            r[e] = *reinterpret_cast<const uint32_t*>(q);
-          } else if constexpr (V == 2) {
-            const f32x2_a4 a = *reinterpret_cast<const f32x2_a4*>(q);
-            r[2 * e] = __float_as_uint(a.x);
-            r[2 * e + 1] = __float_as_uint(a.y);
-          } else {
-            const f32x4_a4 a = *reinterpret_cast<const f32x4_a4*>(q);
+        const int over = max(0, kc * 8 + e - (kleft - 1));
+        vec(r, e, p + (int64_t)(e - over) * ldb + off[0]);
+        constexpr int D = NR / 8;                     // dwords of a vector
 #pragma unroll
-            for (int v = 0; v < 4; ++v) r[4 * e + v] = __float_as_uint(a[v]);
-          }
-        } else {
-          if constexpr (V == 1) {
-            r[e] = *reinterpret_cast<const bf16_t*>(q);
-          } else if constexpr (V == 2) {
-            r[e] = *reinterpret_cast<const u32_a2*>(q);
-          } else {
-            const u32x2_a2 a = *reinterpret_cast<const u32x2_a2*>(q);
-            r[2 * e] = a.x;
-            r[2 * e + 1] = a.y;
-          }
-        }
+        for (int d = 0; d < D; ++d) r[D * e + d] = over ? 0 : r[D * e + d];
       }
     }
   }
@@ -350,8 +396,8 @@ struct Stage {
     else return *reinterpret_cast<const bf16_t*>(p);
   }
 
-  // a step that reaches past the operand: elements outside are zero
-  __device__ __forceinline__ void load_edge(Regs& q_, int step, int kleft, int tid) const {
+  // element by element; those outside are zero
+  __device__ __forceinline__ void load_single(Regs& q_, int step, int kleft, int tid) const {
     uint32_t* r = q_.r;
     const char* p = base + step * step_bytes;
 #pragma unroll
@@ -413,11 +459,13 @@ struct Stage {
   }
 
   __device__ __forceinline__ void load(Regs& q_, int step, int k, int tid) const {
-    if (k - step * BK < BK || single) {
-      load_edge(q_, step, k - step * BK, tid);
+    const int kleft = k - step * BK;
+    if (single) {
+      load_single(q_, step, kleft, tid);
       return;
     }
-    load_full(q_, step);
+    if (kleft < BK) load_tail(q_, step, kleft);
+    else load_full(q_, step);
     if constexpr (SHIFT) {
       if (!aligned) shift(q_, tid);
     }
@@ -512,8 +560,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void dense_gemm(const GemmP P) {
 
   StA sa;
   StB sb;
-  sa.init(reinterpret_cast<const SA*>(P.a) + g * P.a_gs, P.lda, m0, P.m, tid);
-  sb.init(reinterpret_cast<const SB*>(P.b) + g * P.b_gs, P.ldb, n0, P.n, tid);
+  sa.init(reinterpret_cast<const SA*>(P.a) + g * P.a_gs, P.lda, m0, P.m, P.k, tid);
+  sb.init(reinterpret_cast<const SB*>(P.b) + g * P.b_gs, P.ldb, n0, P.n, P.k, tid);
 
   const int total = (P.k + BK - 1) / BK;
   const int s0 = split * P.steps;
