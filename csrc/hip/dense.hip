@@ -172,15 +172,26 @@ __device__ __forceinline__ void ld4(const T* p, float* v, int nv) {
   }
 }
 
-// finished sums of row `row`, columns col .. col + nv - 1 of config g (at most 4)
+// bias and residual of columns col .. col + nv - 1 (at most 4) of config g
+template <typename T>
+__device__ __forceinline__ void ld_bias(const GemmP& P, int g, int col, int nv, float* b) {
+  if (P.bias) ld4(reinterpret_cast<const T*>(P.bias) + g * P.bias_gs + col, b, nv);
+  else b[0] = b[1] = b[2] = b[3] = 0.f;
+}
+
+template <typename T>
+__device__ __forceinline__ const T* at_res(const GemmP& P, int g, int row, int col) {
+  return reinterpret_cast<const T*>(P.res) + g * P.c_gs + (int64_t)row * P.ldr + col;
+}
+
+// finished sums of row `row`, those columns; EPI_FWD: with their bias and, if there
+// is one, residual
 template <int EPI, typename T>
-__device__ __forceinline__ void epilogue(const GemmP& P, int g, int row, int col, int nv,
-                                         float* z) {
+__device__ __forceinline__ void epilogue(const GemmP& P, int g, int row, int col, int nv, float* z,
+                                         const float* b, const float* r) {
   const int64_t o = (int64_t)g * P.c_gs + (int64_t)row * P.ldc + col;
   if constexpr (EPI == EPI_FWD) {
     if (P.bias) {
-      float b[4];
-      ld4(reinterpret_cast<const T*>(P.bias) + g * P.bias_gs + col, b, nv);
 #pragma unroll
       for (int i = 0; i < 4; ++i) z[i] += b[i];
     }
@@ -205,8 +216,6 @@ __device__ __forceinline__ void epilogue(const GemmP& P, int g, int row, int col
       }
     }
     if (P.res) {
-      float r[4];
-      ld4(reinterpret_cast<const T*>(P.res) + g * P.c_gs + (int64_t)row * P.ldr + col, r, nv);
 #pragma unroll
       for (int i = 0; i < 4; ++i) z[i] += r[i];
     }
@@ -216,6 +225,17 @@ __device__ __forceinline__ void epilogue(const GemmP& P, int g, int row, int col
   } else {
     st4(reinterpret_cast<float*>(P.c) + o, z, nv);
   }
+}
+
+template <int EPI, typename T>
+__device__ __forceinline__ void epilogue(const GemmP& P, int g, int row, int col, int nv,
+                                         float* z) {
+  float b[4] = {}, r[4] = {};
+  if constexpr (EPI == EPI_FWD) {
+    ld_bias<T>(P, g, col, nv, b);
+    if (P.res) ld4(at_res<T>(P, g, row, col), r, nv);
+  }
+  epilogue<EPI, T>(P, g, row, col, nv, z, b, r);
 }
 
 // ---------------------------------------------------------------------------
@@ -684,10 +704,39 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void dense_gemm(const GemmP P) {
 
   // Each wave turns its tile through LDS, 16 * ER rows at a time, so that its 64
   // lanes finish and store whole row segments; the loop keeps the epilogue's
-  // code (activation, residual) short
+  // code (activation, residual) short.  A turn's residual is requested a turn
+  // ahead and waits in LDS: loads in the loop, which stay behind its stores, would
+  // be waited for one by one (bf16 8192 x 4096 x 4096 with gelu and act': 384 -> 355
+  // us).
   constexpr int WC = BN / WN, PITCH = WC + 4, ER = IM < 2 ? 1 : 2;
+  constexpr int LC = WC / 4, RS = 64 / LC, SN = 16 * ER / RS;   // lanes a row, rows a step, steps
   static_assert(IM % ER == 0, "rows of a turn");
   float* turn = reinterpret_cast<float*>(smem) + wave * (16 * ER * PITCH);
+  typedef uint32_t Raw __attribute__((ext_vector_type(sizeof(TO))));   // 4 elements
+  Raw* wait = reinterpret_cast<Raw*>(smem + WM * WN * 16 * ER * PITCH * 4) + wave * SN * 64 + lane;
+  const int col = n0 + wn + (lane % LC) * 4, row1 = m0 + wm + lane / LC;
+  const bool have = EPI == EPI_FWD && P.res && P.splits == 1 && col < P.n;
+  float bias[4] = {};
+  Raw ahead[SN];
+  auto fetch = [&](int i0) {
+#pragma unroll
+    for (int s = 0; s < SN; ++s) {
+      const TO* p = at_res<TO>(P, g, min(row1 + i0 * 16 + s * RS, P.m - 1), col);
+      if (col + 4 <= P.n) {
+        __builtin_memcpy(&ahead[s], p, sizeof(Raw));
+      } else {
+        TO v[4] = {};
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+          if (col + i < P.n) v[i] = p[i];
+        __builtin_memcpy(&ahead[s], v, sizeof(Raw));
+      }
+    }
+  };
+  if constexpr (EPI == EPI_FWD) {
+    if (col < P.n && P.splits == 1) ld_bias<TO>(P, g, col, P.n - col, bias);
+    if (have) fetch(0);
+  }
 #pragma unroll
   for (int i0 = 0; i0 < IM; i0 += ER) {
 #pragma unroll
@@ -695,22 +744,37 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void dense_gemm(const GemmP P) {
 #pragma unroll
       for (int j = 0; j < JN; ++j)
         *reinterpret_cast<f32x4*>(turn + (i * 16 + fr) * PITCH + j * 16 + fc * 4) = acc[i0 + i][j];
+    if constexpr (EPI == EPI_FWD) {
+      if (have) {
+#pragma unroll
+        for (int s = 0; s < SN; ++s) wait[s * 64] = ahead[s];
+        if (i0 + ER < IM) fetch(i0 + ER);
+      }
+    }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    constexpr int LC = WC / 4, RS = 64 / LC;        // lanes a row, rows a step
-    const int col = n0 + wn + (lane % LC) * 4;
     if (col < P.n) {
 #pragma unroll 2
-      for (int r = lane / LC; r < 16 * ER; r += RS) {
-        const int row = m0 + wm + i0 * 16 + r;
+      for (int s = 0; s < SN; ++s) {
+        const int row = row1 + i0 * 16 + s * RS;
         if (row >= P.m) break;
-        const f32x4 t = *reinterpret_cast<const f32x4*>(turn + r * PITCH + (lane % LC) * 4);
+        const f32x4 t = *reinterpret_cast<const f32x4*>(turn + (lane / LC + s * RS) * PITCH +
+                                                        (lane % LC) * 4);
         float z[4] = {t[0], t[1], t[2], t[3]};
-        if (P.splits > 1)
+        if (P.splits > 1) {
           st4(P.part + (((int64_t)split * P.G + g) * P.m + row) * P.n + col, z, P.n - col);
-        else
-          epilogue<EPI, TO>(P, g, row, col, P.n - col, z);
+        } else {
+          float r[4] = {};
+          if (have) {
+            const Raw w = wait[s * 64];
+            TO v[4];
+            __builtin_memcpy(v, &w, sizeof(Raw));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = to_f(v[i]);
+          }
+          epilogue<EPI, TO>(P, g, row, col, P.n - col, z, bias, r);
+        }
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -1034,7 +1098,9 @@ static int launch_gemm(GemmP& P, const Plan& p, hipStream_t st) {
   const int64_t blocks = (int64_t)P.G * p.tm * p.tn * p.splits;
   if (blocks > 0x7fffffff) return (int)hipErrorInvalidValue;
   constexpr int stage = 2 * (PA * BM + PB * BN) * BK * 2;
-  constexpr int turn = WM * WN * (BM / WM < 32 ? 16 : 32) * (BN / WN + 4) * 4;   // the epilogue's
+  // the epilogue's: sums, and the residual that waits
+  constexpr int turn = WM * WN * (BM / WM < 32 ? 16 : 32) *
+                       ((BN / WN + 4) * 4 + (EPI == EPI_FWD ? BN / WN * (int)sizeof(TO) : 0));
   constexpr int lds = stage > turn ? stage : turn;
   static_assert(lds <= 160 * 1024, "LDS of a CU");
   auto kern = dense_gemm<SA, SB, PA, PB, KA, KB, BM, BN, BK, WM, WN, PF, EPI, TO>;
