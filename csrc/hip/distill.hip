@@ -284,9 +284,10 @@ __device__ __forceinline__ void grad_row(const RowRegs<T, TH, R>& row, const Gra
     write_row(row, dr, [&](float z) { return grad_of<false, true>(q, z); });
 }
 
-// maximum, both sums and the label's rank of the elements in `row`, which
-// start at class j0 of the logits row; all threads get them.  A whole row of
-// -inf has sums of NaN, a SLICE of nothing but -inf sums of zero.
+// maximum, both sums and the label's rank (exact up to 4, at least 5 beyond) of
+// the elements in `row`, which start at class j0 of the logits row; all threads
+// get them.  A whole row of -inf has sums of NaN, a SLICE of nothing but -inf sums
+// of zero.
 template <typename T, int TH, int R, bool SLICE>
 __device__ __forceinline__ void row_stats(const RowRegs<T, TH, R>& row, int j0, int lab, float zl,
                                           bool hard, bool soft, float itau, float* sm, float& mx,
@@ -296,21 +297,25 @@ __device__ __forceinline__ void row_stats(const RowRegs<T, TH, R>& row, int j0, 
   int before = 0;
   if (lab >= 0) {
     // the maximum, and how many come before the label: counted a wave at a time
-    // in scalar registers; equal values are rare and looked at only where there
-    // are any
+    // in scalar registers, until a wave has seen the five that put the label
+    // behind both places (4096 x 49999 bf16, random labels: 220 -> 205 us); equal
+    // values are looked at only where there are any
     const int l = lab - j0;
     row.vecs(threadIdx.x, [&](int, int j, const float* z) {
-      uint64_t eq = 0;
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        m = fmaxf(m, z[e]);
-        before += __popcll(__ballot(z[e] > zl));
-        eq |= __ballot(z[e] == zl);
-      }
-      if (eq) {
+      for (int e = 0; e < V; ++e) m = fmaxf(m, z[e]);
+      if (before < 5) {
+        uint64_t eq = 0;
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-          before += __popcll(__ballot((z[e] == zl) & (j + e < l)));
+        for (int e = 0; e < V; ++e) {
+          before += __popcll(__ballot(z[e] > zl));
+          eq |= __ballot(z[e] == zl);
+        }
+        if (eq) {
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            before += __popcll(__ballot((z[e] == zl) & (j + e < l)));
+        }
       }
     });
     const int je = row.ej >= 0 ? row.ej : 0x7fffffff;
@@ -453,38 +458,47 @@ __global__ __launch_bounds__(TH) void distill_grad(const DistP P) {
 }
 
 // per configuration: mean loss, and acc += (sum of row losses, top-1, top-5, B)
-__global__ __launch_bounds__(256) void distill_sum(const float* __restrict__ rowloss,
-                                                   const int* __restrict__ rowhit,
-                                                   float* __restrict__ loss,
-                                                   float* __restrict__ acc, int B) {
-  __shared__ double sd[256];
-  __shared__ int s1[256], s5[256];
+template <int TH>
+__global__ __launch_bounds__(TH) void distill_sum(const float* __restrict__ rowloss,
+                                                  const int* __restrict__ rowhit,
+                                                  float* __restrict__ loss,
+                                                  float* __restrict__ acc, int B) {
+  constexpr int W = TH / 64;
+  __shared__ double sd[W];
+  __shared__ int s1[W], s5[W];
   const int g = blockIdx.x, t = threadIdx.x;
   double s = 0.0;
   int h1 = 0, h5 = 0;
-  for (int b = t; b < B; b += 256) {
+#pragma unroll 4
+  for (int b = t; b < B; b += TH) {
     s += (double)rowloss[(int64_t)g * B + b];
     const int h = rowhit[(int64_t)g * B + b];
     h1 += h & 1;
     h5 += h >> 1;
   }
-  sd[t] = s;
-  s1[t] = h1;
-  s5[t] = h5;
-  __syncthreads();
-  for (int o = 128; o > 0; o >>= 1) {
-    if (t < o) {
-      sd[t] += sd[t + o];
-      s1[t] += s1[t + o];
-      s5[t] += s5[t + o];
-    }
-    __syncthreads();
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    s += __shfl_xor(s, o);
+    h1 += __shfl_xor(h1, o);
+    h5 += __shfl_xor(h5, o);
   }
+  if ((t & 63) == 0) {
+    sd[t >> 6] = s;
+    s1[t >> 6] = h1;
+    s5[t >> 6] = h5;
+  }
+  __syncthreads();
   if (t == 0) {
-    loss[g] = (float)(sd[0] / (double)B);
-    acc[g * 4 + 0] += (float)sd[0];
-    acc[g * 4 + 1] += (float)s1[0];
-    acc[g * 4 + 2] += (float)s5[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+      s += sd[w];
+      h1 += s1[w];
+      h5 += s5[w];
+    }
+    loss[g] = (float)(s / (double)B);
+    acc[g * 4 + 0] += (float)s;
+    acc[g * 4 + 1] += (float)h1;
+    acc[g * 4 + 2] += (float)h5;
     acc[g * 4 + 3] += (float)B;
   }
 }
@@ -567,7 +581,10 @@ static int dist_fwd(DistP P, float* loss, float* acc, int64_t ws_floats, float* 
     CER_ROW_DISPATCH(T, P.N, CER_LR);
 #undef CER_LR
   }
-  distill_sum<<<P.G, 256, 0, st>>>(P.rowloss, P.rowhit, loss, acc, P.B);
+  // one block a configuration: 4096 rows 8.8 us with 256 threads, 4.6 with 1024; 32
+  // rows 1.9 us either way
+  if (P.B > 512) distill_sum<1024><<<P.G, 1024, 0, st>>>(P.rowloss, P.rowhit, loss, acc, P.B);
+  else distill_sum<256><<<P.G, 256, 0, st>>>(P.rowloss, P.rowhit, loss, acc, P.B);
   return (int)hipGetLastError();
 }
 
