@@ -127,6 +127,35 @@ def test_negative_and_zero_loss_gradients_and_tau_of_one(dtype, N):
     check(3, 6, N, 5, dtype, True, device=DEV, args=(z, lab, val, idx, alpha, tau))
 
 
+@pytest.mark.parametrize("N", [70, 1000, 5003, 49999, 70001])
+@DTYPES
+def test_places_near_the_fifth(dtype, N):
+    """Labels with 0 to 8 larger logits, gathered or spread, and up to 6 equal
+    ones before and after the label: one row per configuration."""
+    gen = torch.Generator().manual_seed(N)
+    rows, labs = [], []
+    for larger in (0, 1, 3, 4, 5, 8):
+        for same in (0, 1, 2, 6):
+            for near in (True, False):
+                z = -1.0 - torch.rand(N, generator=gen)
+                where = (torch.randperm(60, generator=gen) + torch.randint(0, N - 60, (1,), generator=gen)
+                         if near else torch.randperm(N, generator=gen))
+                z[where[:larger]] = 2.0 + torch.arange(larger)
+                z[where[larger:larger + same + 1]] = 1.0
+                rows.append(z)
+                labs.append(where[larger])
+    G = len(rows)
+    z = torch.cat(rows)[None].to(dtype).to(DEV)
+    lab = torch.stack(labs).int().view(G, 1).to(DEV)
+    acc = torch.zeros(G, 4, device=DEV)
+    idx = torch.zeros(G, 1, 1, dtype=torch.int32, device=DEV)
+    val = torch.zeros(G, 1, 1, device=DEV)
+    L.distill_ce(z.requires_grad_(True), lab, acc, G, val, idx, 0.5, 2.0, unit=True)
+    first, fifth = hits(z.detach(), lab)
+    assert torch.equal(acc[:, 1].long(), first) and torch.equal(acc[:, 2].long(), fifth)
+    assert 0 < first.sum() < fifth.sum() < G
+
+
 def test_alpha_of_zero_and_one():
     z, lab, val, idx, _, _ = inputs(3, 6, 40, 5, ragged=False, device=DEV)
     alpha = torch.tensor([0.0, 1.0, 0.5], device=DEV)
