@@ -23,9 +23,8 @@
 // terms p_i q_j with i + j <= 2, smallest first; what is dropped is below
 // 2^-24 of |x||w| a term, so the result is that of an fp32 product (measured
 // against 64 bits: as near as the library's) at 6/16 of the time of fp32 MFMA.
-// In bf16 mode dz = dy * act'(z) has more than 8 bits: it is kept in fp32,
-// enters dW as DZ_PLANES planes (dW is an fp32 tensor) and dx rounded to bf16 (as
-// dx itself is).  A non-finite fp32 factor gives a non-finite result,
+// In bf16 mode dz = dy * act'(z) has more than 8 bits: it is kept in fp32 and
+// enters dW, an fp32 tensor, as DZ_PLANES planes and dx, a bf16 one, as DX_PLANES.  A non-finite fp32 factor gives a non-finite result,
 // NaN where a single fp32 product would give an infinity; |x| above 3.39e38
 // rounds to infinity.
 #include <atomic>
@@ -942,14 +941,12 @@ constexpr int DA_COLS = 64;
 // rows of a block: 128, more where that keeps the ranges to 4096
 static inline int dact_rows(int M) { return M <= 128 * 4096 ? 128 : (M + 4095) / 4096; }
 
-// D: 0 none (dz is dy, only db is made), 1 u8 mask, 2 fp32 derivative.  dzr (or
-// null): dz rounded to bf16, the operand of dx; dW takes the fp32 one.
+// D: 0 none (dz is dy, only db is made), 1 u8 mask, 2 fp32 derivative
 template <typename T, int D, typename TZ>
 __global__ __launch_bounds__(256) void dense_dact(const T* __restrict__ dy, const void* __restrict__ d,
-                                                  TZ* __restrict__ dz, bf16_t* __restrict__ dzr,
-                                                  float* __restrict__ db, int64_t db_gs,
-                                                  float* __restrict__ part, int M, int C, int N,
-                                                  int rows) {
+                                                  TZ* __restrict__ dz, float* __restrict__ db,
+                                                  int64_t db_gs, float* __restrict__ part, int M,
+                                                  int C, int N, int rows) {
   __shared__ float sm[4][DA_COLS];
   const int c = blockIdx.x * DA_COLS + (threadIdx.x & 63), w = threadIdx.x >> 6;
   const int r0 = blockIdx.y * rows, r1 = min(M, r0 + rows);
@@ -962,7 +959,6 @@ __global__ __launch_bounds__(256) void dense_dact(const T* __restrict__ dy, cons
       if constexpr (D == 1) v = reinterpret_cast<const uint8_t*>(d)[i] ? v : 0.f;
       if constexpr (D == 2) v *= reinterpret_cast<const float*>(d)[i];
       if constexpr (D != 0) st1(dz + i, v);
-      if constexpr (D == 2 && sizeof(T) == 2) dzr[i] = f2bf(v);
       s += v;
     }
   }
@@ -1000,9 +996,13 @@ struct Plan {
   int tile, tm, tn, splits, steps;
 };
 
-// tile sizes by the planes of both operands together: 2 (bf16), 1 + DZ_PLANES
-// (dW of a bf16 layer with a smooth activation), 6 (fp32)
-constexpr int DZ_PLANES = 3;
+// tile sizes by the planes of both operands together: 2 (bf16), 1 + DZ_PLANES and
+// 1 + DX_PLANES (dW and dx of a bf16 layer with a smooth activation), 6 (fp32).
+// Two planes leave 2^-16 of dz, which dx's own rounding to bf16 covers: 8192 x 4096
+// x 4096 with gelu is 1.66e-3 from 64 bits, as fp32 sums rounded once are (they
+// differ by 1.04e-4, with three planes, 160 us more, by 0.77e-4).  One plane is
+// 2.35e-3.
+constexpr int DZ_PLANES = 3, DX_PLANES = 2;
 static constexpr int tile_m(int planes, int t) {
   return t == T_BIG ? (planes == 2 || planes == 6 ? 256 : 128) : t == T_MID ? 128 : t == T_SMALL ? 64 : 32;
 }
@@ -1028,7 +1028,7 @@ static constexpr int tile_occ(int planes, int t) {
 // up to 8 splits: the choice is on average 3 % slower than the best of them,
 // against 9 % for the constants that a first guess gave.
 static Plan choose_plan(int64_t m, int64_t n, int64_t k, int G, int planes, int out_bytes) {
-  const int passes = planes == 6 ? 6 : planes == 2 ? 1 : DZ_PLANES;
+  const int passes = planes == 6 ? 6 : planes - 1;
   const int esz = planes == 2 ? 2 : 4;
   static const double eff_f32[4] = {0.56, 0.33, 0.34, 0.17}, eff_bf16[4] = {0.40, 0.43, 0.19, 0.09};
   static const double latency[4] = {0.76, 0.69, 0.60, 0.35};       // us of a step
@@ -1148,7 +1148,8 @@ static int run_gemm(GemmP& P, const Plan& p, hipStream_t st) {
 
 static inline int planes_of(int kind, int is_bf16, int act) {
   if (!is_bf16) return 6;
-  return kind == 2 && act_smooth(act) ? 1 + DZ_PLANES : 2;
+  if (kind == 0 || !act_smooth(act)) return 2;
+  return 1 + (kind == 2 ? DZ_PLANES : DX_PLANES);
 }
 
 static inline Plan plan_of(int kind, int M, int N, int K, int G, int is_bf16, int act) {
@@ -1216,8 +1217,7 @@ static int dense_fwd(const T* x, int64_t ldx, const T* w, int64_t ws, const T* b
 
 // gradients: dx (or null) [M][G K], dW -> gw (fp32, config stride gs),
 // db -> gb (or null).  d: act'(z) of the forward; dz: scratch [M][G N] (T for
-// relu / relu6; fp32 for the smooth activations, and in bf16 mode [M][G N] bf16
-// behind it; unused for act none).
+// relu / relu6, fp32 for the smooth activations, unused for act none).
 template <typename T>
 static int dense_bwd(const T* dy, const void* d, void* dz, const T* x, int64_t ldx, const T* w,
                      int64_t ws, T* dx, float* gw, int64_t gs, float* gb, int64_t gbs, int M, int N,
@@ -1229,19 +1229,16 @@ static int dense_bwd(const T* dy, const void* d, void* dz, const T* x, int64_t l
   if (part_floats < cer_dense_ws(1, M, N, K, G, is_bf16, act)) return (int)hipErrorInvalidValue;
   const int C = G * N;
   const bool smooth = act_smooth(act);
-  bf16_t* dzr = is_bf16 && smooth ? (bf16_t*)((float*)dz + (int64_t)M * C) : nullptr;
   if (act != ACT_NONE || gb) {
     const int rows = dact_rows(M);
     const dim3 grid((C + DA_COLS - 1) / DA_COLS, (M + rows - 1) / rows);
     if (act == ACT_NONE)
-      dense_dact<T, 0, T><<<grid, 256, 0, st>>>(dy, nullptr, nullptr, nullptr, gb, gbs, part, M, C, N,
-                                                  rows);
+      dense_dact<T, 0, T><<<grid, 256, 0, st>>>(dy, nullptr, nullptr, gb, gbs, part, M, C, N, rows);
     else if (smooth)
-      dense_dact<T, 2, float><<<grid, 256, 0, st>>>(dy, d, (float*)dz, dzr, gb, gbs, part, M, C, N,
+      dense_dact<T, 2, float><<<grid, 256, 0, st>>>(dy, d, (float*)dz, gb, gbs, part, M, C, N,
                                                       rows);
     else
-      dense_dact<T, 1, T><<<grid, 256, 0, st>>>(dy, d, (T*)dz, nullptr, gb, gbs, part, M, C, N,
-                                                  rows);
+      dense_dact<T, 1, T><<<grid, 256, 0, st>>>(dy, d, (T*)dz, gb, gbs, part, M, C, N, rows);
     if (gb && grid.y > 1)
       dense_dbsum<<<grid.x, 256, 0, st>>>(part, grid.y, gb, gbs, C, N);
   }
@@ -1265,12 +1262,14 @@ static int dense_bwd(const T* dy, const void* d, void* dz, const T* x, int64_t l
   }
   if (!dx) return 0;
   GemmP P = {};
-  P.a = dzr ? dzr : z; P.lda = C; P.a_gs = N;
+  P.a = z; P.lda = C; P.a_gs = N;
   P.b = w; P.ldb = K; P.b_gs = ws;
   P.m = M; P.n = K; P.k = N; P.G = G;
   P.c = dx; P.ldc = (int64_t)G * K; P.c_gs = K;
   P.part = part;
   const Plan p = plan_of(1, M, N, K, G, is_bf16, act);
+  if constexpr (is_bf16)
+    if (smooth) return run_gemm<float, T, DX_PLANES, 1, false, true, EPI_T, T>(P, p, st);
   constexpr int PL = is_bf16 ? 1 : 3;
   return run_gemm<T, T, PL, PL, false, true, EPI_T, T>(P, p, st);
 }

@@ -111,9 +111,8 @@ struct LinearActBackward : public Node {
     const bool need_dx = task_should_compute_output(0);
     const int64_t n = cer_dense_ws(1, p.M, p.N, p.K, p.G, p.bf16, p.act);
     TORCH_CHECK(n >= 0, "linear_act: sizes out of range");
-    // one temporary: the workspace and dz (fp32, and beside it bf16 in that mode)
-    const int64_t c = p.M * p.G * p.N;
-    const Tensor tmp = floats(xv, n + (p.act ? c + (p.bf16 ? (c + 1) / 2 : 0) : 0));
+    // one temporary: the workspace and dz
+    const Tensor tmp = floats(xv, n + (p.act ? p.M * p.G * p.N : 0));
     if (need_dx) out[0] = at::empty({p.M, p.G * p.K}, xv.options());
     done((p.bf16 ? cer_dense_bwd : cer_dense_bwd_f32)(
              dy.data_ptr(), d.defined() ? d.data_ptr() : nullptr, p.act ? fptr(tmp) + n : nullptr,

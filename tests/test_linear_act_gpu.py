@@ -423,3 +423,32 @@ def test_residual_is_the_input():
     r = x.detach().clone().requires_grad_(True)
     g1, g2 = torch.autograd.grad(P.linear_act(x, w, b, "gelu", r), [x, r], dy)
     assert torch.equal(gx, g1 + g2)
+
+
+@pytest.mark.parametrize("act", SMOOTH)
+@pytest.mark.parametrize("size", [(2, 70, 33, 24), (1, 3, 300, 40), (1, 520, 261, 24),
+                                  (1, 4100, 2104, 24)], ids=lambda s: "x".join(map(str, s)))
+def test_bf16_input_gradient_is_rounded_once(size, act):
+    """dx of a bf16 layer: z exact (x and w on a grid), dz off by the evaluation
+    of act' (2^-20 (1 + |z|) of dy) and by what its two planes leave (2^-16), N
+    fp32 additions, and one rounding to bf16."""
+    G, M, K, N = size
+    arena, w, b = make(G, N, K, torch.bfloat16, device=DEV)
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    w.master().copy_((w.master() * 16).round().clamp(-8, 8) / 16)
+    b.master().copy_((b.master() * 4).round() / 4)
+    arena.sync_work()
+    x = ((torch.randn(M, G * K, generator=gen, device=DEV) * 4).round().clamp(-8, 8) / 8).bfloat16()
+    dy = torch.randn(M, G * N, generator=gen, device=DEV).bfloat16()
+    x.requires_grad_(True)
+    dx, = torch.autograd.grad(P.linear_act(x, w, b, act), [x], dy)
+    for g in range(G):
+        ws = w.work()[g].double()
+        z = x.detach()[:, g * K:(g + 1) * K].double() @ ws.t() + b.work()[g].double()
+        z.requires_grad_(True)
+        dyg = dy[:, g * N:(g + 1) * N].double()
+        dz, = torch.autograd.grad(ACT64[act](z), [z], dyg)
+        want, S = dz @ ws, dz.abs() @ ws.abs()
+        e = (2.0 ** -16 + (N + 1) * 2.0 ** -24) * S + 1.01 * 2.0 ** -20 * (
+            (dyg.abs() * (1 + z.detach().abs())) @ ws.abs())
+        _within(dx[:, g * K:(g + 1) * K], want, e + 2.0 ** -8 * (want.abs() + e), ("dx", g))
