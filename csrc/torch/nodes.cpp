@@ -174,8 +174,29 @@ struct Teacher {
   double alpha0, tau0;
 };
 
+// A backward reads these again beside sums that the forward made of them: one that
+// was written in between is refused.  An inference tensor counts no writes; it is
+// copied.
+static SavedVariable saved(const Tensor& t) {
+  return SavedVariable(t.defined() && t.is_inference() ? t.clone() : t, false);
+}
+
+struct SavedTeacher {
+  SavedVariable labels, val, idx, alpha, tau;
+  double alpha0 = 0, tau0 = 0;
+
+  SavedTeacher() = default;
+  explicit SavedTeacher(const Teacher& t)
+      : labels(saved(t.labels)), val(saved(t.val)), idx(saved(t.idx)), alpha(saved(t.alpha)),
+        tau(saved(t.tau)), alpha0(t.alpha0), tau0(t.tau0) {}
+
+  Teacher unpack() const {
+    return {labels.unpack(), val.unpack(), idx.unpack(), alpha.unpack(), tau.unpack(), alpha0, tau0};
+  }
+};
+
 struct DistillBackward : public Node {
-  Teacher t;
+  SavedTeacher teacher;
   SavedVariable z;
   Tensor stats, d;              // d: the finished gradient of a unit loss gradient
   int64_t G;
@@ -192,6 +213,7 @@ struct DistillBackward : public Node {
       return out;
     }
     const Tensor zv = z.unpack();
+    const Teacher t = teacher.unpack();
     const c10::OptionalDeviceGuard guard(zv.device());
     const Tensor dloss = grads[0].contiguous();
     const bool bf16 = zv.scalar_type() == at::kBFloat16;
@@ -210,7 +232,7 @@ struct DistillBackward : public Node {
     z.reset_data();
     stats.reset();
     d.reset();
-    t = Teacher{};
+    teacher = SavedTeacher();
   }
 };
 
@@ -244,7 +266,7 @@ static Tensor distill_ce(const Tensor& z, const Tensor& labels, const Tensor& ac
       node->d = std::move(d);
     } else {
       node->z = SavedVariable(z, false);
-      node->t = std::move(t);
+      node->teacher = SavedTeacher(t);
       node->stats = std::move(buf);
     }
     torch::autograd::set_history(loss, node);

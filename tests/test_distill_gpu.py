@@ -504,3 +504,43 @@ def test_more_than_two_to_the_31_elements():
     d, dm = d * 40 / B, dm * 40 / B
     tol = 2.0 ** -20 * 40 * dm
     assert ((grads[0][tail].double() - d).abs() <= tol + 2.0 ** -8 * (d.abs() + tol) + 1e-30).all()
+
+
+def test_inputs_written_before_the_backward_are_refused():
+    """The general gradient reads labels, entries and weights again; the unit
+    gradient is finished in the forward."""
+    for name in ("logits", "labels", "top_val", "top_idx", "alpha", "tau", None):
+        for unit in (False, True):
+            z, lab, val, idx, alpha, tau = inputs(2, 6, 30, 4, device=DEV)
+            x = z.clone().requires_grad_(True)
+            h = x * 1.0
+            t = {"logits": h, "labels": lab, "top_val": val, "top_idx": idx, "alpha": alpha,
+                 "tau": tau}
+            loss = L.distill_ce(h, lab, torch.zeros(2, 4, device=DEV), 2, val, idx, alpha, tau,
+                                unit=unit)
+            if name is not None:
+                t[name].mul_(1)                         # a write, whatever it writes
+            if name is None or unit:
+                d, = torch.autograd.grad(loss, [x], torch.ones(2, device=DEV))
+                assert torch.isfinite(d).all()
+            else:
+                with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                    torch.autograd.grad(loss, [x], torch.ones(2, device=DEV))
+
+
+def test_teacher_made_in_inference_mode():
+    """Such tensors count no writes: the gradient is of the values at the call."""
+    z, lab, val, idx, alpha, tau = inputs(2, 6, 30, 4, device=DEV)
+    with torch.inference_mode():
+        ival, iidx, ialpha = val.clone(), idx.clone(), alpha.clone()
+    grads = []
+    for v, i, a in ((val, idx, alpha), (ival, iidx, ialpha)):
+        x = z.clone().requires_grad_(True)
+        loss = L.distill_ce(x, lab, torch.zeros(2, 4, device=DEV), 2, v, i, a, tau)
+        if v is ival:
+            with torch.inference_mode():
+                ival.zero_()
+                iidx.zero_()
+                ialpha.zero_()
+        grads.append(torch.autograd.grad(loss, [x], torch.ones(2, device=DEV))[0])
+    assert torch.equal(*grads)
