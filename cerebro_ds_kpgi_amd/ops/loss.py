@@ -147,7 +147,8 @@ class DistillCE(torch.autograd.Function):
         d, = ctx.saved_tensors
         if not ctx.unit:                # else dloss is ones by the caller's contract
             d = (d.view(d.shape[0], ctx.G, -1) * dloss.view(1, ctx.G, 1)).view(d.shape)
-        return (d.to(ctx.dtype),) + (None,) * 8
+        # a copy: the caller may write its gradient and run a kept graph again
+        return (d.to(ctx.dtype, copy=True),) + (None,) * 8
 
 
 def _distill_torch(logits, labels, acc, G, val, idx, alpha, tau):

@@ -12,6 +12,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/graph_task.h>
 
 #include <optional>
 
@@ -209,7 +210,8 @@ struct DistillBackward : public Node {
     if (unit) {
       TORCH_CHECK(d.defined(), "distill_ce: backward through the graph a second time; its gradient "
                                "was freed (retain_graph=True keeps it)");
-      out[0] = d;
+      // a graph that is kept may be run again: the caller may write its gradient
+      out[0] = torch::autograd::get_current_graph_task_keep_graph() ? d.clone() : d;
       return out;
     }
     const Tensor zv = z.unpack();

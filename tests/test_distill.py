@@ -237,3 +237,14 @@ def test_top_logits_cpu(dtype):
         assert torch.equal(v.nan_to_num(9e9), vr.nan_to_num(9e9))
     zz = z.clone().requires_grad_(True)
     assert not L.top_logits(zz, 3, 2)[0].requires_grad
+
+
+@pytest.mark.parametrize("unit", [True, False])
+def test_gradients_of_a_kept_graph_are_the_callers(unit):
+    z, lab, val, idx, alpha, tau = inputs(2, 6, 30, 4)
+    x = z.clone().requires_grad_(True)
+    loss = L.distill_ce(x, lab, torch.zeros(2, 4), 2, val, idx, alpha, tau, unit=unit)
+    first, = torch.autograd.grad(loss, [x], torch.ones(2), retain_graph=True)
+    want = first.clone()
+    first.mul_(100.0)
+    assert torch.equal(torch.autograd.grad(loss, [x], torch.ones(2))[0], want)

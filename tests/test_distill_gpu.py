@@ -544,3 +544,20 @@ def test_teacher_made_in_inference_mode():
                 ialpha.zero_()
         grads.append(torch.autograd.grad(loss, [x], torch.ones(2, device=DEV))[0])
     assert torch.equal(*grads)
+
+
+@pytest.mark.parametrize("unit", [True, False])
+def test_gradients_of_a_kept_graph_are_the_callers(unit):
+    z, lab, val, idx, alpha, tau = inputs(2, 6, 30, 4, device=DEV)
+    x = z.clone().requires_grad_(True)
+    ones = torch.ones(2, device=DEV)
+    loss = L.distill_ce(x, lab, torch.zeros(2, 4, device=DEV), 2, val, idx, alpha, tau, unit=unit)
+    first, = torch.autograd.grad(loss, [x], ones, retain_graph=True)
+    want = first.clone()
+    first.mul_(100.0)                            # a caller that scales or clips in place
+    second, = torch.autograd.grad(loss, [x], ones, retain_graph=True)
+    assert torch.equal(second, want)
+    loss.backward(ones, retain_graph=True)
+    x.grad.zero_()
+    third, = torch.autograd.grad(loss, [x], ones)
+    assert torch.equal(third, want)
