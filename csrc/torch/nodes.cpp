@@ -10,10 +10,13 @@
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/graph_task.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
+#include <initializer_list>
 #include <optional>
 
 using torch::Tensor;
@@ -71,6 +74,19 @@ static void rows_fit(const char* name, int64_t rows) {
 
 static void done(int rc, const char* name) {
   TORCH_CHECK(rc == 0, name, " failed with hipError ", rc);
+}
+
+// What a tracer would record of these calls are the empty outputs, and what a dual
+// number would get is no tangent, that is a derivative of zero: both are refused.
+static void eager_and_reverse(const char* name, std::initializer_list<const Tensor*> inputs) {
+  using c10::impl::TorchDispatchModeKey;
+  using c10::impl::TorchDispatchModeTLS;
+  TORCH_CHECK_NOT_IMPLEMENTED(
+      !torch::jit::tracer::isTracing() && !TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY),
+      name, " cannot be traced");
+  for (const Tensor* t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), name,
+                                " has no forward-mode derivative");
 }
 
 static void once(const char* name) {
@@ -138,6 +154,8 @@ static Tensor linear_act(const Tensor& x, const std::optional<Tensor>& anchor,
                          const std::optional<Tensor>& residual, const Tensor& work,
                          const std::optional<Tensor>& grad, int64_t w_off, int64_t b_off, int64_t N,
                          int64_t K, int64_t act, bool train) {
+  eager_and_reverse("linear_act",
+                    {&x, anchor ? &*anchor : &x, residual ? &*residual : &x, &work});
   rows_fit("linear_act", x.size(0));
   const c10::OptionalDeviceGuard guard(x.device());
   Dense p{work, grad.value_or(Tensor()), w_off, b_off, x.size(0), N, K, work.size(0), act,
@@ -242,6 +260,7 @@ static Tensor distill_ce(const Tensor& z, const Tensor& labels, const Tensor& ac
                          const Tensor& val, const Tensor& idx, const std::optional<Tensor>& alpha,
                          double alpha0, const std::optional<Tensor>& tau, double tau0, bool unit,
                          bool train) {
+  eager_and_reverse("distill_ce", {&z, &val, alpha ? &*alpha : &z, tau ? &*tau : &z});
   rows_fit("distill_ce", z.size(0));
   const c10::OptionalDeviceGuard guard(z.device());
   const bool bf16 = z.scalar_type() == at::kBFloat16;
@@ -278,6 +297,7 @@ static Tensor distill_ce(const Tensor& z, const Tensor& labels, const Tensor& ac
 
 // ---------------------------------------------------------------------------
 static std::tuple<Tensor, Tensor> top_logits(const Tensor& z, int64_t G, int64_t k) {
+  eager_and_reverse("top_logits", {});
   rows_fit("top_logits", z.size(0) * G);
   const c10::OptionalDeviceGuard guard(z.device());
   const bool bf16 = z.scalar_type() == at::kBFloat16;

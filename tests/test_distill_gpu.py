@@ -561,3 +561,27 @@ def test_gradients_of_a_kept_graph_are_the_callers(unit):
     x.grad.zero_()
     third, = torch.autograd.grad(loss, [x], ones)
     assert torch.equal(third, want)
+
+
+def test_tracers_and_dual_numbers_are_refused():
+    """Neither can see into the kernels: a trace would hold empty outputs, a dual
+    number would come back without its tangent."""
+    from test_linear_act import make
+    from torch.autograd import forward_ad
+    arena, w, b = make(device=DEV)
+    z, lab, val, idx, alpha, tau = inputs(2, 4, 6, 3, device=DEV)
+    x = torch.randn(4, 10, device=DEV)
+
+    def loss(z):
+        return L.distill_ce(z, lab, torch.zeros(2, 4, device=DEV), 2, val, idx, alpha, tau)
+    for f, t in ((lambda x: P.linear_act(x, w, b, "silu"), x), (loss, z),
+                 (lambda z: L.top_logits(z, 2, 2), z)):
+        with pytest.raises(NotImplementedError, match="cannot be traced"):
+            torch.jit.trace(f, (t,))
+    with forward_ad.dual_level():
+        for f, t in ((lambda x: P.linear_act(x, w, b, "silu"), x), (loss, z),
+                     (lambda r: P.linear_act(x, w, b, "silu", r), torch.randn(4, 6, device=DEV))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                f(forward_ad.make_dual(t, torch.ones_like(t)))
+        # a teacher's logits have no derivative to lose
+        L.top_logits(forward_ad.make_dual(z, torch.ones_like(z)), 2, 2)

@@ -103,3 +103,37 @@ def test_refusals():
     _, w3, b3 = make(dtype=torch.bfloat16, trainable=False)
     with pytest.raises(ValueError, match="parks"):
         P.linear_act(x.bfloat16(), w3, b3)
+
+
+def test_kernels_refuse_tracers_and_dual_numbers():
+    """At the door of the compiled calls, before anything is looked at."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from cerebro_ds_kpgi_amd.ops import _hip
+    arena, w, b = make()
+    n = _hip.nodes()
+    i32 = torch.int32
+
+    def linear(x, r=None):
+        return n.linear_act(x, None, r, arena.work, arena.grad, w.spec.offset, b.spec.offset, 3, 5,
+                            0, False)
+
+    def distill(z, val=torch.zeros(2, 4, 1), tau=torch.ones(2)):
+        return n.distill_ce(z, torch.zeros(2, 4, dtype=i32), torch.zeros(2, 4), 2, val,
+                            torch.zeros(2, 4, 1, dtype=i32), None, 0.5, tau, 0.0, False, False)
+
+    def top(z):
+        return n.top_logits(z, 2, 1)
+    x, r = torch.randn(4, 10), torch.randn(4, 6)
+    for f, t in ((lambda t: linear(t), x), (lambda t: distill(t), r), (lambda t: top(t), r)):
+        with pytest.raises(NotImplementedError, match="cannot be traced"):
+            torch.jit.trace(f, (t,))
+        with pytest.raises(NotImplementedError, match="cannot be traced"):
+            make_fx(f)(t)
+    with torch.autograd.forward_ad.dual_level():
+        def dual(t):
+            return torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+        for f in (lambda: linear(dual(x)), lambda: linear(x, dual(r)), lambda: distill(dual(r)),
+                  lambda: distill(r, dual(torch.zeros(2, 4, 1))),
+                  lambda: distill(r, tau=dual(torch.ones(2)))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                f()
