@@ -108,7 +108,8 @@ def _logit_rows(what, logits, G):
     if logits.shape[0] == 0:
         raise ValueError("{}: no rows".format(what))
     if logits.stride(1) != 1 or logits.stride(0) < logits.shape[1]:
-        logits = logits.contiguous()
+        # the reshape gives a single row its own length as pitch, whatever it had
+        logits = logits.reshape(-1, logits.shape[1]).contiguous()
     return logits, logits.shape[1] // G
 
 

@@ -248,3 +248,21 @@ def test_gradients_of_a_kept_graph_are_the_callers(unit):
     want = first.clone()
     first.mul_(100.0)
     assert torch.equal(torch.autograd.grad(loss, [x], torch.ones(2))[0], want)
+
+
+def one_row_layouts(z):
+    """[1, W] views of a row whose pitch is below W."""
+    col = z.reshape(-1).clone()[:, None]                        # [W, 1]
+    yield col.t()
+    yield z.contiguous().as_strided(z.shape, (0, 1))
+    yield torch.cat([col, col], 1)[:, :1].t()
+
+
+def test_a_single_row_has_a_pitch():
+    z = torch.randn(1, 10)
+    for x in one_row_layouts(z):
+        assert x.stride(0) < 10
+        rows, N = L._logit_rows("test", x, 2)
+        assert rows.stride() == (10, 1) and N == 5 and torch.equal(rows, z)
+    # one class and one config: any stride between elements that are not there
+    assert L._logit_rows("test", torch.randn(6, 3)[:, 1:2], 1)[0].stride(0) >= 1

@@ -585,3 +585,17 @@ def test_tracers_and_dual_numbers_are_refused():
                 f(forward_ad.make_dual(t, torch.ones_like(t)))
         # a teacher's logits have no derivative to lose
         L.top_logits(forward_ad.make_dual(z, torch.ones_like(z)), 2, 2)
+
+
+def test_a_single_row_of_any_pitch():
+    from test_distill import one_row_layouts
+    z, lab, val, idx, alpha, tau = inputs(2, 1, 60, 4, device=DEV)
+
+    def run(x):
+        x = x.detach().requires_grad_(True)
+        acc = torch.zeros(2, 4, device=DEV)
+        loss = L.distill_ce(x, lab, acc, 2, val, idx, alpha, tau)
+        return [loss.detach(), acc, torch.autograd.grad(loss.sum(), [x])[0], *L.top_logits(x, 2, 7)]
+    want = run(z)
+    for x in one_row_layouts(z):
+        assert all(torch.equal(a, b) for a, b in zip(run(x), want))
