@@ -100,6 +100,22 @@ static Tensor floats(const Tensor& like, int64_t n) {
 
 static float* fptr(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
 
+// All that a backward reads goes through SavedVariable: hooks on saved tensors
+// (offload, checkpoints) see it, and an input that was written in between is
+// refused.  An inference tensor counts no writes; it is copied.
+static SavedVariable saved(const Tensor& t) {
+  return SavedVariable(t.defined() && t.is_inference() ? t.clone() : t, false);
+}
+
+// What a hook gives back has the values but not always the layout: elements of a
+// row adjacent, and for a matrix a pitch of at least its width.
+static Tensor adjacent(const Tensor& t) {
+  const int64_t last = t.dim() - 1;
+  const bool is = (t.size(last) <= 1 || t.stride(last) == 1) &&
+                  (t.dim() != 2 || t.stride(0) >= t.size(1));
+  return is ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
 // ---------------------------------------------------------------------------
 struct Dense {
   Tensor work, grad;            // the arena's rows [G, n]
@@ -114,15 +130,16 @@ struct Dense {
 
 struct LinearActBackward : public Node {
   Dense p;
-  SavedVariable x;
-  Tensor d;
+  SavedVariable x, derivative;  // act'(z)
 
   variable_list apply(variable_list&& grads) override {
     variable_list out(3);
     const Tensor g0 = grads[0];
     if (!g0.defined()) return out;
     once("linear_act");
-    const Tensor xv = x.unpack();
+    const Tensor xv = adjacent(x.unpack());
+    Tensor d = derivative.unpack();
+    if (d.defined()) d = d.contiguous();
     const c10::OptionalDeviceGuard guard(xv.device());
     const Tensor dy = g0.contiguous();
     const bool need_dx = task_should_compute_output(0);
@@ -144,7 +161,7 @@ struct LinearActBackward : public Node {
 
   void release_variables() override {
     x.reset_data();
-    d.reset();
+    derivative.reset_data();
   }
 };
 
@@ -181,7 +198,7 @@ static Tensor linear_act(const Tensor& x, const std::optional<Tensor>& anchor,
                                                              residual.value_or(Tensor())));
     node->p = std::move(p);
     node->x = SavedVariable(x, false);
-    node->d = std::move(d);
+    node->derivative = saved(d);
     torch::autograd::set_history(y, node);
   }
   return y;
@@ -193,13 +210,7 @@ struct Teacher {
   double alpha0, tau0;
 };
 
-// A backward reads these again beside sums that the forward made of them: one that
-// was written in between is refused.  An inference tensor counts no writes; it is
-// copied.
-static SavedVariable saved(const Tensor& t) {
-  return SavedVariable(t.defined() && t.is_inference() ? t.clone() : t, false);
-}
-
+// read again in the backward, beside sums that the forward made of them
 struct SavedTeacher {
   SavedVariable labels, val, idx, alpha, tau;
   double alpha0 = 0, tau0 = 0;
@@ -210,14 +221,18 @@ struct SavedTeacher {
         tau(saved(t.tau)), alpha0(t.alpha0), tau0(t.tau0) {}
 
   Teacher unpack() const {
-    return {labels.unpack(), val.unpack(), idx.unpack(), alpha.unpack(), tau.unpack(), alpha0, tau0};
+    Teacher t{labels.unpack().contiguous(), adjacent(val.unpack()), adjacent(idx.unpack()),
+              alpha.unpack(), tau.unpack(), alpha0, tau0};
+    if (t.alpha.defined()) t.alpha = t.alpha.contiguous();
+    if (t.tau.defined()) t.tau = t.tau.contiguous();
+    return t;
   }
 };
 
 struct DistillBackward : public Node {
   SavedTeacher teacher;
-  SavedVariable z;
-  Tensor stats, d;              // d: the finished gradient of a unit loss gradient
+  SavedVariable z, stats;
+  SavedVariable finished;       // the gradient for a unit loss gradient
   int64_t G;
   bool unit;
 
@@ -226,13 +241,13 @@ struct DistillBackward : public Node {
     if (!grads[0].defined()) return out;
     once("distill_ce");
     if (unit) {
-      TORCH_CHECK(d.defined(), "distill_ce: backward through the graph a second time; its gradient "
-                               "was freed (retain_graph=True keeps it)");
+      const Tensor d = finished.unpack();
       // a graph that is kept may be run again: the caller may write its gradient
       out[0] = torch::autograd::get_current_graph_task_keep_graph() ? d.clone() : d;
       return out;
     }
-    const Tensor zv = z.unpack();
+    const Tensor zv = adjacent(z.unpack());
+    const Tensor sums = stats.unpack().contiguous();
     const Teacher t = teacher.unpack();
     const c10::OptionalDeviceGuard guard(zv.device());
     const Tensor dloss = grads[0].contiguous();
@@ -242,7 +257,7 @@ struct DistillBackward : public Node {
              zv.data_ptr(), zv.stride(0), t.labels.data_ptr<int>(), t.val.data_ptr(),
              t.val.scalar_type() == at::kFloat, t.val.stride(0), t.val.stride(1),
              t.idx.data_ptr<int>(), t.idx.stride(0), t.idx.stride(1), fptr(t.alpha), t.alpha0,
-             fptr(t.tau), t.tau0, fptr(dloss), fptr(stats), out[0].data_ptr(), zv.size(0), G,
+             fptr(t.tau), t.tau0, fptr(dloss), fptr(sums), out[0].data_ptr(), zv.size(0), G,
              zv.size(1) / G, t.val.size(2), stream_of(zv)),
          "cer_distill_bwd");
     return out;
@@ -250,8 +265,8 @@ struct DistillBackward : public Node {
 
   void release_variables() override {
     z.reset_data();
-    stats.reset();
-    d.reset();
+    stats.reset_data();
+    finished.reset_data();
     teacher = SavedTeacher();
   }
 };
@@ -284,11 +299,11 @@ static Tensor distill_ce(const Tensor& z, const Tensor& labels, const Tensor& ac
     node->G = G;
     node->unit = unit;
     if (unit) {
-      node->d = std::move(d);
+      node->finished = saved(d);
     } else {
       node->z = SavedVariable(z, false);
       node->teacher = SavedTeacher(t);
-      node->stats = std::move(buf);
+      node->stats = saved(buf.narrow(0, 0, 4 * G * B));
     }
     torch::autograd::set_history(loss, node);
   }

@@ -599,3 +599,33 @@ def test_a_single_row_of_any_pitch():
     want = run(z)
     for x in one_row_layouts(z):
         assert all(torch.equal(a, b) for a, b in zip(run(x), want))
+
+
+@pytest.mark.parametrize("unit", [True, False])
+@pytest.mark.parametrize("B", [1, 6])
+def test_hooks_and_checkpoints_see_what_is_saved(B, unit):
+    from torch.autograd.graph import saved_tensors_hooks
+    from torch.utils.checkpoint import checkpoint
+    z, lab, val, idx, alpha, tau = inputs(2, B, 30, 4, device=DEV)
+    x = z.clone().requires_grad_(True)
+    ones = torch.ones(2, device=DEV)
+
+    def loss(x):
+        return L.distill_ce(x, lab, torch.zeros(2, 4, device=DEV), 2, val, idx[:1].expand(2, -1, -1),
+                            alpha, tau, unit=unit)
+    want, = torch.autograd.grad(loss(x), [x], ones)
+    packed = []
+
+    def pack(t):
+        packed.append(tuple(t.shape))
+        return t.cpu()
+
+    def unpack(t):
+        return t.to(DEV) if t.dim() < 2 else t.transpose(-1, -2).contiguous().to(DEV).transpose(-1, -2)
+    with saved_tensors_hooks(pack, unpack):
+        y = loss(x)
+    assert (B, 60) in packed
+    assert unit or (2, B, 4) in packed and (2, B) in packed and (2,) in packed
+    assert torch.equal(torch.autograd.grad(y, [x], ones)[0], want)
+    y = checkpoint(loss, x, use_reentrant=False)
+    assert torch.equal(torch.autograd.grad(y, [x], ones)[0], want)

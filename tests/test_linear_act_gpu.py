@@ -452,3 +452,37 @@ def test_bf16_input_gradient_is_rounded_once(size, act):
         e = (2.0 ** -16 + (N + 1) * 2.0 ** -24) * S + 1.01 * 2.0 ** -20 * (
             (dyg.abs() * (1 + z.detach().abs())) @ ws.abs())
         _within(dx[:, g * K:(g + 1) * K], want, e + 2.0 ** -8 * (want.abs() + e), ("dx", g))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("act", ["none", "relu", "gelu"])
+@pytest.mark.parametrize("M", [1, 7])
+def test_hooks_and_checkpoints_see_what_is_saved(M, act, dtype):
+    from torch.autograd.graph import saved_tensors_hooks
+    from torch.utils.checkpoint import checkpoint
+    arena, w, b = make(2, 12, 12, dtype, device=DEV)
+    x = torch.randn(M, 24, device=DEV).to(dtype).requires_grad_(True)
+    dy = torch.randn(M, 24, device=DEV).to(dtype)
+
+    def block(x):
+        return P.linear_act(x, w, b, act, x)
+    want, = torch.autograd.grad(block(x), [x], dy)
+    want = [want, w.grad().clone(), b.grad().clone()]
+    packed = []
+
+    def pack(t):
+        packed.append((tuple(t.shape), t.dtype))
+        return t.cpu()
+    # what comes back has another layout
+    with saved_tensors_hooks(pack, lambda t: t.t().contiguous().to(DEV).t()):
+        y = block(x)
+    assert ((M, 24), dtype) in packed
+    if act != "none":
+        assert ((M, 24), torch.uint8 if act == "relu" else torch.float32) in packed
+    arena.grad.fill_(5.0)
+    got = [torch.autograd.grad(y, [x], dy)[0], w.grad(), b.grad()]
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    arena.grad.fill_(5.0)
+    y = checkpoint(block, x, use_reentrant=False)
+    got = [torch.autograd.grad(y, [x], dy)[0], w.grad(), b.grad()]
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
