@@ -412,15 +412,16 @@ __global__ __launch_bounds__(SL_TH) void distill_rows(const DistP P) {
   int nthere;
   const RowW w = teacher<SL_TH>(P, g, b, lab, ti, tp, sm, plogp, nthere);
   // join the slices in their order; one of nothing but -inf brings its sums
-  // (zero, or NaN where it holds NaN) as they are
+  // (zero, or NaN where it holds NaN) as they are, unless the whole row is
   float mx = -INFINITY, s1 = 0.f, s2 = 0.f, cnt = 0.f;
   const int64_t st = (int64_t)P.G * P.B * 4;
   const float* p = P.part + ((int64_t)g * P.B + b) * 4;
   for (int s = 0; s < P.slices; ++s) mx = fmaxf(mx, p[s * st]);
   for (int s = 0; s < P.slices; ++s) {
-    const float x = p[s * st] - mx;
-    s1 += p[s * st + 1] * (x == -INFINITY ? 1.f : ex2(x * LOG2E));
-    s2 += p[s * st + 2] * (x == -INFINITY ? 1.f : ex2(x * LOG2E * w.itau));
+    const float m = p[s * st], x = m - mx;
+    const bool none = m == -INFINITY && mx != -INFINITY;
+    s1 += p[s * st + 1] * (none ? 1.f : ex2(x * LOG2E));
+    s2 += p[s * st + 2] * (none ? 1.f : ex2(x * LOG2E * w.itau));
     cnt += p[s * st + 3];
   }
   const float c = w.soft ? cross<T, SL_TH>(P, zr, ti, tp, w, mx, s2, sm) : 0.f;

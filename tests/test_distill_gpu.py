@@ -629,3 +629,21 @@ def test_hooks_and_checkpoints_see_what_is_saved(B, unit):
     assert torch.equal(torch.autograd.grad(y, [x], ones)[0], want)
     y = checkpoint(loss, x, use_reentrant=False)
     assert torch.equal(torch.autograd.grad(y, [x], ones)[0], want)
+
+
+@pytest.mark.parametrize("N", [1000, 70001, 140001])
+@DTYPES
+def test_lowest_values_beside_a_huge_one(dtype, N):
+    """The type's lowest value below a maximum of 1e37: their difference is beyond
+    fp32, the probability zero all the same -- also of a slice of nothing else."""
+    z = torch.full((2, N), torch.finfo(dtype).min, dtype=dtype, device=DEV)
+    z[:, 5] = 1e37
+    lab = torch.full((1, 2), 5, dtype=torch.int32, device=DEV)
+    idx = torch.full((1, 2, 1), 5, dtype=torch.int32, device=DEV)
+    val = torch.zeros(1, 2, 1, device=DEV)
+    for unit in (True, False):
+        for tau in (1.0, 2.0):
+            x = z.clone().requires_grad_(True)
+            loss = L.distill_ce(x, lab, torch.zeros(1, 4, device=DEV), 1, val, idx, 0.5, tau, unit=unit)
+            d, = torch.autograd.grad(loss, [x], torch.ones(1, device=DEV))
+            assert float(loss) == 0 and not d.any()
