@@ -152,7 +152,7 @@ __device__ __forceinline__ RowW teacher(const DistP& P, int g, int b, int lab, i
     block_sum3<TH>(s, t, u, sm);
     const float is = 1.f / s;
     for (int k = threadIdx.x; k < P.K; k += TH) tp[k] *= is;
-    plogp = t * is - __logf(s);
+    plogp = t * is - logf(s);
   }
   return w;
 }
@@ -162,7 +162,7 @@ template <typename T, int TH>
 __device__ __forceinline__ float cross(const DistP& P, const T* zr, const int* ti, const float* tp,
                                        const RowW& w, float mx, float s2, float* sm) {
   float c = 0.f, d0 = 0.f, d1 = 0.f;
-  const float l2 = __logf(s2);
+  const float l2 = logf(s2);
   for (int k = threadIdx.x; k < P.K; k += TH)
     if (ti[k] >= 0 && tp[k] > 0.f) c += tp[k] * ((ld1(zr + ti[k]) - mx) * w.itau - l2);
   block_sum3<TH>(c, d0, d1, sm);
@@ -174,7 +174,7 @@ __device__ __forceinline__ void row_result(const DistP& P, int g, int b, int lab
                                            float plogp, float c, float mx, float s1, float zl,
                                            float cnt) {
   float row = 0.f;
-  if (w.hard) row += (1.f - w.a) * (__logf(s1) + (mx - zl));
+  if (w.hard) row += (1.f - w.a) * (logf(s1) + (mx - zl));
   if (w.soft) row += w.a * w.tau * w.tau * (plogp - c);
   if (w.bad) row = NAN;
   const int64_t o = (int64_t)g * P.B + b;
@@ -185,10 +185,11 @@ __device__ __forceinline__ void row_result(const DistP& P, int g, int b, int lab
 }
 
 // coefficients of a row's gradient: before the entries it is
-// sgn (2^((z - mx) k + o1) + 2^((z - mx) k2 + o2)), the factors c / sum in the
-// exponents
+// c1 2^((z - mx) log2 e) + c2 2^((z - mx) k2).  The factors stay out of the exponents,
+// whose rounding is relative to their size: log2(c / s) of -16 to -32 there made
+// every term 2^-20 wrong (fp32 8192 x 1000: 2.9e-7 from 64 bits, so 0.5e-7).
 struct GradW {
-  float mx, k2, o1, o2, sgn, ch, cs;
+  float mx, k2, c1, c2, ch, cs;
   bool hard, soft, one;
 };
 
@@ -202,13 +203,11 @@ __device__ __forceinline__ GradW grad_weights(const DistP& P, const RowW& w, int
   q.k2 = LOG2E * w.itau;
   q.ch = (1.f - w.a) * sc;
   q.cs = w.a * w.tau * sc;
-  q.sgn = sc < 0.f ? -1.f : 1.f;
   q.mx = mx;
-  q.o1 = __log2f(q.ch * q.sgn / s1);
-  q.o2 = __log2f(q.cs * q.sgn / s2);
   // at tau = 1 both terms have one exponential
   q.one = q.hard && q.soft && w.tau == 1.f;
-  if (q.one) q.o1 = __log2f((q.ch + q.cs) * q.sgn / s1);
+  q.c1 = (q.one ? q.ch + q.cs : q.ch) / s1;
+  q.c2 = q.cs / s2;
   return q;
 }
 
@@ -216,15 +215,14 @@ template <bool HARD, bool SOFT>
 __device__ __forceinline__ float grad_of(const GradW& q, float z) {
   const float x = z - q.mx;
   float d = 0.f;
-  if (HARD) d = ex2(fmaf(x, LOG2E, q.o1));
-  if (SOFT) d = HARD ? d + ex2(fmaf(x, q.k2, q.o2)) : ex2(fmaf(x, q.k2, q.o2));
+  if (HARD) d = q.c1 * ex2(x * LOG2E);
+  if (SOFT) d = HARD ? fmaf(q.c2, ex2(x * q.k2), d) : q.c2 * ex2(x * q.k2);
   return d;
 }
 
 __device__ __forceinline__ float grad_base(const GradW& q, float z) {
-  const float d = q.hard ? (q.soft && !q.one ? grad_of<true, true>(q, z) : grad_of<true, false>(q, z))
-                         : (q.soft ? grad_of<false, true>(q, z) : 0.f);
-  return d * q.sgn;
+  return q.hard ? (q.soft && !q.one ? grad_of<true, true>(q, z) : grad_of<true, false>(q, z))
+                : (q.soft ? grad_of<false, true>(q, z) : 0.f);
 }
 
 // The label's and the teacher's classes in [lo, hi): written whole, after the
@@ -274,8 +272,6 @@ template <typename T, int TH, int R>
 __device__ __forceinline__ void grad_row(const RowRegs<T, TH, R>& row, const GradW& q, T* dr) {
   if (!q.hard && !q.soft)
     write_row(row, dr, [&](float) { return 0.f; });
-  else if (q.sgn < 0.f)          // a negative loss gradient
-    write_row(row, dr, [&](float z) { return grad_base(q, z); });
   else if (q.hard && q.soft && !q.one)
     write_row(row, dr, [&](float z) { return grad_of<true, true>(q, z); });
   else if (q.hard)
