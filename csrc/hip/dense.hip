@@ -51,8 +51,43 @@ static inline bool act_known(int a) {
 }
 __host__ __device__ static inline bool act_smooth(int a) { return a >= ACT_GELU; }
 
+// 1 / (1 + e), 0 <= e <= 1: the hardware's reciprocal and one Newton step
+__device__ __forceinline__ float rcp1p(float e) {
+  const float x = 1.f + e, r = __builtin_amdgcn_rcpf(x);
+  return fmaf(fmaf(-x, r, 1.f), r, r);
+}
+
+// Polynomials of the normal distribution, coefficients from the constant up: least
+// squares reweighted until the largest relative error of Phi stops falling (4 000
+// and 8 000 points, in 64 bits).
+//   |z| <= 1.5: (Phi(z) - 1/2) / z in z^2, to 2^-30
+//   1.5 <= a:   Phi(-a) exp(a^2 / 2) in 1 / (a + 1.5), to 2^-25
+__device__ __forceinline__ float phi_mid(float z2) {
+  float p = 4.0268761836159683e-07f;
+  p = fmaf(p, z2, -8.652973519929219e-06f);
+  p = fmaf(p, z2, 1.1417106e-04f);
+  p = fmaf(p, z2, -1.1862358e-03f);
+  p = fmaf(p, z2, 9.9730734e-03f);
+  p = fmaf(p, z2, -6.6490285e-02f);
+  return fmaf(p, z2, 3.9894226e-01f);
+}
+
+__device__ __forceinline__ float phi_tail(float a) {
+  const float t = __builtin_amdgcn_rcpf(a + 1.5f);
+  float p = -6.780151844024658f;
+  p = fmaf(p, t, 11.185012817382812f);
+  p = fmaf(p, t, -6.108560085296631f);
+  p = fmaf(p, t, 0.24226641654968262f);
+  p = fmaf(p, t, 0.4250870943069458f);
+  p = fmaf(p, t, 0.6031176447868347f);
+  p = fmaf(p, t, 0.39877673983573914f);
+  return fmaf(p, t, 2.4561902591813123e-06f);
+}
+
 // act(z), and act'(z) in d.  NaN passes through every branch (comparisons with
-// NaN are false), unlike fmaxf.
+// NaN are false), unlike fmaxf.  The smooth ones are as near to 64 bits as erf, tanh
+// and exp in fp32 (standard normal z: gelu 3.6e-8, its derivative 3.7e-8), and keep
+// their relative error far below zero: nothing is left of 1 by subtraction.
 __device__ __forceinline__ float act_fwd(float z, int act, float& d) {
   if (act == ACT_NONE) {
     d = 1.f;
@@ -66,51 +101,32 @@ __device__ __forceinline__ float act_fwd(float z, int act, float& d) {
     d = (z > 0.f && z < 6.f) ? 1.f : 0.f;
     return z <= 0.f ? 0.f : (z >= 6.f ? 6.f : z);
   }
+  const float a = fabsf(z);
+  // beyond the float range of exp the limits, not inf * 0
+  if (a > 1e4f) {
+    d = z < 0.f ? 0.f : 1.f;
+    return z < 0.f ? 0.f : z;
+  }
   if (act == ACT_GELU) {
-    // Phi(z) by Abramowitz & Stegun 7.1.26 (|error of erf| <= 1.5e-7), whose
-    // exp(-z^2/2) is also the density that act' needs: one exponential and one
-    // reciprocal for both
-    const float x = fabsf(z) * 0.70710678118654752f;
-    const float e = __expf(-x * x);
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
-    float p = fmaf(t, 1.061405429f, -1.453152027f);
-    p = fmaf(t, p, 1.421413741f);
-    p = fmaf(t, p, -0.284496736f);
-    p = fmaf(t, p, 0.254829592f);
-    const float tail = 0.5f * p * t * e;              // Phi(-|z|)
-    const float cdf = z < 0.f ? tail : 1.f - tail;
-    d = fmaf(z, e * 0.39894228040143268f, cdf);
-    // beyond the float range of exp the limits, not inf * 0
-    if (fabsf(z) > 1e4f) {
-      d = z < 0.f ? 0.f : 1.f;
-      return z < 0.f ? 0.f : z;
-    }
+    const float z2 = z * z, e = expf(-0.5f * z2);
+    const float tail = phi_tail(a) * e;
+    const float cdf = a < 1.5f ? fmaf(z, phi_mid(z2), 0.5f) : z < 0.f ? tail : 1.f - tail;
+    d = fmaf(z * 0.39894228040143268f, e, cdf);
     return z * cdf;
   }
   if (act == ACT_GELU_TANH) {
     const float c = 0.79788456080286536f;
     const float u = c * z * fmaf(0.044715f * z, z, 1.f);
-    // tanh(u) = 1 - 2 / (exp(2u) + 1); exp overflows to inf -> 1, 0 -> -1
-    const float q = __builtin_amdgcn_rcpf(__expf(2.f * u) + 1.f);   // (1 - tanh u) / 2
-    const float s = 1.f - q;                                        // (1 + tanh u) / 2
-    if (fabsf(z) > 1e4f) {
-      d = z < 0.f ? 0.f : 1.f;
-      return z < 0.f ? 0.f : z;
-    }
+    // (1 + tanh u) / 2 = 1 / (1 + exp(-2u)), and q = (1 - tanh u) / 2
+    const float e = expf(-2.f * fabsf(u)), r = rcp1p(e), er = e * r;
+    const float s = z < 0.f ? er : r, q = z < 0.f ? r : er;
     d = fmaf(2.f * z * s * q, c * fmaf(0.134145f * z, z, 1.f), s);
     return z * s;
   }
   // silu
-  const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z));
-  if (z < -1e4f) {
-    d = 0.f;
-    return 0.f;
-  }
-  if (z > 1e4f) {
-    d = 1.f;
-    return z;
-  }
-  d = s * fmaf(z, 1.f - s, 1.f);
+  const float e = expf(-a), r = rcp1p(e), er = e * r;
+  const float s = z < 0.f ? er : r, q = z < 0.f ? r : er;
+  d = s * fmaf(z, q, 1.f);
   return z * s;
 }
 

@@ -12,6 +12,8 @@ Lipschitz constant (below 1.13 for act, below 1.1 for act') plus 2^-20 for its
 evaluation in fp32 (relative to 1 + |z|).
 """
 
+import math
+
 import pytest
 import torch
 
@@ -486,3 +488,39 @@ def test_hooks_and_checkpoints_see_what_is_saved(M, act, dtype):
     y = checkpoint(block, x, use_reentrant=False)
     got = [torch.autograd.grad(y, [x], dy)[0], w.grad(), b.grad()]
     assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_activations_in_fp32():
+    """One input, one weight of 1: y is act(x) and dx act'(x), whose steps count.
+    In 2^-24 of the value (half a step): gelu below -1.5 a polynomial (3), its
+    argument and exp (2 each), exp's argument (z^2 / 2), two products; within 1.5
+    three steps of z times the polynomial, 0.7, and two of Phi.  silu exp, the
+    reciprocal and their product (2, 2, 1), one product.  tanh gelu three steps
+    of u, doubled in exp(2u)."""
+    arena, w, _ = make(1, 1, 1, bias=False, device=DEV)
+    w.master().fill_(1.0)
+    arena.sync_work()
+    h = 2.0 ** -24
+    for act, far in (("gelu", 12.0), ("silu", 80.0), ("gelu_tanh", 5.0)):
+        gen = torch.Generator(device=DEV).manual_seed(0)
+        u = torch.rand(1 << 17, 1, generator=gen, device=DEV) * 2 - 1
+        x = torch.cat([u[::2] * far, u[1::2] * 3]).requires_grad_(True)
+        y = P.linear_act(x, w, None, act)
+        dx, = torch.autograd.grad(y, [x], torch.ones_like(y))
+        z = x.detach().double().requires_grad_(True)
+        if act == "gelu":               # erfc keeps the digits of the far tail
+            cdf = 0.5 * torch.special.erfc(-z * math.sqrt(0.5))
+            want = z * cdf
+            cdf = cdf.detach()
+            tol = z.abs() * (cdf * (9 + z * z / 2) + 0.7 * (z.abs() < 1.5)) * h
+        elif act == "silu":
+            want = z / (1 + torch.exp(-z))
+            tol = 6 * h * want.abs()
+        else:
+            t = math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)
+            want = z / (1 + torch.exp(-2 * t))
+            tol = (8 + 6 * t.abs()) * h * want.abs()
+        d, = torch.autograd.grad(want.sum(), [z])
+        _within(y.detach(), want.detach(), tol.detach(), act)
+        # sums of terms below 1.13, 0.25 |exp's argument|, 0.7: a few steps of 1
+        _within(dx, d, torch.full_like(d, (4 if act == "gelu" else 8) * h), act + "'")
