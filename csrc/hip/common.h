@@ -9,6 +9,11 @@
 #include <hip/hip_bf16.h>
 #include <stdint.h>
 
+// a launch has fewer than 2^32 threads along x
+static inline bool grid_fits(int64_t blocks, int threads) {
+  return blocks <= 0x7fffffff && blocks * threads < ((int64_t)1 << 32);
+}
+
 #define CER_API extern "C" __attribute__((visibility("default")))
 
 typedef uint16_t bf16_t;  // raw bf16 bits (round-to-nearest-even conversions below)

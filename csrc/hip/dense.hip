@@ -1028,6 +1028,7 @@ static constexpr int tile_n(int planes, int t) {
 static constexpr int tile_k(int planes, int t) {
   return t == T_THIN ? 64 : planes == 2 ? (t == T_MID ? 32 : 64) : 32;
 }
+static constexpr int tile_threads(int t) { return t == T_BIG ? 512 : 256; }
 // blocks of a CU (LDS and registers)
 static constexpr int tile_occ(int planes, int t) {
   return t == T_BIG ? 1 : t == T_MID ? 2 : t == T_SMALL ? (planes == 2 ? 4 : 3) : planes == 2 ? 3 : 2;
@@ -1042,7 +1043,8 @@ static constexpr int tile_occ(int planes, int t) {
 // constants are fitted to 282 products (1 - 16 configurations, 1 - 16384 rows, 2
 // - 8192 columns, all three forms, both types), each timed under every tile and
 // up to 8 splits: the choice is on average 3 % slower than the best of them,
-// against 9 % for the constants that a first guess gave.
+// against 9 % for the constants that a first guess gave.  splits == 0: no tile
+// covers the product in one launch.
 static Plan choose_plan(int64_t m, int64_t n, int64_t k, int G, int planes, int out_bytes) {
   const int passes = planes == 6 ? 6 : planes - 1;
   const int esz = planes == 2 ? 2 : 4;
@@ -1061,6 +1063,7 @@ static Plan choose_plan(int64_t m, int64_t n, int64_t k, int G, int planes, int 
     for (int64_t s = 1; s <= 16 && s <= (total + 1) / 2; s = s < 4 ? s + 1 : s + s / 3) {
       const int64_t steps = (total + s - 1) / s, sp = (total + steps - 1) / steps;
       const double blocks = (double)nt * sp;
+      if (!grid_fits(nt * sp, tile_threads(t))) continue;
       const double rounds = ceil(blocks / (256.0 * occ));
       // a part-filled round runs as fast as its fullest CU
       const double share = rounds > 1 ? occ : ceil(blocks / 256.0);
@@ -1112,7 +1115,7 @@ static int launch_gemm(GemmP& P, const Plan& p, hipStream_t st) {
   P.splits = p.splits;
   P.steps = p.steps;
   const int64_t blocks = (int64_t)P.G * p.tm * p.tn * p.splits;
-  if (blocks > 0x7fffffff) return (int)hipErrorInvalidValue;
+  if (p.splits < 1 || !grid_fits(blocks, WM * WN * 64)) return (int)hipErrorInvalidValue;
   constexpr int stage = 2 * (PA * BM + PB * BN) * BK * 2;
   // the epilogue's: sums, and the residual that waits
   constexpr int turn = WM * WN * (BM / WM < 32 ? 16 : 32) *
@@ -1178,9 +1181,10 @@ static inline Plan plan_of(int kind, int M, int N, int K, int G, int is_bf16, in
 
 static inline bool sizes_ok(int M, int N, int K, int G, int64_t ldx) {
   // byte offsets inside a tile are 32-bit: 255 rows of the longest pitch and a
-  // chunk
+  // chunk.  Row numbers are ints, also those of the last tile and of the last of
+  // 4096 row ranges, 2^19 rows and more past M
   const int64_t most = ((int64_t)1 << 32) / (256 * 4);
-  return M > 0 && N > 0 && K > 0 && G > 0 && (int64_t)G * N < most && (int64_t)G * K < most &&
+  return M > 0 && M <= 0x7fffffff - (1 << 20) && N > 0 && K > 0 && G > 0 && (int64_t)G * N < most && (int64_t)G * K < most &&
          N < most && K < most && ldx >= (int64_t)G * K && ldx < most;
 }
 
@@ -1190,10 +1194,11 @@ CER_API int64_t cer_dense_ws(int kind, int M, int N, int K, int G, int is_bf16, 
   if (!sizes_ok(M, N, K, G, (int64_t)G * K) || !act_known(act)) return -1;
   auto need = [&](int kd, int64_t m, int64_t n) {
     const Plan p = plan_of(kd, M, N, K, G, is_bf16, act);
-    return p.splits > 1 ? (int64_t)p.splits * G * m * n : 0;
+    return p.splits < 1 ? -1 : p.splits > 1 ? (int64_t)p.splits * G * m * n : 0;
   };
   if (kind == 0) return gemv_better(M, N, K, G, is_bf16) ? 0 : need(0, M, N);
   const int64_t a = need(1, M, K), b = need(2, N, K);
+  if (a < 0 || b < 0) return -1;
   const int64_t nb = (M + dact_rows(M) - 1) / dact_rows(M);
   const int64_t c = nb > 1 ? nb * G * N : 0;
   return a > b ? (a > c ? a : c) : (b > c ? b : c);

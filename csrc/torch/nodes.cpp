@@ -67,9 +67,10 @@ static void* stream_of(const Tensor& t) {
   return c10::hip::getCurrentHIPStream(t.device().index()).stream();
 }
 
-// row counts go to the kernels as int
-static void rows_fit(const char* name, int64_t rows) {
-  TORCH_CHECK_VALUE(rows <= INT32_MAX, name, ": ", rows, " rows are more than 2^31 - 1");
+// sizes go to the kernels as int
+static void ints(const char* name, std::initializer_list<int64_t> sizes) {
+  for (int64_t n : sizes)
+    TORCH_CHECK_VALUE(n <= INT32_MAX, name, ": ", n, " rows or columns are more than 2^31 - 1");
 }
 
 static void done(int rc, const char* name) {
@@ -173,13 +174,14 @@ static Tensor linear_act(const Tensor& x, const std::optional<Tensor>& anchor,
                          int64_t K, int64_t act, bool train) {
   eager_and_reverse("linear_act",
                     {&x, anchor ? &*anchor : &x, residual ? &*residual : &x, &work});
-  rows_fit("linear_act", x.size(0));
+  ints("linear_act", {x.size(0), x.size(1), work.size(0) * N});
   const c10::OptionalDeviceGuard guard(x.device());
   Dense p{work, grad.value_or(Tensor()), w_off, b_off, x.size(0), N, K, work.size(0), act,
           x.scalar_type() == at::kBFloat16};
   const int64_t n = cer_dense_ws(0, p.M, N, K, p.G, p.bf16, act);
-  TORCH_CHECK_VALUE(n >= 0, "linear_act: M=", p.M, " N=", N, " K=", K, " G=", p.G,
-                    " is beyond the kernels' 32-bit tile offsets");
+  TORCH_CHECK_VALUE(n >= 0 && (!train || cer_dense_ws(1, p.M, N, K, p.G, p.bf16, act) >= 0),
+                    "linear_act: M=", p.M, " N=", N, " K=", K, " G=", p.G,
+                    " is beyond the kernels' 32-bit offsets and grids");
   const Tensor ws = floats(x, n);
   Tensor y = at::empty({p.M, p.G * N}, x.options());
   Tensor d;
@@ -276,11 +278,13 @@ static Tensor distill_ce(const Tensor& z, const Tensor& labels, const Tensor& ac
                          double alpha0, const std::optional<Tensor>& tau, double tau0, bool unit,
                          bool train) {
   eager_and_reverse("distill_ce", {&z, &val, alpha ? &*alpha : &z, tau ? &*tau : &z});
-  rows_fit("distill_ce", z.size(0));
-  const c10::OptionalDeviceGuard guard(z.device());
   const bool bf16 = z.scalar_type() == at::kBFloat16;
   const int64_t B = z.size(0), N = z.size(1) / G;
+  ints("distill_ce", {B, G, N});
+  const c10::OptionalDeviceGuard guard(z.device());
   const int64_t n = cer_distill_ws(B, G, N, bf16);
+  TORCH_CHECK_VALUE(n >= 0, "distill_ce: B=", B, " G=", G, " N=", N,
+                    " is beyond the kernels' grids");
   Tensor loss = at::empty({G}, z.options().dtype(at::kFloat));
   Tensor buf = floats(z, 4 * G * B + n);        // stats for the backward, workspace
   Tensor d;
@@ -313,13 +317,15 @@ static Tensor distill_ce(const Tensor& z, const Tensor& labels, const Tensor& ac
 // ---------------------------------------------------------------------------
 static std::tuple<Tensor, Tensor> top_logits(const Tensor& z, int64_t G, int64_t k) {
   eager_and_reverse("top_logits", {});
-  rows_fit("top_logits", z.size(0) * G);
-  const c10::OptionalDeviceGuard guard(z.device());
   const bool bf16 = z.scalar_type() == at::kBFloat16;
   const int64_t B = z.size(0), N = z.size(1) / G;
+  ints("top_logits", {B * G, N});
+  const c10::OptionalDeviceGuard guard(z.device());
+  const int64_t n = cer_top_ws(B, G, N, k, bf16);
+  TORCH_CHECK_VALUE(n >= 0, "top_logits: B=", B, " G=", G, " N=", N, " k=", k,
+                    " is beyond the kernels' grids");
   Tensor val = at::empty({G, B, k}, z.options());
   Tensor idx = at::empty({G, B, k}, z.options().dtype(at::kInt));
-  const int64_t n = cer_top_ws(B, G, N, k, bf16);
   Tensor ws = n > 0 ? at::empty({n}, z.options().dtype(at::kLong)) : Tensor();
   done((bf16 ? cer_top_logits : cer_top_logits_f32)(
            z.data_ptr(), z.stride(0), val.data_ptr(), idx.data_ptr<int>(), B, G, N, k,

@@ -137,3 +137,26 @@ def test_kernels_refuse_tracers_and_dual_numbers():
                   lambda: distill(r, tau=dual(torch.ones(2)))):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 f()
+
+
+def test_rows_beyond_the_kernels_integers_are_refused():
+    """Row numbers are ints, with room for the last tile and the last range of
+    rows; a launch has fewer than 2^32 threads."""
+    import ctypes
+    from cerebro_ds_kpgi_amd.ops import _hip
+    ws = _hip.lib().cer_dense_ws
+    ws.restype = ctypes.c_int64
+    for bf16 in (0, 1):
+        for act in (0, 1, 7):
+            for kind in (0, 1):
+                assert ws(kind, 2 ** 29 + 3, 1, 1, 1, bf16, act) >= 0
+                assert ws(kind, 2 ** 31 - 2 ** 21, 4, 1, 1, bf16, act) >= 0
+                for M in (2 ** 31 - 2 ** 20, 2 ** 31 - 1):
+                    assert ws(kind, M, 1, 1, 1, bf16, act) == -1
+            # 2^31 x 2^21 outputs: no tile covers them in one launch
+            assert ws(0, 2 ** 31 - 2 ** 21, 2 ** 21, 1, 1, bf16, act) == -1
+    arena, w, b = make(1, 1, 1)
+    for M in (2 ** 31 - 1, 2 ** 31 + 5):
+        with pytest.raises(ValueError, match="32-bit|2\\^31"):
+            _hip.nodes().linear_act(torch.zeros(1, 1).expand(M, 1), None, None, arena.work,
+                                    arena.grad, w.spec.offset, b.spec.offset, 1, 1, 0, False)

@@ -524,3 +524,23 @@ def test_activations_in_fp32():
         _within(y.detach(), want.detach(), tol.detach(), act)
         # sums of terms below 1.13, 0.25 |exp's argument|, 0.7: a few steps of 1
         _within(dx, d, torch.full_like(d, (4 if act == "gelu" else 8) * h), act + "'")
+
+
+def test_rows_beyond_a_grid_of_small_tiles():
+    """2^29 + 3 rows of one column: a tile of 32 rows would take 2^32 threads."""
+    M = 2 ** 29 + 3
+    arena, w, b = make(1, 1, 1, torch.bfloat16, device=DEV)
+    w.master().fill_(2.0)
+    b.master().fill_(0.5)
+    arena.sync_work()
+    x = torch.zeros(M, 1, dtype=torch.bfloat16, device=DEV)
+    dy = torch.zeros_like(x)
+    rows = torch.tensor([0, 31, 2 ** 28, 2 ** 29 - 1, 2 ** 29, M - 1], device=DEV)
+    x[rows, 0] = torch.arange(1, 7, device=DEV).bfloat16()
+    dy[rows, 0] = torch.tensor([1.0, -2.0, 4.0, 8.0, 16.0, 32.0], device=DEV).bfloat16()
+    x.requires_grad_(True)
+    y = P.linear_act(x, w, b, "none")
+    dx, = torch.autograd.grad(y, [x], dy)
+    assert torch.equal(y.detach(), 2 * x.detach() + 0.5) and torch.equal(dx, 2 * dy)
+    xs, ds = x.detach()[rows, 0].double(), dy[rows, 0].double()
+    assert float(w.grad()) == float((xs * ds).sum()) and float(b.grad()) == float(ds.sum())
