@@ -503,6 +503,8 @@ __global__ __launch_bounds__(TH) void distill_sum(const float* __restrict__ rowl
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
+CER_API int64_t cer_distill_ws(int B, int G, int N, int is_bf16);
+
 template <typename T>
 static int64_t slice_of(int N) {
   // longest row of distill_row: 1024 threads x 16 vectors
@@ -527,10 +529,13 @@ static int64_t slice_of(int N) {
     else LAUNCH(1024, 16);                              \
   } while (0)
 
+static inline int row_threads(int N, int v) {       // of CER_ROW_DISPATCH and the slices
+  return N <= 64 * v ? 64 : N <= 256 * 26 * v ? 256 : N <= 512 * 16 * v ? 512 : N <= 1024 * 16 * v ? 1024 : SL_TH;
+}
+
 template <typename T>
 static bool dist_ok(const DistP& P) {
-  return P.z && P.labels && P.B > 0 && P.G > 0 &&
-         P.G <= 65535 && P.N > 0 && P.K >= 0 && P.K <= KMAX && (P.K == 0 || (P.val && P.idx)) &&
+  return P.z && P.labels && cer_distill_ws(P.B, P.G, P.N, sizeof(T) == 2) >= 0 && P.K >= 0 && P.K <= KMAX && (P.K == 0 || (P.val && P.idx)) &&
          P.ldz >= (int64_t)P.G * P.N;
 }
 
@@ -539,7 +544,6 @@ static int launch_grad(DistP P, hipStream_t st) {
   const int64_t sl = slice_of<T>(P.N);
   P.slice = sl ? (int)sl : P.N;
   P.slices = (P.N + P.slice - 1) / P.slice;
-  if ((int64_t)P.slices * P.B > 0x7fffffff) return (int)hipErrorInvalidValue;
   const dim3 grid(P.slices * P.B, P.G);
   if (sl) {
     distill_grad<T, SL_TH, SL_R><<<grid, SL_TH, 0, st>>>(P);
@@ -565,7 +569,6 @@ static int dist_fwd(DistP P, float* loss, float* acc, int64_t ws_floats, float* 
   P.part = ws + 2 * rows;
   if (sl) {
     P.slice = (int)sl;
-    if ((int64_t)P.slices * P.B > 0x7fffffff) return (int)hipErrorInvalidValue;
     distill_stats<T><<<dim3(P.slices * P.B, P.G), SL_TH, 0, st>>>(P);
     distill_rows<T><<<dim3(P.B, P.G), SL_TH, 0, st>>>(P);
     if (P.dz) {
@@ -599,10 +602,12 @@ static DistP dist_params(const void* z, int64_t ldz, const int* labels, const vo
   return P;
 }
 
-// floats of workspace of a forward
+// floats of workspace of a forward, -1 for sizes out of range
 CER_API int64_t cer_distill_ws(int B, int G, int N, int is_bf16) {
-  if (B <= 0 || G <= 0 || N <= 0) return -1;
+  if (B <= 0 || G <= 0 || G > 65535 || N <= 0 || N >= 0x7ffffff0) return -1;
   const int64_t sl = is_bf16 ? slice_of<bf16_t>(N) : slice_of<float>(N);
+  const int64_t slices = sl ? (N + sl - 1) / sl : 1;
+  if (!grid_fits(slices * B, row_threads(N, is_bf16 ? 8 : 4))) return -1;
   return (int64_t)B * G * (2 + (sl ? 4 * ((N + sl - 1) / sl) : 0));
 }
 

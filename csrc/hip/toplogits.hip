@@ -411,6 +411,12 @@ static inline bool top_sizes(int B, int G, int N, int K) {
          (int64_t)B * G <= 0x7fffffff;
 }
 
+template <typename T>
+static int top_threads(int chunk) {
+  constexpr int V = 16 / (int)sizeof(T);
+  return chunk <= 64 * V ? 64 : chunk <= 256 * 8 * V ? 256 : chunk <= 512 * 16 * V ? 512 : 1024;
+}
+
 static inline int top_room(int K) { return K < 32 ? 64 : 2 * K; }
 
 // 64-bit numbers of workspace, -1 for sizes out of range
@@ -420,7 +426,7 @@ static int64_t top_ws(int B, int G, int N, int K) {
   const int64_t rows = (int64_t)B * G;
   const int c = top_chunk<T>(rows, N, K);
   const int64_t chunks = (N + c - 1) / c;
-  if (rows * chunks > 0x7fffffff) return -1;
+  if (!grid_fits(rows * chunks, top_threads<T>(c)) || !grid_fits(rows, chunks > 1 ? TM_TH : 1)) return -1;
   return chunks > 1 ? rows * chunks * top_room(K) : 0;
 }
 
@@ -449,6 +455,7 @@ static int top_launch(const T* z, int64_t ldz, T* val, int* idx, int B, int G, i
   // blocks on a CU
   P.cand = n <= 64 * V ? 512 : K <= 256 ? 1024 : TOP_CAND;
 #define CER_TOP(TH, R) top_rows<T, TH, R><<<grid, TH, P.cand * sizeof(uint64_t), st>>>(P)
+  // (top_threads knows these)
   if (n <= 64 * V) CER_TOP(64, 1);
   else if (n <= 256 * V) CER_TOP(256, 1);
   else if (n <= 256 * 4 * V) CER_TOP(256, 4);

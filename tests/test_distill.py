@@ -266,3 +266,28 @@ def test_a_single_row_has_a_pitch():
         assert rows.stride() == (10, 1) and N == 5 and torch.equal(rows, z)
     # one class and one config: any stride between elements that are not there
     assert L._logit_rows("test", torch.randn(6, 3)[:, 1:2], 1)[0].stride(0) >= 1
+
+
+def test_sizes_beyond_the_kernels_are_refused():
+    """Classes are ints (2^32 + 5 of them were taken for 5), a launch has fewer
+    than 2^32 threads and 65536 configurations."""
+    import ctypes
+    from cerebro_ds_kpgi_amd.ops import _hip
+    lib, n = _hip.lib(), _hip.nodes()
+    ws, top = lib.cer_distill_ws, lib.cer_top_ws
+    ws.restype = top.restype = ctypes.c_int64
+    for bf16 in (0, 1):
+        assert ws(2 ** 26 - 1, 1, 2, bf16) > 0 and ws(2 ** 26, 1, 2, bf16) == -1
+        assert ws(2 ** 24 - 1, 1, 600, bf16) > 0 and ws(2 ** 24, 1, 600, bf16) == -1
+        assert ws(2 ** 20, 1, 2 ** 24, bf16) == -1 and ws(1, 1, 2 ** 31 - 1, bf16) == -1
+        assert ws(1, 65535, 5, bf16) > 0 and ws(1, 65536, 5, bf16) == -1
+        assert top(2 ** 26 - 1, 1, 2, 1, bf16) == 0 and top(2 ** 26, 1, 2, 1, bf16) == -1
+        assert top(1, 2 ** 24, 600, 1, bf16) == -1 and top(2 ** 22, 1, 70000, 1, bf16) == -1
+    i32 = torch.int32
+    for N in (2 ** 31 - 1, 2 ** 31 + 8, 2 ** 32 + 5):
+        z = torch.zeros(1, 1).expand(1, N)
+        with pytest.raises(ValueError, match="grids|2\\^31"):
+            n.top_logits(z, 1, 3)
+        with pytest.raises(ValueError, match="grids|2\\^31"):
+            n.distill_ce(z, torch.zeros(1, 1, dtype=i32), torch.zeros(1, 4), 1, torch.zeros(1, 1, 1),
+                         torch.zeros(1, 1, 1, dtype=i32), None, 0.5, None, 1.0, False, False)
