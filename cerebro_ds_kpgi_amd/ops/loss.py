@@ -145,6 +145,9 @@ class DistillCE(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dloss):
+        if torch.is_grad_enabled():
+            raise RuntimeError("distill_ce has no second derivative (its backward ran with "
+                               "create_graph=True)")
         d, = ctx.saved_tensors
         if not ctx.unit:                # else dloss is ones by the caller's contract
             d = (d.view(d.shape[0], ctx.G, -1) * dloss.view(1, ctx.G, 1)).view(d.shape)

@@ -782,6 +782,9 @@ class PackedLinearAct(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
+        if torch.is_grad_enabled():
+            raise RuntimeError("linear_act has no second derivative (its backward ran with "
+                               "create_graph=True)")
         x, d = ctx.saved_tensors
         wref, bref = ctx.wref, ctx.bref
         G = wref.G

@@ -291,3 +291,14 @@ def test_sizes_beyond_the_kernels_are_refused():
         with pytest.raises(ValueError, match="grids|2\\^31"):
             n.distill_ce(z, torch.zeros(1, 1, dtype=i32), torch.zeros(1, 4), 1, torch.zeros(1, 1, 1),
                          torch.zeros(1, 1, 1, dtype=i32), None, 0.5, None, 1.0, False, False)
+
+
+def test_no_second_derivative_on_the_cpu():
+    """Not even in part: through the loss gradient of a squared loss."""
+    z, lab, val, idx, alpha, tau = inputs(2, 4, 6, 3)
+    for unit in (True, False):
+        x = z.clone().requires_grad_(True)
+        loss = L.distill_ce(x, lab, torch.zeros(2, 4), 2, val, idx, alpha, tau, unit=unit)
+        with pytest.raises(RuntimeError, match="second derivative"):
+            d, = torch.autograd.grad((loss * loss).sum(), [x], create_graph=True)
+            torch.autograd.grad(d.sum(), [x])

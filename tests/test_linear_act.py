@@ -160,3 +160,13 @@ def test_rows_beyond_the_kernels_integers_are_refused():
         with pytest.raises(ValueError, match="32-bit|2\\^31"):
             _hip.nodes().linear_act(torch.zeros(1, 1).expand(M, 1), None, None, arena.work,
                                     arena.grad, w.spec.offset, b.spec.offset, 1, 1, 0, False)
+
+
+def test_no_second_derivative_on_the_cpu():
+    """The weights are no leaves, so a second derivative would lack their part."""
+    arena, w, b = make()
+    x = torch.randn(4, 10, requires_grad=True)
+    y = P.linear_act(x, w, b, "silu")
+    with pytest.raises(RuntimeError, match="second derivative"):
+        d, = torch.autograd.grad((y * y).sum(), [x], create_graph=True)
+        torch.autograd.grad(d.sum(), [x])
