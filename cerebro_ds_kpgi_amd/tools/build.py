@@ -103,7 +103,8 @@ def build_nodes(jobs=8):
     link = ["-L" + d for d in ext.library_paths()] + ["-lc10", "-lc10_hip", "-ltorch_cpu",
                                                       "-ltorch", "-ltorch_python"]
     out = os.path.join(LIBDIR, "cerebro_nodes.so")
-    return _build("nodes", srcs, [], out, os.environ.get("CXX", "g++"), flags, link, jobs)
+    headers = [os.path.join(ROOT, "csrc", "hip", "nodes_api.h")]
+    return _build("nodes", srcs, headers, out, os.environ.get("CXX", "g++"), flags, link, jobs)
 
 
 def build_all(jobs=8):

@@ -31,6 +31,7 @@
 #include <math.h>
 
 #include "common.h"
+#include "nodes_api.h"
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -1295,34 +1296,14 @@ static int dense_bwd(const T* dy, const void* d, void* dz, const T* x, int64_t l
   return run_gemm<T, T, PL, PL, false, true, EPI_T, T>(P, p, st);
 }
 
-CER_API int cer_dense_fwd(const bf16_t* x, int64_t ldx, const bf16_t* w, int64_t ws,
-                          const bf16_t* b, int64_t bs, const bf16_t* r, int64_t ldr, bf16_t* y,
-                          void* d, int M, int N, int K, int G, int act, float* part,
-                          int64_t part_floats, hipStream_t st) {
-  return dense_fwd<bf16_t>(x, ldx, w, ws, b, bs, r, ldr, y, d, M, N, K, G, act, part, part_floats,
-                           st);
-}
-
-CER_API int cer_dense_fwd_f32(const float* x, int64_t ldx, const float* w, int64_t ws,
-                              const float* b, int64_t bs, const float* r, int64_t ldr, float* y,
-                              void* d, int M, int N, int K, int G, int act, float* part,
-                              int64_t part_floats, hipStream_t st) {
-  return dense_fwd<float>(x, ldx, w, ws, b, bs, r, ldr, y, d, M, N, K, G, act, part, part_floats,
-                          st);
-}
-
-CER_API int cer_dense_bwd(const bf16_t* dy, const void* d, void* dz, const bf16_t* x, int64_t ldx,
-                          const bf16_t* w, int64_t ws, bf16_t* dx, float* gw, int64_t gs, float* gb,
-                          int64_t gbs, int M, int N, int K, int G, int act, float* part,
-                          int64_t part_floats, hipStream_t st) {
-  return dense_bwd<bf16_t>(dy, d, dz, x, ldx, w, ws, dx, gw, gs, gb, gbs, M, N, K, G, act, part,
-                           part_floats, st);
-}
-
-CER_API int cer_dense_bwd_f32(const float* dy, const void* d, void* dz, const float* x, int64_t ldx,
-                              const float* w, int64_t ws, float* dx, float* gw, int64_t gs,
-                              float* gb, int64_t gbs, int M, int N, int K, int G, int act,
-                              float* part, int64_t part_floats, hipStream_t st) {
-  return dense_bwd<float>(dy, d, dz, x, ldx, w, ws, dx, gw, gs, gb, gbs, M, N, K, G, act, part,
-                          part_floats, st);
-}
+#define CER_DENSE(T, F, B)                                                                         \
+  CER_API CER_DENSE_FWD(F) {                                                                       \
+    return dense_fwd((const T*)x, ldx, (const T*)w, ws, (const T*)b, bs, (const T*)r, ldr, (T*)y,  \
+                     d, M, N, K, G, act, part, part_floats, st);                                   \
+  }                                                                                                \
+  CER_API CER_DENSE_BWD(B) {                                                                       \
+    return dense_bwd((const T*)dy, d, dz, (const T*)x, ldx, (const T*)w, ws, (T*)dx, gw, gs, gb,   \
+                     gbs, M, N, K, G, act, part, part_floats, st);                                 \
+  }
+CER_DENSE(bf16_t, cer_dense_fwd, cer_dense_bwd)
+CER_DENSE(float, cer_dense_fwd_f32, cer_dense_bwd_f32)

@@ -20,6 +20,7 @@
 // (distill_row); rows beyond what a block's registers hold are cut into slices
 // (distill_stats, distill_rows, distill_grad) and read twice.  All statistics
 // are fp32, the sums over the batch fp64 in a fixed order: no atomics.
+#include "nodes_api.h"
 #include "rowreg.h"
 
 constexpr float LOG2E = 1.4426950408889634f;
@@ -503,8 +504,6 @@ __global__ __launch_bounds__(TH) void distill_sum(const float* __restrict__ rowl
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-CER_API int64_t cer_distill_ws(int B, int G, int N, int is_bf16);
-
 template <typename T>
 static int64_t slice_of(int N) {
   // longest row of distill_row: 1024 threads x 16 vectors
@@ -611,33 +610,20 @@ CER_API int64_t cer_distill_ws(int B, int G, int N, int is_bf16) {
   return (int64_t)B * G * (2 + (sl ? 4 * ((N + sl - 1) / sl) : 0));
 }
 
-// loss [G], acc [G][4] +=, stats [G][B][4] for the backward; dz (or null): the
-// gradient for dloss = 1
-#define CER_DISTILL_FWD(NAME, T)                                                                  \
-  CER_API int NAME(const T* z, int64_t ldz, const int* labels, const void* val, int val_f32,      \
-                   int64_t val_gs, int64_t val_bs, const int* idx, int64_t idx_gs, int64_t idx_bs,                \
-                   const float* alpha, float alpha0, const float* tau, float tau0, float* stats,  \
-                   T* dz, float* loss,                                                            \
-                   float* acc, int B, int G, int N, int K, float* ws, int64_t ws_floats,          \
-                   hipStream_t st) {                                                              \
-    return dist_fwd<T>(dist_params(z, ldz, labels, val, val_f32, val_gs, val_bs, idx, idx_gs, idx_bs,      \
-                                   alpha, alpha0, tau, tau0, nullptr, stats, dz, B, G, N, K),                   \
-                       loss, acc, ws_floats, ws, st);                                             \
+// fwd: loss [G], acc [G][4] +=, stats [G][B][4] for the backward; dz (or null): the
+// gradient for dloss = 1.  bwd: dz from the forward's stats and dloss [G].
+#define CER_DISTILL(T, F, B_)                                                                      \
+  CER_API CER_DISTILL_FWD(F) {                                                                     \
+    return dist_fwd<T>(dist_params(z, ldz, labels, val, val_f32, val_gs, val_bs, idx, idx_gs,      \
+                                   idx_bs, alpha, alpha0, tau, tau0, nullptr, stats, dz, B, G, N,  \
+                                   K),                                                             \
+                       loss, acc, ws_floats, ws, st);                                              \
+  }                                                                                                \
+  CER_API CER_DISTILL_BWD(B_) {                                                                    \
+    const DistP P = dist_params(z, ldz, labels, val, val_f32, val_gs, val_bs, idx, idx_gs, idx_bs, \
+                                alpha, alpha0, tau, tau0, dloss, stats, dz, B, G, N, K);           \
+    if (!dist_ok<T>(P) || !stats || !dz || !dloss) return (int)hipErrorInvalidValue;               \
+    return launch_grad<T>(P, st);                                                                  \
   }
-CER_DISTILL_FWD(cer_distill_fwd, bf16_t)
-CER_DISTILL_FWD(cer_distill_fwd_f32, float)
-
-// dz from the forward's stats and dloss [G]
-#define CER_DISTILL_BWD(NAME, T)                                                                  \
-  CER_API int NAME(const T* z, int64_t ldz, const int* labels, const void* val, int val_f32,      \
-                   int64_t val_gs, int64_t val_bs, const int* idx, int64_t idx_gs, int64_t idx_bs,                \
-                   const float* alpha, float alpha0, const float* tau, float tau0,                \
-                   const float* dloss, float* stats, T* dz,                                       \
-                   int B, int G, int N, int K, hipStream_t st) {                                  \
-    DistP P = dist_params(z, ldz, labels, val, val_f32, val_gs, val_bs, idx, idx_gs, idx_bs, alpha, alpha0, \
-                          tau, tau0, dloss, stats, dz, B, G, N, K);                                          \
-    if (!dist_ok<T>(P) || !stats || !dz || !dloss) return (int)hipErrorInvalidValue;              \
-    return launch_grad<T>(P, st);                                                                 \
-  }
-CER_DISTILL_BWD(cer_distill_bwd, bf16_t)
-CER_DISTILL_BWD(cer_distill_bwd_f32, float)
+CER_DISTILL(bf16_t, cer_distill_fwd, cer_distill_bwd)
+CER_DISTILL(float, cer_distill_fwd_f32, cer_distill_bwd_f32)

@@ -18,6 +18,7 @@
 // registers, and long rows that are too few to fill the chip, are cut into
 // chunks; a chunk hands on its candidates unordered (or its K largest, if those
 // are too many) and top_merge selects among them in the same way.
+#include "nodes_api.h"
 #include "rowreg.h"
 
 constexpr int TOP_KMAX = 1024;
@@ -468,12 +469,10 @@ static int top_launch(const T* z, int64_t ldz, T* val, int* idx, int B, int G, i
   return (int)hipGetLastError();
 }
 
-CER_API int cer_top_logits(const bf16_t* z, int64_t ldz, bf16_t* val, int* idx, int B, int G, int N,
-                           int K, uint64_t* ws, int64_t ws_n, hipStream_t st) {
-  return top_launch<bf16_t>(z, ldz, val, idx, B, G, N, K, ws, ws_n, st);
+CER_API CER_TOP_LOGITS(cer_top_logits) {
+  return top_launch((const bf16_t*)z, ldz, (bf16_t*)val, idx, B, G, N, K, (uint64_t*)ws, ws_n, st);
 }
 
-CER_API int cer_top_logits_f32(const float* z, int64_t ldz, float* val, int* idx, int B, int G,
-                               int N, int K, uint64_t* ws, int64_t ws_n, hipStream_t st) {
-  return top_launch<float>(z, ldz, val, idx, B, G, N, K, ws, ws_n, st);
+CER_API CER_TOP_LOGITS(cer_top_logits_f32) {
+  return top_launch((const float*)z, ldz, (float*)val, idx, B, G, N, K, (uint64_t*)ws, ws_n, st);
 }

@@ -19,51 +19,14 @@
 #include <initializer_list>
 #include <optional>
 
+#include "../hip/nodes_api.h"
+
 using torch::Tensor;
 using torch::autograd::Node;
 using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
-// libcerebro_hip.so (csrc/hip/dense.hip, csrc/hip/distill.hip)
-extern "C" {
-#define DENSE_FWD(NAME)                                                                           \
-  int NAME(const void* x, int64_t ldx, const void* w, int64_t ws, const void* b, int64_t bs,      \
-           const void* r, int64_t ldr, void* y, void* d, int M, int N, int K, int G, int act,     \
-           float* part, int64_t part_floats, void* st);
-#define DENSE_BWD(NAME)                                                                           \
-  int NAME(const void* dy, const void* d, void* dz, const void* x, int64_t ldx, const void* w,    \
-           int64_t ws, void* dx, float* gw, int64_t gs, float* gb, int64_t gbs, int M, int N,     \
-           int K, int G, int act, float* part, int64_t part_floats, void* st);
-#define DISTILL_FWD(NAME)                                                                         \
-  int NAME(const void* z, int64_t ldz, const int* labels, const void* val, int val_f32,           \
-           int64_t val_gs, int64_t val_bs, const int* idx, int64_t idx_gs, int64_t idx_bs,        \
-           const float* alpha, float alpha0, const float* tau, float tau0, float* stats, void* dz, \
-           float* loss, float* acc, int B, int G, int N, int K, float* ws, int64_t ws_floats,     \
-           void* st);
-#define DISTILL_BWD(NAME)                                                                         \
-  int NAME(const void* z, int64_t ldz, const int* labels, const void* val, int val_f32,           \
-           int64_t val_gs, int64_t val_bs, const int* idx, int64_t idx_gs, int64_t idx_bs,        \
-           const float* alpha, float alpha0, const float* tau, float tau0, const float* dloss,    \
-           float* stats, void* dz, int B, int G, int N, int K, void* st);
-#define TOP_LOGITS(NAME)                                                                          \
-  int NAME(const void* z, int64_t ldz, void* val, int* idx, int B, int G, int N, int K,           \
-           int64_t* ws, int64_t ws_n, void* st);
-TOP_LOGITS(cer_top_logits)
-TOP_LOGITS(cer_top_logits_f32)
-int64_t cer_top_ws(int B, int G, int N, int K, int is_bf16);
-DENSE_FWD(cer_dense_fwd)
-DENSE_FWD(cer_dense_fwd_f32)
-DENSE_BWD(cer_dense_bwd)
-DENSE_BWD(cer_dense_bwd_f32)
-DISTILL_FWD(cer_distill_fwd)
-DISTILL_FWD(cer_distill_fwd_f32)
-DISTILL_BWD(cer_distill_bwd)
-DISTILL_BWD(cer_distill_bwd_f32)
-int64_t cer_dense_ws(int kind, int M, int N, int K, int G, int is_bf16, int act);
-int64_t cer_distill_ws(int B, int G, int N, int is_bf16);
-}
-
-static void* stream_of(const Tensor& t) {
+static hipStream_t stream_of(const Tensor& t) {
   return c10::hip::getCurrentHIPStream(t.device().index()).stream();
 }
 
