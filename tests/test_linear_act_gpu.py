@@ -544,3 +544,105 @@ def test_rows_beyond_a_grid_of_small_tiles():
     assert torch.equal(y.detach(), 2 * x.detach() + 0.5) and torch.equal(dx, 2 * dy)
     xs, ds = x.detach()[rows, 0].double(), dy[rows, 0].double()
     assert float(w.grad()) == float((xs * ds).sum()) and float(b.grad()) == float(ds.sum())
+
+
+@pytest.mark.parametrize("size", [(1, 4096, 64, 64), (2, 100, 64, 64), (1, 64, 64, 4096),
+                                  (1, 64, 4096, 64), (1, 7, 64, 64)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_fp32_products_have_three_planes(size):
+    """Products that sum 64 terms: 6 * 64 roundings of 2^-24 / sqrt(3) at most,
+    independent, are 6.7e-7 in the norm, the dropped products 6e-8; the bound is
+    2^-20.  Two planes would leave 2^-16 / sqrt(3) of each factor: 4.5e-6 was
+    measured with them."""
+    G, M, K, N = size
+    arena, w, b = make(G, N, K, bias=False, device=DEV)
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.randn(M, G * K, generator=gen, device=DEV, requires_grad=True)
+    dy = torch.randn(M, G * N, generator=gen, device=DEV)
+    y = P.linear_act(x, w, None, "none")
+    dx, = torch.autograd.grad(y, [x], dy)
+    for g in range(G):
+        xs, ds = x.detach()[:, g * K:(g + 1) * K].double(), dy[:, g * N:(g + 1) * N].double()
+        ws = w.work()[g].double()
+        for terms, got, want in ((K, y.detach()[:, g * N:(g + 1) * N], xs @ ws.t()),
+                                 (N, dx[:, g * K:(g + 1) * K], ds @ ws),
+                                 (M, w.grad()[g], ds.t() @ xs)):
+            if terms <= 64:
+                rel = float((got.double() - want).norm() / want.norm())
+                assert rel <= 2.0 ** -20, (terms, rel)
+
+
+@pytest.mark.parametrize("act", SMOOTH)
+def test_bf16_weight_gradient_has_three_planes(act):
+    """The same of dW = dz^T x where dz is the only factor that does not fit bf16;
+    z is exact, and act' off by 8 2^-24 (test_activations_in_fp32)."""
+    M, K, N = 64, 64, 1000
+    arena, w, b = make(1, N, K, torch.bfloat16, device=DEV)
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    w.master().copy_((w.master() * 16).round().clamp(-8, 8) / 16)
+    b.master().copy_((b.master() * 4).round() / 4)
+    arena.sync_work()
+    x = ((torch.randn(M, K, generator=gen, device=DEV) * 4).round().clamp(-8, 8) / 8).bfloat16()
+    x.requires_grad_(True)
+    dy = torch.randn(M, N, generator=gen, device=DEV).bfloat16()
+    torch.autograd.grad(P.linear_act(x, w, b, act), [x], dy)
+    z = (x.detach().double() @ w.work()[0].double().t() + b.work()[0].double()).requires_grad_(True)
+    dz, = torch.autograd.grad(ACT64[act](z), [z], dy.double())
+    want = dz.t() @ x.detach().double()
+    assert float((w.grad()[0].double() - want).norm() / want.norm()) <= 2.0 ** -20
+
+
+EXACT = [(1, 3, 8192, 130), (1, 8192, 40, 24), (1, 1, 4099, 30), (1, 2, 4099, 30), (1, 4, 4099, 30),
+         (1, 8, 4099, 30), (1, 9, 4099, 30), (1, 5, 1031, 1100), (16, 256, 1000, 500),
+         (1, 2047, 1027, 515), (2, 300, 1001, 333), (1, 33, 4608, 1000), (1, 4098, 101, 2050)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("act", ["none", "relu"])
+@pytest.mark.parametrize("size", EXACT, ids=lambda s: "x".join(map(str, s)))
+def test_sums_on_a_grid_are_exact(size, act, dtype):
+    """Multiples of 2^-7 that sum to at most 2^13 fit fp32 in any order: no term of
+    any reduction may be missing.  bf16 outputs are those sums rounded once."""
+    G, M, K, N = size
+    arena, w, b = make(G, N, K, dtype, device=DEV)
+    gen = torch.Generator(device=DEV).manual_seed(3)
+
+    def grid(*shape):
+        return torch.randint(-8, 9, shape, generator=gen, device=DEV).float() / 8
+    w.master().copy_(grid(G, N, K) / 2)
+    b.master().copy_(grid(G, N) + 1 / 16)
+    arena.sync_work()
+    x, r, dy = grid(M, G * K).to(dtype), grid(M, G * N).to(dtype), grid(M, G * N).to(dtype)
+    x.requires_grad_(True)
+    y = P.linear_act(x, w, b, act, r)
+    dx, = torch.autograd.grad(y, [x], dy)
+    for g in range(G):
+        xs, ds = x.detach()[:, g * K:(g + 1) * K].double(), dy[:, g * N:(g + 1) * N].double()
+        ws = w.work()[g].double()
+        z = xs @ ws.t() + b.work()[g].double()
+        a, dz = (z.clamp(min=0), ds * (z > 0)) if act == "relu" else (z, ds)
+        want = a + r[:, g * N:(g + 1) * N].double()
+        assert torch.equal(y.detach()[:, g * N:(g + 1) * N], want.float().to(dtype))
+        assert torch.equal(dx[:, g * K:(g + 1) * K], (dz @ ws).float().to(dtype))
+        assert torch.equal(w.grad()[g].double(), dz.t() @ xs)
+        assert torch.equal(b.grad()[g].double(), dz.sum(0))
+
+
+def test_weight_gradient_of_more_than_two_to_the_31_elements():
+    """Every row of 600 000 counts: halves that sum to at most 6e5, exactly."""
+    M, K, N = 600_000, 8, 4096
+    arena, w, b = make(1, N, K, torch.bfloat16, device=DEV)
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    x = (torch.randint(-2, 3, (M, K), generator=gen, device=DEV).float() / 2).bfloat16()
+    dy = torch.empty(M, N, dtype=torch.bfloat16, device=DEV)
+    dw, db = torch.zeros(N, K, dtype=torch.float64, device=DEV), torch.zeros(N, dtype=torch.float64,
+                                                                              device=DEV)
+    for i in range(0, M, 50_000):
+        d = torch.randint(-1, 2, (50_000, N), generator=gen, device=DEV).float()
+        dy[i:i + 50_000] = d.bfloat16()
+        dw += d.double().t() @ x[i:i + 50_000].double()
+        db += d.double().sum(0)
+    x.requires_grad_(True)
+    y = P.linear_act(x, w, b, "none")
+    torch.autograd.grad(y, [x], dy)
+    assert torch.equal(w.grad()[0].double(), dw) and torch.equal(b.grad()[0].double(), db)
