@@ -815,14 +815,23 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void dense_gemm(const GemmP P) {
 //   2048 x 1000 bf16    5.1 /  8.9   4.5 /  9.1   4.9 /  9.3   6.0 /  9.7
 //   8192 x 64 fp32      4.6 / 16.9   5.0 / 15.7   5.1 / 16.6   6.3 / 16.4
 //   100 x 8000 bf16     5.5 /  5.2   6.0 /  5.2   7.5 /  5.1  11.1 /  5.3
+//   100 x 60000 bf16   15.2 /  7.6  19.9 /  7.7
+//   104 x 8000 bf16     4.0 /  4.5   4.4 /  4.5
+//   300 x 8000 bf16     5.2 /  5.8   5.9 /  5.9
+//   301 x 60000 bf16   18.6 / 13.6  23.9 / 16.1
+//   516 x 60000 bf16   20.6 / 19.6  23.8 / 19.6
+//   1537 x 40000 bf16  24.6 / 32.5  28.8 / 37.8
+//   300 x 60000 fp32   15.2 / 28.3  17.4 / 28.2
 // With more rows the products on the vector units weigh more than the second
-// launch, the sooner the more weights there are: gemv_better.
+// launch, the sooner the more weights there are; and a short bf16 row that ends
+// inside a vector spends as long on its last elements as on all others, which many
+// columns cannot hide: gemv_better.
 // ---------------------------------------------------------------------------
 constexpr int GEMV_ROWS = 8;
 
 static inline bool gemv_better(int M, int N, int K, int G, int is_bf16) {
   const int64_t bytes = (int64_t)G * N * K * (is_bf16 ? 2 : 4);
-  if (M <= 2) return true;
+  if (M <= 2) return !is_bf16 || K % 8 == 0 || K >= 512 || (int64_t)G * N < 16000;
   if (M <= 4) return K >= 512 && (!is_bf16 || bytes <= (32 << 20));
   return M <= GEMV_ROWS && K >= 512 && bytes <= (8 << 20);
 }

@@ -646,3 +646,11 @@ def test_weight_gradient_of_more_than_two_to_the_31_elements():
     y = P.linear_act(x, w, b, "none")
     torch.autograd.grad(y, [x], dy)
     assert torch.equal(w.grad()[0].double(), dw) and torch.equal(b.grad()[0].double(), db)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("K,N", [(100, 15999), (100, 16000), (104, 16000), (511, 20001), (513, 20001)])
+@pytest.mark.parametrize("M", [1, 2])
+def test_few_rows_over_many_columns(M, K, N, dtype):
+    """Either side of the rule for short rows that end inside a vector."""
+    check(1, M, K, N, dtype, "silu", train=False)
