@@ -513,8 +513,17 @@ static int64_t slice_of(int N) {
 // Threads and vectors of the block for a row of N.  Few waves with long rows
 // rather than many with short ones: the row's reductions are barriers, and
 // blocks of 256 leave several of them on a CU (8192 x 16000 bf16: 512 x 8 253 us,
-// 256 x 8 150 us; 4096 x 30000: 512 x 8 186 us, 256 x 16 141 us; 4096 x 49999:
-// 512 x 16 251 us, 256 x 26 229 us).
+// 256 x 8 150 us; 4096 x 30000: 512 x 8 186 us, 256 x 16 141 us).  26 vectors are the
+// most that three such blocks can hold on a CU (166 of 168 registers a lane); with
+// more, two fit, and 512 threads are better.  us, unit gradient, 4096 rows of
+//   bf16:     33000  40000  49999  53000  54000  60000  65536
+//   256 x 26    152    167    202    211
+//   512 x 16    179    197    231    231    237    251    261
+//   256 x 32    184    205    241    245    250    268    281
+//   fp32:     16500  20000  24999  26500  27000  30000  32768
+//   256 x 26    136    156    190    198
+//   512 x 16    152    167    197    203    208    225    233
+//   256 x 32    153    172    205    212    217    230    241
 #define CER_ROW_DISPATCH(T, N, LAUNCH)                  \
   do {                                                  \
     constexpr int V_ = 16 / sizeof(T);                  \
