@@ -66,19 +66,38 @@ static float* fptr(const Tensor& t) { return t.defined() ? t.data_ptr<float>() :
 
 // All that a backward reads goes through SavedVariable: hooks on saved tensors
 // (offload, checkpoints) see it, and an input that was written in between is
-// refused.  An inference tensor counts no writes; it is copied.
-static SavedVariable saved(const Tensor& t) {
-  return SavedVariable(t.defined() && t.is_inference() ? t.clone() : t, false);
-}
+// refused.  An inference tensor counts no writes; it is copied.  What a hook gives
+// back is read by kernels: other sizes, types or devices are refused, another layout
+// is copied (elements of a row adjacent, a matrix's pitch at least its width).
+class Saved {
+  SavedVariable v_;
+  at::ScalarType type_ = at::kFloat;
+  at::DimVector sizes_;
 
-// What a hook gives back has the values but not always the layout: elements of a
-// row adjacent, and for a matrix a pitch of at least its width.
-static Tensor adjacent(const Tensor& t) {
-  const int64_t last = t.dim() - 1;
-  const bool is = (t.size(last) <= 1 || t.stride(last) == 1) &&
-                  (t.dim() != 2 || t.stride(0) >= t.size(1));
-  return is ? t : t.clone(at::MemoryFormat::Contiguous);
-}
+ public:
+  Saved() = default;
+  explicit Saved(const Tensor& t)
+      : v_(t.defined() && t.is_inference() ? t.clone() : t, false) {
+    if (!t.defined()) return;
+    type_ = t.scalar_type();
+    sizes_ = t.sizes();
+  }
+
+  Tensor unpack(const c10::Device& device) const {
+    const Tensor t = v_.unpack();
+    if (!t.defined()) return t;
+    TORCH_CHECK(t.scalar_type() == type_ && t.sizes() == sizes_ && t.device() == device &&
+                    t.layout() == at::kStrided,
+                "a hook on saved tensors gave back ", t.scalar_type(), " ", t.sizes(), " on ",
+                t.device(), " for ", type_, " ", at::IntArrayRef(sizes_), " on ", device);
+    const int64_t last = t.dim() - 1;
+    const bool adjacent = last < 0 || ((t.size(last) <= 1 || t.stride(last) == 1) &&
+                                       (last != 1 || t.stride(0) >= t.size(1)));
+    return adjacent ? t : t.clone(at::MemoryFormat::Contiguous);
+  }
+
+  void free() { v_.reset_data(); }
+};
 
 // ---------------------------------------------------------------------------
 struct Dense {
@@ -94,15 +113,15 @@ struct Dense {
 
 struct LinearActBackward : public Node {
   Dense p;
-  SavedVariable x, derivative;  // act'(z)
+  Saved x, derivative;          // act'(z)
 
   variable_list apply(variable_list&& grads) override {
     variable_list out(3);
     const Tensor g0 = grads[0];
     if (!g0.defined()) return out;
     once("linear_act");
-    const Tensor xv = adjacent(x.unpack());
-    Tensor d = derivative.unpack();
+    const Tensor xv = x.unpack(p.work.device());
+    Tensor d = derivative.unpack(p.work.device());
     if (d.defined()) d = d.contiguous();
     const c10::OptionalDeviceGuard guard(xv.device());
     const Tensor dy = g0.contiguous();
@@ -124,8 +143,8 @@ struct LinearActBackward : public Node {
   }
 
   void release_variables() override {
-    x.reset_data();
-    derivative.reset_data();
+    x.free();
+    derivative.free();
   }
 };
 
@@ -162,8 +181,8 @@ static Tensor linear_act(const Tensor& x, const std::optional<Tensor>& anchor,
     node->set_next_edges(torch::autograd::collect_next_edges(x, anchor.value_or(Tensor()),
                                                              residual.value_or(Tensor())));
     node->p = std::move(p);
-    node->x = SavedVariable(x, false);
-    node->derivative = saved(d);
+    node->x = Saved(x);
+    node->derivative = Saved(d);
     torch::autograd::set_history(y, node);
   }
   return y;
@@ -177,17 +196,17 @@ struct Teacher {
 
 // read again in the backward, beside sums that the forward made of them
 struct SavedTeacher {
-  SavedVariable labels, val, idx, alpha, tau;
+  Saved labels, val, idx, alpha, tau;
   double alpha0 = 0, tau0 = 0;
 
   SavedTeacher() = default;
   explicit SavedTeacher(const Teacher& t)
-      : labels(saved(t.labels)), val(saved(t.val)), idx(saved(t.idx)), alpha(saved(t.alpha)),
-        tau(saved(t.tau)), alpha0(t.alpha0), tau0(t.tau0) {}
+      : labels(t.labels), val(t.val), idx(t.idx), alpha(t.alpha), tau(t.tau), alpha0(t.alpha0),
+        tau0(t.tau0) {}
 
-  Teacher unpack() const {
-    Teacher t{labels.unpack().contiguous(), adjacent(val.unpack()), adjacent(idx.unpack()),
-              alpha.unpack(), tau.unpack(), alpha0, tau0};
+  Teacher unpack(const c10::Device& device) const {
+    Teacher t{labels.unpack(device).contiguous(), val.unpack(device), idx.unpack(device),
+              alpha.unpack(device), tau.unpack(device), alpha0, tau0};
     if (t.alpha.defined()) t.alpha = t.alpha.contiguous();
     if (t.tau.defined()) t.tau = t.tau.contiguous();
     return t;
@@ -196,8 +215,9 @@ struct SavedTeacher {
 
 struct DistillBackward : public Node {
   SavedTeacher teacher;
-  SavedVariable z, stats;
-  SavedVariable finished;       // the gradient for a unit loss gradient
+  Saved z, stats;
+  Saved finished;               // the gradient for a unit loss gradient
+  c10::Device device = c10::kCUDA;
   int64_t G;
   bool unit;
 
@@ -206,14 +226,14 @@ struct DistillBackward : public Node {
     if (!grads[0].defined()) return out;
     once("distill_ce");
     if (unit) {
-      const Tensor d = finished.unpack();
+      const Tensor d = finished.unpack(device);
       // a graph that is kept may be run again: the caller may write its gradient
       out[0] = torch::autograd::get_current_graph_task_keep_graph() ? d.clone() : d;
       return out;
     }
-    const Tensor zv = adjacent(z.unpack());
-    const Tensor sums = stats.unpack().contiguous();
-    const Teacher t = teacher.unpack();
+    const Tensor zv = z.unpack(device);
+    const Tensor sums = stats.unpack(device).contiguous();
+    const Teacher t = teacher.unpack(device);
     const c10::OptionalDeviceGuard guard(zv.device());
     const Tensor dloss = grads[0].contiguous();
     const bool bf16 = zv.scalar_type() == at::kBFloat16;
@@ -229,9 +249,9 @@ struct DistillBackward : public Node {
   }
 
   void release_variables() override {
-    z.reset_data();
-    stats.reset_data();
-    finished.reset_data();
+    z.free();
+    stats.free();
+    finished.free();
     teacher = SavedTeacher();
   }
 };
@@ -265,12 +285,13 @@ static Tensor distill_ce(const Tensor& z, const Tensor& labels, const Tensor& ac
     node->set_next_edges(torch::autograd::collect_next_edges(z));
     node->G = G;
     node->unit = unit;
+    node->device = z.device();
     if (unit) {
-      node->finished = saved(d);
+      node->finished = Saved(d);
     } else {
-      node->z = SavedVariable(z, false);
+      node->z = Saved(z);
       node->teacher = SavedTeacher(t);
-      node->stats = saved(buf.narrow(0, 0, 4 * G * B));
+      node->stats = Saved(buf.narrow(0, 0, 4 * G * B));
     }
     torch::autograd::set_history(loss, node);
   }

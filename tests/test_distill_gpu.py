@@ -673,3 +673,17 @@ def test_fp32_gradient_is_as_near_as_its_exponentials(B, N, unit):
     rest.scatter_(1, lab[0].long()[:, None], False).scatter_(1, idx[0].long(), False)
     err = (d.double() - want)[rest]
     assert float(err.norm() / want[rest].norm()) <= 2.0 ** -23
+
+
+def test_hooks_that_give_back_something_else_are_refused():
+    from torch.autograd.graph import saved_tensors_hooks
+    z, lab, val, idx, alpha, tau = inputs(2, 6, 30, 4, device=DEV)
+    x = z.clone().requires_grad_(True)
+    for unit, shapes in ((True, [(6, 60)]), (False, [(6, 60), (2, 6), (2, 6, 4), (2,), (48,)])):
+        for wrong in (lambda t: t.double(), lambda t: t.cpu(), lambda t: t[:1], lambda t: t[None]):
+            for shape in shapes:
+                with saved_tensors_hooks(lambda t: t, lambda t: wrong(t) if t.shape == shape else t):
+                    loss = L.distill_ce(x, lab, torch.zeros(2, 4, device=DEV), 2, val, idx, alpha, tau,
+                                        unit=unit)
+                with pytest.raises(RuntimeError, match="a hook on saved tensors"):
+                    torch.autograd.grad(loss, [x], torch.ones(2, device=DEV))

@@ -654,3 +654,31 @@ def test_weight_gradient_of_more_than_two_to_the_31_elements():
 def test_few_rows_over_many_columns(M, K, N, dtype):
     """Either side of the rule for short rows that end inside a vector."""
     check(1, M, K, N, dtype, "silu", train=False)
+
+
+def test_hooks_that_give_back_something_else_are_refused():
+    """Kernels read what a hook returns: its sizes, type and device are checked."""
+    from torch.autograd.graph import saved_tensors_hooks
+    arena, w, b = make(1, 12, 10, device=DEV)
+    x = torch.randn(7, 10, device=DEV, requires_grad=True)
+    for wrong in (lambda t: t.bfloat16(), lambda t: t.cpu(), lambda t: t[:3], lambda t: t.flatten()):
+        for shape in ((7, 10), (7, 12)):            # x, act'(z)
+            with saved_tensors_hooks(lambda t: t, lambda t: wrong(t) if t.shape == shape else t):
+                y = P.linear_act(x, w, b, "gelu")
+            with pytest.raises(RuntimeError, match="a hook on saved tensors"):
+                torch.autograd.grad(y.sum(), [x])
+
+
+def test_input_made_in_inference_mode():
+    """A frozen extractor's output in front of a trained head."""
+    arena, w, b = make(1, 12, 10, device=DEV)
+    anchor = torch.zeros((), device=DEV, requires_grad=True)
+    with torch.inference_mode():
+        x = torch.randn(7, 10, device=DEV)
+    P.linear_act(x.clone(), w, b, "gelu", anchor=anchor).sum().backward()
+    want = w.grad().clone()
+    y = P.linear_act(x, w, b, "gelu", anchor=anchor)
+    with torch.inference_mode():
+        x.zero_()
+    y.sum().backward()
+    assert torch.equal(w.grad(), want)
