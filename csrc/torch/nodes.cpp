@@ -157,6 +157,9 @@ static Tensor linear_act(const Tensor& x, const std::optional<Tensor>& anchor,
   eager_and_reverse("linear_act",
                     {&x, anchor ? &*anchor : &x, residual ? &*residual : &x, &work});
   ints("linear_act", {x.size(0), x.size(1), work.size(0) * N});
+  // statistics live behind the parameters and have no gradient
+  TORCH_CHECK_VALUE(w_off >= 0 && w_off + N * K <= work.size(1) && b_off + N <= work.size(1),
+                    "linear_act: the weight or bias is no trainable parameter of its arena");
   const c10::OptionalDeviceGuard guard(x.device());
   Dense p{work, grad.value_or(Tensor()), w_off, b_off, x.size(0), N, K, work.size(0), act,
           x.scalar_type() == at::kBFloat16};

@@ -170,3 +170,20 @@ def test_no_second_derivative_on_the_cpu():
     with pytest.raises(RuntimeError, match="second derivative"):
         d, = torch.autograd.grad((y * y).sum(), [x], create_graph=True)
         torch.autograd.grad(d.sum(), [x])
+
+
+def test_statistics_and_parameters_of_other_layouts_are_refused():
+    """A running mean lies behind the parameters, where the gradients have
+    nothing: its gradient would be written past their end."""
+    from cerebro_ds_kpgi_amd.ops import _hip
+    spec = [ParamSpec("d/kernel", (3, 5), "weight"), ParamSpec("bn/mean", (3,), "running_mean")]
+    arena = Arena(ModelLayout(spec), 2, "cpu", torch.float32)
+    big = ModelLayout([ParamSpec("a", (300, 5), "weight"), ParamSpec("b", (3,), "bias")]).specs[1]
+    w = ParamRef(arena, spec[0])
+    x = torch.randn(4, 10)
+    for other in (spec[1], big):
+        with pytest.raises(ValueError, match="no trainable parameter"):
+            _hip.nodes().linear_act(x, None, None, arena.work, arena.grad, spec[0].offset,
+                                    other.offset, 3, 5, 0, True)
+        with pytest.raises((ValueError, RuntimeError)):
+            P.linear_act(x, w, ParamRef(arena, other))
