@@ -257,7 +257,10 @@ def distill_ce(logits, labels, acc, G, top_val, top_idx, alpha=0.5, tau=1.0, uni
     ``softmax_ce``; unlabelled rows are no hits (with N == 2 every row is a top-5
     hit).  Gradient in ``logits`` only.  ``unit=True``: the caller
     back-propagates a gradient of ones, and the forward writes the gradient in
-    the same pass over the logits.  (Capturing a backward: see ``nn.linear_act``.)
+    the same pass over the logits.  Otherwise the backward reads logits, labels,
+    entries, alpha and tau again: one that was written in between is refused.  No
+    second or forward-mode derivatives, no tracing.  (Capturing a backward: see
+    ``nn.linear_act``.)
     """
     z, N = _logit_rows("distill_ce", logits, G)
     B, dev = z.shape[0], z.device

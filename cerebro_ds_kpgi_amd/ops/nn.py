@@ -817,7 +817,7 @@ def linear_act(x, wref, bref=None, act="none", residual=None, anchor=None):
     """y = residual + act(x W^T + b), config by config, in one GEMM.
 
     ``x [..., G*K]`` and ``residual [..., G*N]`` in the arena's compute dtype
-    (fp32 or bf16), any number of rows, ``wref`` a ``[N, K]`` and ``bref`` a
+    (fp32 or bf16), up to 2^31 - 2^20 rows, ``wref`` a ``[N, K]`` and ``bref`` a
     ``[N]`` parameter of the same arena; ``act`` one of ``LINEAR_ACTS`` (gelu
     is the erf form).  Differentiable in ``x`` and ``residual``; with either of
     them, or ``anchor``, requiring a gradient the backward writes the weight and
@@ -825,7 +825,14 @@ def linear_act(x, wref, bref=None, act="none", residual=None, anchor=None):
     it does not add, so a parameter is used once per step.  Rounding: fp32
     products run on three bf16 planes per factor (as near to the exact sum as
     fp32 products), bf16 products are exact with fp32 sums, and every output is rounded
-    once; act'(z) is kept in fp32 between the passes.
+    once; act'(z) is kept in fp32 between the passes, and dy act'(z) of a bf16 layer
+    enters dW with 24 bits and dx with 16.
+
+    The backward reads x again (written in between, it is refused) and the weights,
+    which must not change before it.  No second or forward-mode derivatives, no
+    tracing.  Before a backward is captured into a HIP graph, drop the outputs of
+    eager passes over the same leaves: torch ties a leaf's gradient node to the
+    stream of the oldest live pass.
     """
     code = LINEAR_ACTS.get(act)
     arena = wref.arena

@@ -723,7 +723,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void dense_gemm(const GemmP P) {
   // code (activation, residual) short.  A turn's residual is requested a turn
   // ahead and waits in LDS: loads in the loop, which stay behind its stores, would
   // be waited for one by one (bf16 8192 x 4096 x 4096 with gelu and act': 384 -> 355
-  // us).
+  // us; 376 us since gelu is exact to fp32).
   constexpr int WC = BN / WN, PITCH = WC + 4, ER = IM < 2 ? 1 : 2;
   constexpr int LC = WC / 4, RS = 64 / LC, SN = 16 * ER / RS;   // lanes a row, rows a step, steps
   static_assert(IM % ER == 0, "rows of a turn");
